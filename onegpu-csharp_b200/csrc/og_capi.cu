@@ -190,7 +190,9 @@ struct og_int8_gemm {
     int stream_k = 0;  // 0: whole tiles + the split tail of int32 products; 1: whole tiles only; 2: stream-K
     std::string variant;
     std::string last = "none";
-    std::vector<void*> scratch;  // int32 byte-sum buffers; older ones live until destroy (recorded work may name them)
+    // Device buffers freed with the instance: byte sums and staged operands, older ones too (recorded work may name them)
+    std::vector<void*> scratch;
+    int32_t* sums = nullptr;  // the latest byte-sum buffer, scratch_elements int32
     int64_t scratch_elements = 0;
     void* sk_buf = nullptr;      // stream-K hand-over buffer of the tensor-core product, allocated on first need
     int64_t sk_bytes = 0;
@@ -483,13 +485,14 @@ og::GemmLaunch make_launch(og_int8_gemm* g, const og_int8_gemm_problem* p, const
 
 // Returns device memory for `elements` int32 byte sums from the instance's scratch, growing it geometrically.
 int32_t* own_scratch(og_int8_gemm* g, int64_t elements) {
-    if (!g->scratch.empty() && g->scratch_elements >= elements) return static_cast<int32_t*>(g->scratch.back());
-    int64_t len = std::max<int64_t>(elements, g->scratch.empty() ? 4096 : g->scratch_elements * 2);
+    if (g->sums != nullptr && g->scratch_elements >= elements) return g->sums;
+    int64_t len = std::max<int64_t>(elements, g->sums == nullptr ? 4096 : g->scratch_elements * 2);
     void* p = nullptr;
     check_cuda(cudaMalloc(&p, static_cast<size_t>(len) * sizeof(int32_t)), "Int8Gemm scratch");
     g->scratch.push_back(p);
+    g->sums = static_cast<int32_t*>(p);
     g->scratch_elements = len;
-    return static_cast<int32_t*>(p);
+    return g->sums;
 }
 
 // Chooses the kernel and records the product (and, for the tensor-core path with zero points, the byte sums).
@@ -1166,7 +1169,7 @@ OG_API og_status og_int8_gemm_reserve_scratch(og_int8_gemm* g, int64_t elements)
         if (elements < 0 || elements > kMaxElements)
             throw OgError{OG_ERROR_ARGUMENT_RANGE, kGemm, "elements",
                           "must be between 0 and " + std::to_string(kMaxElements), "", "", ""};
-        if (elements == 0 || (!g->scratch.empty() && g->scratch_elements >= elements)) return;
+        if (elements == 0 || (g->sums != nullptr && g->scratch_elements >= elements)) return;
         use(g->device);
         own_scratch(g, std::max<int64_t>(elements, 4096));
     });
