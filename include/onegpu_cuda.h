@@ -261,6 +261,36 @@ OG_API og_status og_int8_gemm_encode_dequantize(og_int8_gemm* gemm, og_encoder* 
                                                 const og_operand* b_scale, const og_operand* zero_point_a,
                                                 const og_operand* zero_point_b, const og_operand* float_bias,
                                                 const og_operand* int_bias);
+/* What the epilogue of the activated product and the mixture-of-experts layer apply to a value v. */
+typedef enum og_activation {
+    OG_ACTIVATION_NONE = 0,      /* v */
+    OG_ACTIVATION_RELU = 1,      /* max(v, 0); NaN stays NaN */
+    OG_ACTIVATION_GELU = 2,      /* v / 2 * (1 + erf(v / sqrt 2)) */
+    OG_ACTIVATION_GELU_TANH = 3, /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
+    OG_ACTIVATION_SILU = 4       /* v / (1 + exp(-v)) */
+} og_activation;
+
+/* The product of a layer with 8-bit weights, finished in its epilogue. No counterpart in the reference.
+ *   c[b, m, n] = activation(float(sum + intBias[n]) * (aScale[m] * bScale[n]) + floatBias[n]) + residual[b, m, n]
+ * sum is the exact int32 sum of EncodeInt32; the scale product, the scaling, the bias and the residual are one float32
+ * rounding each. c is float32 or float16 (rounded once, at the end). a_scale holds one value, or one per row (the same
+ * for every batch, like zero_point_a: what og_dynamic_quantize_encode_rows writes); b_scale one value or one per column.
+ * zero_point_a, zero_point_b, float_bias, int_bias and residual may be NULL. The residual has c's type, is dense like c,
+ * starts at its operand's offset, and may be c itself (the same elements); a partial overlap is refused. */
+OG_API og_status og_int8_gemm_encode_activated(og_int8_gemm* gemm, og_encoder* encoder,
+                                               const og_int8_gemm_problem* problem, const og_buffer* a,
+                                               const og_buffer* b, const og_buffer* c, const og_operand* a_scale,
+                                               const og_operand* b_scale, const og_operand* zero_point_a,
+                                               const og_operand* zero_point_b, const og_operand* float_bias,
+                                               const og_operand* int_bias, int32_t activation,
+                                               const og_operand* residual);
+/* Its argument checks alone (no device needed): EncodeFloat's order and names, then "activation" and "residual". */
+OG_API og_status og_int8_gemm_check_activated(const og_int8_gemm_problem* problem, const og_buffer* a,
+                                              const og_buffer* b, const og_buffer* c, const og_operand* a_scale,
+                                              const og_operand* b_scale, const og_operand* zero_point_a,
+                                              const og_operand* zero_point_b, const og_operand* float_bias,
+                                              const og_operand* int_bias, int32_t activation,
+                                              const og_operand* residual);
 /* Int8Gemm.EncodeRequantized<TA,TB,TY> (Int8Gemm.cs:336-363). scratch (Int8Scratch, Int8Gemm.cs:37) may be NULL; its
  * buffer is an int32 buffer and its offset an element offset. */
 OG_API og_status og_int8_gemm_encode_requantized(og_int8_gemm* gemm, og_encoder* encoder,
@@ -336,6 +366,20 @@ OG_API og_status og_dynamic_quantize_encode(og_dynamic_quantize* dq, og_encoder*
 OG_API og_status og_dynamic_quantize_check(const og_buffer* x, int32_t offset_x, int32_t count, const og_buffer* y,
                                            int32_t offset_y, const og_buffer* scale, int32_t offset_scale,
                                            const og_buffer* zero_point, int32_t offset_zero_point);
+/* DynamicQuantizeLinear of every row (token) of a rows x columns tensor on its own. No counterpart in the reference.
+ * x is float32 or float16, its rows row_stride_x elements apart (0: dense); y uint8, dense; scale float32 and
+ * zero_point uint8, one per row. Each row has the bits of og_dynamic_quantize_encode on it alone (a float16 row as its
+ * float32 values). rows may be 0. */
+OG_API og_status og_dynamic_quantize_encode_rows(og_dynamic_quantize* dq, og_encoder* encoder, const og_buffer* x,
+                                                 int32_t offset_x, int32_t rows, int32_t columns, int32_t row_stride_x,
+                                                 const og_buffer* y, int32_t offset_y, const og_buffer* scale,
+                                                 int32_t offset_scale, const og_buffer* zero_point,
+                                                 int32_t offset_zero_point);
+/* Its argument checks alone (no device needed). */
+OG_API og_status og_dynamic_quantize_check_rows(const og_buffer* x, int32_t offset_x, int32_t rows, int32_t columns,
+                                                int32_t row_stride_x, const og_buffer* y, int32_t offset_y,
+                                                const og_buffer* scale, int32_t offset_scale,
+                                                const og_buffer* zero_point, int32_t offset_zero_point);
 
 /* ---- DequantizeKernels (src/RecursiveAI.OneGpu.Kernels/DequantizeKernels.cs:29-298) ------------------------------ */
 

@@ -59,6 +59,9 @@ public struct Int8GemmProblem
 /// IsVector, one per row of A (its zero point) or per column (zero point of B, scale, bias).</summary>
 public readonly record struct Int8Operand<T>(GpuBuffer<T> Buffer, int Offset, bool IsVector = false) where T : unmanaged;
 
+/// <summary>What an epilogue applies to its values (og_activation). No counterpart in the reference.</summary>
+public enum Int8Activation { None = 0, Relu = 1, Gelu = 2, GeluTanh = 3, Silu = 4 }
+
 /// <summary>Int8Scratch (Int8Gemm.cs:37): caller-placed int32 scratch of EncodeRequantized.</summary>
 public readonly record struct Int8Scratch(GpuBuffer<int> Buffer, int Offset = 0);
 
@@ -217,6 +220,34 @@ public sealed unsafe class Int8Gemm : IDisposable
                                                                       intBias is null ? null : &ib));
     }
 
+    /// <summary>activation(float(sum + intBias) * (aScale[m] * bScale[n]) + floatBias[n]) + residual[m, n], float or
+    /// Half results: aScale holds one value or one per row (DynamicQuantizeKernels.EncodeRows), the residual has c's
+    /// type and layout and may be c itself. No counterpart in the reference's shipped API.</summary>
+    public void EncodeActivated<TA, TB, TC>(GpuCommandEncoder encoder, in Int8GemmProblem problem, GpuBuffer<TA> a,
+                                            GpuBuffer<TB> b, GpuBuffer<TC> c, Int8Operand<float> aScale,
+                                            Int8Operand<float> bScale, Int8Operand<TA>? zeroPointA = null,
+                                            Int8Operand<TB>? zeroPointB = null, Int8Operand<float>? floatBias = null,
+                                            Int8Operand<int>? intBias = null,
+                                            Int8Activation activation = Int8Activation.None,
+                                            Int8Operand<TC>? residual = null)
+        where TA : unmanaged
+        where TB : unmanaged
+        where TC : unmanaged
+    {
+        var p = problem.Native();
+        OgBuffer va = NativeCheck.View(a), vb = NativeCheck.View(b), vc = NativeCheck.View(c);
+        OgOperand sa = NativeCheck.Operand<float>(aScale), sb = NativeCheck.Operand<float>(bScale);
+        OgOperand za = NativeCheck.Operand(zeroPointA), zb = NativeCheck.Operand(zeroPointB);
+        OgOperand fb = NativeCheck.Operand(floatBias), ib = NativeCheck.Operand(intBias);
+        OgOperand rs = NativeCheck.Operand(residual);
+        NativeCheck.Check(Cuda.Native.og_int8_gemm_encode_activated(Handle, Encoder(encoder), &p, &va, &vb, &vc, &sa, &sb,
+                                                                    zeroPointA is null ? null : &za,
+                                                                    zeroPointB is null ? null : &zb,
+                                                                    floatBias is null ? null : &fb,
+                                                                    intBias is null ? null : &ib, (int)activation,
+                                                                    residual is null ? null : &rs));
+    }
+
     /// <summary>Waits for the device, then releases the instance's scratch (Int8Gemm.cs:378-391).</summary>
     public void Dispose()
     {
@@ -265,6 +296,25 @@ public sealed unsafe class DynamicQuantizeKernels : IDisposable
                                                                  y is null ? null : &vy, offsetY,
                                                                  scale is null ? null : &vs, offsetScale,
                                                                  zeroPoint is null ? null : &vz, offsetZeroPoint));
+    }
+
+    /// <summary>DynamicQuantizeLinear of every row (token) on its own: x float or Half, rows rowStrideX elements apart
+    /// (0: dense), one scale and zero point per row. No counterpart in the reference's shipped API.</summary>
+    public void EncodeRows<T>(GpuCommandEncoder encoder, GpuBuffer<T> x, int offsetX, int rows, int columns,
+                              int rowStrideX, GpuBuffer<byte> y, int offsetY, GpuBuffer<float> scale, int offsetScale,
+                              GpuBuffer<byte> zeroPoint, int offsetZeroPoint)
+        where T : unmanaged
+    {
+        ArgumentNullException.ThrowIfNull(encoder);
+        var enc = encoder as CudaCommandEncoder
+                  ?? throw new GpuUnsupportedException("the encoder belongs to another backend", "Backend", "CUDA", null);
+        OgBuffer vx = NativeCheck.View(x), vy = NativeCheck.View(y), vs = NativeCheck.View(scale);
+        OgBuffer vz = NativeCheck.View(zeroPoint);
+        NativeCheck.Check(Cuda.Native.og_dynamic_quantize_encode_rows(Handle, enc.Handle, x is null ? null : &vx, offsetX,
+                                                                      rows, columns, rowStrideX,
+                                                                      y is null ? null : &vy, offsetY,
+                                                                      scale is null ? null : &vs, offsetScale,
+                                                                      zeroPoint is null ? null : &vz, offsetZeroPoint));
     }
 
     public void Dispose()

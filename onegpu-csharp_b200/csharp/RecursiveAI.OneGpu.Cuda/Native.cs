@@ -105,6 +105,9 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int og_int8_gemm_encode_dequantize(nint gemm, nint encoder,
         OgProblem* p, OgBuffer* a, OgBuffer* b, OgBuffer* c, OgOperand* aScale, OgOperand* bScale, OgOperand* zpA,
         OgOperand* zpB, OgOperand* floatBias, OgOperand* intBias);
+    [LibraryImport(Lib)] internal static partial int og_int8_gemm_encode_activated(nint gemm, nint encoder,
+        OgProblem* p, OgBuffer* a, OgBuffer* b, OgBuffer* c, OgOperand* aScale, OgOperand* bScale, OgOperand* zpA,
+        OgOperand* zpB, OgOperand* floatBias, OgOperand* intBias, int activation, OgOperand* residual);
     // EncodeInt32 queued straight onto a stream, using only memory the library reserved when it was loaded.
     [LibraryImport(Lib)] internal static partial int og_int8_gemm_int32_noalloc(nint stream, OgProblem* p,
         OgBuffer* a, OgBuffer* b, OgBuffer* c, OgOperand* zpA, OgOperand* zpB, OgOperand* bias);
@@ -119,6 +122,9 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int og_int8_gemm_check_dequantize(OgProblem* p, OgBuffer* a,
         OgBuffer* b, OgBuffer* c, OgOperand* aScale, OgOperand* bScale, OgOperand* zpA, OgOperand* zpB,
         OgOperand* floatBias, OgOperand* intBias);
+    [LibraryImport(Lib)] internal static partial int og_int8_gemm_check_activated(OgProblem* p, OgBuffer* a,
+        OgBuffer* b, OgBuffer* c, OgOperand* aScale, OgOperand* bScale, OgOperand* zpA, OgOperand* zpB,
+        OgOperand* floatBias, OgOperand* intBias, int activation, OgOperand* residual);
     [LibraryImport(Lib)] internal static partial int og_int8_gemm_check_requantized(OgProblem* p, OgBuffer* a,
         OgBuffer* b, OgBuffer* y, OgOperand* multiplier, int zeroPointY, OgOperand* zpA, OgOperand* zpB,
         OgOperand* intBias, OgOperand* scratch);
@@ -130,6 +136,12 @@ internal static unsafe partial class Native
         int offsetZeroPoint);
     [LibraryImport(Lib)] internal static partial int og_dynamic_quantize_check(OgBuffer* x, int offsetX, int count,
         OgBuffer* y, int offsetY, OgBuffer* scale, int offsetScale, OgBuffer* zeroPoint, int offsetZeroPoint);
+    [LibraryImport(Lib)] internal static partial int og_dynamic_quantize_encode_rows(nint dq, nint encoder,
+        OgBuffer* x, int offsetX, int rows, int columns, int rowStrideX, OgBuffer* y, int offsetY, OgBuffer* scale,
+        int offsetScale, OgBuffer* zeroPoint, int offsetZeroPoint);
+    [LibraryImport(Lib)] internal static partial int og_dynamic_quantize_check_rows(OgBuffer* x, int offsetX, int rows,
+        int columns, int rowStrideX, OgBuffer* y, int offsetY, OgBuffer* scale, int offsetScale, OgBuffer* zeroPoint,
+        int offsetZeroPoint);
 
     [LibraryImport(Lib)] internal static partial int og_dequantize_create(nint device, nint* kernels);
     [LibraryImport(Lib)] internal static partial int og_dequantize_destroy(nint kernels);

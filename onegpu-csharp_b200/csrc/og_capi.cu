@@ -416,6 +416,80 @@ Prepared check_requantized(const og_int8_gemm_problem* p, const og_buffer* a, co
     return pr;
 }
 
+// Whether `extent` elements of two typed buffers from their offsets share memory without being the same elements.
+bool overlaps_shifted(const og_buffer* a, int64_t offset_a, const og_buffer* b, int64_t offset_b, int64_t extent) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a->ptr) + offset_a * elem_size(a->type);
+    const uintptr_t b0 = reinterpret_cast<uintptr_t>(b->ptr) + offset_b * elem_size(b->type);
+    return a0 != b0 && a0 < b0 + extent * elem_size(b->type) && b0 < a0 + extent * elem_size(a->type);
+}
+
+// The activated form: the dequantize form's operands with aScale one value or one per row, results float or half, an
+// activation, and a residual of the result's type and layout (the result itself, or elsewhere).
+Prepared check_activated(const og_int8_gemm_problem* p, const og_buffer* a, const og_buffer* b, const og_buffer* c,
+                         const og_operand* a_scale, const og_operand* b_scale, const og_operand* za,
+                         const og_operand* zb, const og_operand* fbias, const og_operand* ibias, int32_t activation,
+                         const og_operand* residual) {
+    if (c == nullptr || c->ptr == nullptr) null_arg(kGemm, "c");
+    Prepared pr = prepare(p, a, b, za, zb);
+    if (c->type != OG_F16) require_type(kGemm, c, "c", OG_F32);
+    range(kGemm, "c", c->length, p->offset_c, result_count(p));
+    if (a_scale == nullptr) null_arg(kGemm, "aScale");
+    if (b_scale == nullptr) null_arg(kGemm, "bScale");
+    check_vector("aScale", a_scale, p->m);
+    require_type(kGemm, &a_scale->buffer, "aScale", OG_F32);
+    check_vector("bScale", b_scale, p->n);
+    require_type(kGemm, &b_scale->buffer, "bScale", OG_F32);
+    if (fbias != nullptr) {
+        check_column_vector("floatBias", fbias, p->n);
+        require_type(kGemm, &fbias->buffer, "floatBias", OG_F32);
+    }
+    if (ibias != nullptr) {
+        check_column_vector("intBias", ibias, p->n);
+        require_type(kGemm, &ibias->buffer, "intBias", OG_I32);
+    }
+    if (activation < OG_ACTIVATION_NONE || activation > OG_ACTIVATION_SILU)
+        shape(kGemm, "activation", std::to_string(activation) + " is not an og_activation");
+    if (residual != nullptr) {
+        if (residual->buffer.ptr == nullptr) null_arg(kGemm, "residual");
+        require_type(kGemm, &residual->buffer, "residual", c->type);
+        range(kGemm, "residual", residual->buffer.length, residual->offset, result_count(p));
+        if (overlaps_shifted(&residual->buffer, residual->offset, c, p->offset_c, result_count(p)))
+            shape(kGemm, "residual", "overlaps c without being the same elements");
+    }
+    return pr;
+}
+
+void require_own_encoder(const char* op, const og_encoder* enc, const og_device* device) {
+    if (enc == nullptr) null_arg(op, "encoder");
+    if (enc->device != device)
+        throw OgError{OG_ERROR_INVALID_HANDLE, op, "encoder", "the encoder belongs to another device", "", "", ""};
+}
+
+void check_dq_rows(const og_buffer* x, int32_t offset_x, int32_t rows, int32_t columns, int32_t row_stride_x,
+                   const og_buffer* y, int32_t offset_y, const og_buffer* scale, int32_t offset_scale,
+                   const og_buffer* zp, int32_t offset_zp) {
+    if (x == nullptr || x->ptr == nullptr) null_arg(kDq, "x");
+    if (y == nullptr || y->ptr == nullptr) null_arg(kDq, "y");
+    if (scale == nullptr || scale->ptr == nullptr) null_arg(kDq, "scale");
+    if (zp == nullptr || zp->ptr == nullptr) null_arg(kDq, "zeroPoint");
+    if (x->type != OG_F16) require_type(kDq, x, "x", OG_F32);
+    require_type(kDq, y, "y", OG_U8);
+    require_type(kDq, scale, "scale", OG_F32);
+    require_type(kDq, zp, "zeroPoint", OG_U8);
+    if (rows < 0) shape(kDq, "rows", "must not be negative, got " + std::to_string(rows));
+    if (columns < 1) shape(kDq, "columns", std::to_string(columns) + " must be at least 1");
+    if (row_stride_x != 0 && row_stride_x < columns)
+        shape(kDq, "rowStrideX",
+              std::to_string(row_stride_x) + " is smaller than the row of " + std::to_string(columns));
+    const int64_t stride = row_stride_x == 0 ? columns : row_stride_x;
+    const int64_t count = static_cast<int64_t>(rows) * columns;
+    if (count > kMaxElements) shape(kDq, "rows", "the tensor holds more elements than the kernels address");
+    range(kDq, "x", x->length, offset_x, rows == 0 ? 0 : (rows - 1) * stride + columns);
+    range(kDq, "y", y->length, offset_y, count);
+    range(kDq, "scale", scale->length, offset_scale, rows);
+    range(kDq, "zeroPoint", zp->length, offset_zp, rows);
+}
+
 void check_dq(const og_buffer* x, int32_t offset_x, int32_t count, const og_buffer* y, int32_t offset_y,
               const og_buffer* scale, int32_t offset_scale, const og_buffer* zp, int32_t offset_zp) {
     if (x == nullptr || x->ptr == nullptr) null_arg(kDq, "x");
@@ -465,7 +539,7 @@ og::GemmLaunch make_launch(og_int8_gemm* g, const og_int8_gemm_problem* p, const
     L.stream_k = g->stream_k;
     og::Epilogue& e = L.epi;
     e.out_kind = out_kind;
-    const int esize = out_kind == og::OUT_I32 || out_kind == og::OUT_F32 ? 4 : 1;
+    const int esize = og::out_bytes(out_kind);
     e.c = static_cast<uint8_t*>(out_base) + static_cast<int64_t>(p->offset_c) * esize;
     e.ldc = p->n;
     e.batch_stride_c = static_cast<int64_t>(p->m) * p->n;
@@ -1276,6 +1350,44 @@ OG_API og_status og_int8_gemm_encode_dequantize(og_int8_gemm* g, og_encoder* enc
     });
 }
 
+OG_API og_status og_int8_gemm_check_activated(const og_int8_gemm_problem* p, const og_buffer* a, const og_buffer* b,
+                                              const og_buffer* c, const og_operand* a_scale, const og_operand* b_scale,
+                                              const og_operand* za, const og_operand* zb, const og_operand* fbias,
+                                              const og_operand* ibias, int32_t activation,
+                                              const og_operand* residual) {
+    return guard([&] { check_activated(p, a, b, c, a_scale, b_scale, za, zb, fbias, ibias, activation, residual); });
+}
+
+OG_API og_status og_int8_gemm_encode_activated(og_int8_gemm* g, og_encoder* enc, const og_int8_gemm_problem* p,
+                                               const og_buffer* a, const og_buffer* b, const og_buffer* c,
+                                               const og_operand* a_scale, const og_operand* b_scale,
+                                               const og_operand* za, const og_operand* zb, const og_operand* fbias,
+                                               const og_operand* ibias, int32_t activation,
+                                               const og_operand* residual) {
+    return guard([&] {
+        live_gemm(g);
+        if (c == nullptr || c->ptr == nullptr) null_arg(kGemm, "c");
+        require_own_encoder(kGemm, enc, g->device);
+        const Prepared pr = check_activated(p, a, b, c, a_scale, b_scale, za, zb, fbias, ibias, activation, residual);
+        if (!pr.ok) {
+            g->last = "none";
+            return;
+        }
+        use(g->device);
+        og::GemmLaunch L =
+            make_launch(g, p, pr, a, b, za, zb, c->type == OG_F16 ? og::OUT_ACT_F16 : og::OUT_ACT_F32, c->ptr);
+        L.epi.int_bias = reinterpret_cast<const int32_t*>(operand_ptr(ibias));
+        L.epi.scale = reinterpret_cast<const float*>(operand_ptr(b_scale));
+        L.epi.scale_vector = b_scale->is_vector;
+        L.epi.row_scale = reinterpret_cast<const float*>(operand_ptr(a_scale));
+        L.epi.row_scale_vector = a_scale->is_vector;
+        L.epi.float_bias = reinterpret_cast<const float*>(operand_ptr(fbias));
+        L.epi.activation = activation;
+        L.epi.residual = operand_ptr(residual);
+        record_gemm(g, enc, L, nullptr);
+    });
+}
+
 OG_API og_status og_int8_gemm_encode_requantized(og_int8_gemm* g, og_encoder* enc, const og_int8_gemm_problem* p,
                                                  const og_buffer* a, const og_buffer* b, const og_buffer* y,
                                                  const og_operand* mult, int32_t zero_y, const og_operand* za,
@@ -1358,6 +1470,37 @@ OG_API og_status og_dynamic_quantize_encode(og_dynamic_quantize* q, og_encoder* 
         enc->ops.push_back(
             [=](cudaStream_t s) { return og::launch_dynamic_quantize(xp, n, yp, sp, zpp, scr, sms, status, s); });
         enc->dispatches += og::dq_single_kernel(xp, n, yp) ? 1 : 2;
+    });
+}
+
+OG_API og_status og_dynamic_quantize_check_rows(const og_buffer* x, int32_t offset_x, int32_t rows, int32_t columns,
+                                                int32_t row_stride_x, const og_buffer* y, int32_t offset_y,
+                                                const og_buffer* scale, int32_t offset_scale, const og_buffer* zp,
+                                                int32_t offset_zp) {
+    return guard([&] {
+        check_dq_rows(x, offset_x, rows, columns, row_stride_x, y, offset_y, scale, offset_scale, zp, offset_zp);
+    });
+}
+
+OG_API og_status og_dynamic_quantize_encode_rows(og_dynamic_quantize* q, og_encoder* enc, const og_buffer* x,
+                                                 int32_t offset_x, int32_t rows, int32_t columns, int32_t row_stride_x,
+                                                 const og_buffer* y, int32_t offset_y, const og_buffer* scale,
+                                                 int32_t offset_scale, const og_buffer* zp, int32_t offset_zp) {
+    return guard([&] {
+        if (q == nullptr) throw OgError{OG_ERROR_INVALID_HANDLE, kDq, "dq", "null handle", "", "", ""};
+        require_own_encoder(kDq, enc, q->device);
+        check_dq_rows(x, offset_x, rows, columns, row_stride_x, y, offset_y, scale, offset_scale, zp, offset_zp);
+        if (rows == 0) return;
+        const bool half = x->type == OG_F16;
+        const uint8_t* xp = static_cast<const uint8_t*>(x->ptr) + static_cast<int64_t>(offset_x) * elem_size(x->type);
+        uint8_t* yp = static_cast<uint8_t*>(y->ptr) + offset_y;
+        float* sp = static_cast<float*>(scale->ptr) + offset_scale;
+        uint8_t* zpp = static_cast<uint8_t*>(zp->ptr) + offset_zp;
+        const int64_t stride = row_stride_x == 0 ? columns : row_stride_x;
+        enc->ops.push_back([=](cudaStream_t s) {
+            return og::launch_dynamic_quantize_rows(xp, half, rows, columns, stride, yp, sp, zpp, s);
+        });
+        enc->dispatches += 1;
     });
 }
 

@@ -12,6 +12,7 @@
 // an all-zero range gives scale 1 and zero point 0, y = clamp(round_half_even(x / scale) + zero point, 0, 255) and
 // NaN gives 0. The divisions are IEEE round-to-nearest (__fdiv_rn), rounding is rintf (half to even), and minimum and
 // maximum do not depend on the order they are found in, so the bits equal the CPU's.
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -406,6 +407,158 @@ cudaError_t launch_dynamic_quantize(const float* x, int64_t count, uint8_t* y, f
     if (err != cudaSuccess) return err;
     // Pass 2 is QuantizeLinear per tensor with the scale and zero point pass 1 stored for the caller.
     return launch_quantize_u8_tensor(x, count, y, scale_out, zp_out, stream);
+}
+
+// ---- one scale and zero point per row (token) ----------------------------------------------------------------------
+//
+// The same arithmetic with the range taken over each row of `columns` elements (rows row_stride apart in x, dense in
+// y). x may be float16 (widened exactly). HBM-bound: a row is read once into registers (KEEP vectors of 16 bytes per
+// thread; what a longer row holds beyond that is read again, an L2 hit), its range folded across the row's threads, and
+// its codes written from the registers. Vectors start at x's first 16-byte boundary in the row; where y is not aligned
+// there (or a row's ends do not fill a vector) bytes are written one by one.
+constexpr int DQR_THREADS = 256;
+constexpr int DQR_KEEP = 4;
+
+template <bool HALF>
+struct DqRow {
+    static constexpr int E = HALF ? 8 : 4;  // elements of one 16-byte vector
+    __device__ __forceinline__ static float at(const void* x, int64_t i) {
+        if constexpr (HALF)
+            return __half2float(__ldg(static_cast<const __half*>(x) + i));
+        else
+            return __ldg(static_cast<const float*>(x) + i);
+    }
+    __device__ __forceinline__ static void unpack(const uint4& w, float (&v)[E]) {
+        const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (HALF) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            } else {
+                v[i] = __uint_as_float(q[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ static void fold(const uint4& w, float& mn, float& mx) {
+        float v[E];
+        unpack(w, v);
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            mn = fminf(mn, v[i]);
+            mx = fmaxf(mx, v[i]);
+        }
+    }
+    __device__ __forceinline__ static void store(const uint4& w, uint8_t* y, bool aligned, const DqQuant& q) {
+        float v[E];
+        unpack(w, v);
+        if (aligned) {
+            if constexpr (HALF)
+                *reinterpret_cast<uint2*>(y) = make_uint2(q.four(make_float4(v[0], v[1], v[2], v[3])),
+                                                          q.four(make_float4(v[4], v[5], v[6], v[7])));
+            else
+                *reinterpret_cast<uint32_t*>(y) = q.four(make_float4(v[0], v[1], v[2], v[3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; i++) y[i] = static_cast<uint8_t>(q.one(v[i]));
+        }
+    }
+};
+
+// TPR threads per row: a warp, or the whole block.
+template <bool HALF, int TPR>
+__global__ void __launch_bounds__(DQR_THREADS)
+    dq_rows_kernel(const void* __restrict__ x, int64_t rows, int columns, int64_t row_stride, uint8_t* __restrict__ y,
+                   float* __restrict__ scale_out, uint8_t* __restrict__ zp_out) {
+    using Row = DqRow<HALF>;
+    constexpr int E = Row::E;
+    __shared__ float smin[32], smax[32];
+    __shared__ float range[2];
+    pdl_trigger();
+    pdl_wait();
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (DQR_THREADS / TPR) + threadIdx.x / TPR;
+    if (row >= rows) return;  // whole warps (a block's one row always exists)
+    const int t = threadIdx.x % TPR;
+    const int64_t size = HALF ? 2 : 4;
+    const uint8_t* xr = static_cast<const uint8_t*>(x) + row * row_stride * size;
+    uint8_t* yr = y + row * columns;
+    int head = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / size);
+    if (head > columns) head = columns;
+    const uint4* xv = reinterpret_cast<const uint4*>(xr + head * size);
+    const int nvec = (columns - head) / E;
+    const int tail0 = head + nvec * E;
+    const uint4 none = HALF ? make_uint4(0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u)   // NaN, skipped
+                            : make_uint4(0x7FC00000u, 0x7FC00000u, 0x7FC00000u, 0x7FC00000u);  // by fminf / fmaxf
+    float mn = INFINITY, mx = -INFINITY;
+    uint4 keep[DQR_KEEP];
+#pragma unroll
+    for (int j = 0; j < DQR_KEEP; j++) keep[j] = t + j * TPR < nvec ? __ldg(xv + t + j * TPR) : none;
+    for (int i = t; i < head + (columns - tail0); i += TPR) {
+        const float v = Row::at(xr, i < head ? i : tail0 + i - head);
+        mn = fminf(mn, v);
+        mx = fmaxf(mx, v);
+    }
+    for (int i = t + DQR_KEEP * TPR; i < nvec; i += TPR) Row::fold(__ldg(xv + i), mn, mx);
+#pragma unroll
+    for (int j = 0; j < DQR_KEEP; j++) Row::fold(keep[j], mn, mx);
+    if constexpr (TPR == 32) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            mn = fminf(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, o));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+        }
+    } else {
+        block_min_max(mn, mx, smin, smax);
+        if (threadIdx.x == 0) {
+            range[0] = mn;
+            range[1] = mx;
+        }
+        __syncthreads();
+        mn = range[0];
+        mx = range[1];
+    }
+    DqQuant q;
+    int zp;
+    dq_scale_zero_point(mn, mx, q.s, zp);
+    if (t == 0) {
+        scale_out[row] = q.s;
+        zp_out[row] = static_cast<uint8_t>(zp);
+    }
+    q.zf = static_cast<float>(zp);
+    q.r = __frcp_rn(q.s);
+    q.r_ok = fabsf(q.r) >= 1.17549435e-38f && fabsf(q.r) <= 3.40282347e+38f;  // normal and finite
+    q.cz = __fadd_rn(q.zf, 12582912.0f);  // exact: an integer below 2^24
+    uint8_t* yv = yr + head;
+    const bool aligned = (reinterpret_cast<uintptr_t>(yv) & (E - 1)) == 0;
+#pragma unroll
+    for (int j = 0; j < DQR_KEEP; j++)
+        if (t + j * TPR < nvec) Row::store(keep[j], yv + static_cast<int64_t>(t + j * TPR) * E, aligned, q);
+    for (int i = t + DQR_KEEP * TPR; i < nvec; i += TPR)
+        Row::store(__ldg(xv + i), yv + static_cast<int64_t>(i) * E, aligned, q);
+    for (int i = t; i < head + (columns - tail0); i += TPR) {
+        const int c = i < head ? i : tail0 + i - head;
+        yr[c] = static_cast<uint8_t>(q.one(Row::at(xr, c)));
+    }
+}
+
+template <bool HALF>
+static cudaError_t launch_rows_t(const void* x, int64_t rows, int columns, int64_t row_stride, uint8_t* y, float* scale,
+                                 uint8_t* zp, cudaStream_t stream) {
+    if (columns <= 1024) {
+        constexpr int PER_BLOCK = DQR_THREADS / 32;
+        const unsigned blocks = static_cast<unsigned>((rows + PER_BLOCK - 1) / PER_BLOCK);
+        return launch_pdl(dq_rows_kernel<HALF, 32>, dim3(blocks), dim3(DQR_THREADS), 0, stream, x, rows, columns,
+                          row_stride, y, scale, zp);
+    }
+    return launch_pdl(dq_rows_kernel<HALF, DQR_THREADS>, dim3(static_cast<unsigned>(rows)), dim3(DQR_THREADS), 0, stream,
+                      x, rows, columns, row_stride, y, scale, zp);
+}
+
+cudaError_t launch_dynamic_quantize_rows(const void* x, bool half, int64_t rows, int columns, int64_t row_stride,
+                                         uint8_t* y, float* scale, uint8_t* zp, cudaStream_t stream) {
+    return half ? launch_rows_t<true>(x, rows, columns, row_stride, y, scale, zp, stream)
+                : launch_rows_t<false>(x, rows, columns, row_stride, y, scale, zp, stream);
 }
 
 }  // namespace og

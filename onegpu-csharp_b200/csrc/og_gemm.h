@@ -135,5 +135,9 @@ size_t dq_scratch_bytes();
 bool dq_single_kernel(const float* x, int64_t count, const uint8_t* y);
 cudaError_t launch_dynamic_quantize(const float* x, int64_t count, uint8_t* y, float* scale_out, uint8_t* zp_out,
                                     DqScratch* scratch, int num_sms, int* error_flag, cudaStream_t stream);
+// The same with one scale and zero point per row of a rows x columns tensor of float32 or float16 (half): rows start
+// row_stride elements apart in x and are dense in y.
+cudaError_t launch_dynamic_quantize_rows(const void* x, bool half, int64_t rows, int columns, int64_t row_stride,
+                                         uint8_t* y, float* scale, uint8_t* zp, cudaStream_t stream);
 
 }  // namespace og

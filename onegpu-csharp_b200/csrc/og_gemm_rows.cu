@@ -98,6 +98,8 @@ __device__ __forceinline__ void store_one(const Epilogue& e, int b, int m, int n
         __stcs(static_cast<int32_t*>(e.c) + idx, static_cast<int32_t>(s));
     } else if constexpr (OUT == OUT_F32) {
         __stcs(static_cast<float*>(e.c) + idx, finish_float(e, n, s));
+    } else if constexpr (out_activated(OUT)) {
+        store_activated<OUT>(e, idx, m, n, s);
     } else {
         static_cast<uint8_t*>(e.c)[idx] = finish_byte(e, n, s, OUT == OUT_U8);
     }
@@ -807,6 +809,10 @@ LaunchFn prepare_gemm_rows(const GemmLaunch& L, cudaError_t* err) {
                                     : bind_rows_stream_t<false, OUT_I32>(p, ma, mb, grid, idesc);
             case OUT_F32: return km ? bind_rows_stream_t<true, OUT_F32>(p, ma, mb, grid, idesc)
                                     : bind_rows_stream_t<false, OUT_F32>(p, ma, mb, grid, idesc);
+            case OUT_ACT_F32: return km ? bind_rows_stream_t<true, OUT_ACT_F32>(p, ma, mb, grid, idesc)
+                                        : bind_rows_stream_t<false, OUT_ACT_F32>(p, ma, mb, grid, idesc);
+            case OUT_ACT_F16: return km ? bind_rows_stream_t<true, OUT_ACT_F16>(p, ma, mb, grid, idesc)
+                                        : bind_rows_stream_t<false, OUT_ACT_F16>(p, ma, mb, grid, idesc);
             case OUT_U8: return km ? bind_rows_stream_t<true, OUT_U8>(p, ma, mb, grid, idesc)
                                    : bind_rows_stream_t<false, OUT_U8>(p, ma, mb, grid, idesc);
             default: return km ? bind_rows_stream_t<true, OUT_S8>(p, ma, mb, grid, idesc)
@@ -819,6 +825,10 @@ LaunchFn prepare_gemm_rows(const GemmLaunch& L, cudaError_t* err) {
                                 : bind_rows_t<false, OUT_I32>(p, ma, mb, grid, idesc);
         case OUT_F32: return km ? bind_rows_t<true, OUT_F32>(p, ma, mb, grid, idesc)
                                 : bind_rows_t<false, OUT_F32>(p, ma, mb, grid, idesc);
+        case OUT_ACT_F32: return km ? bind_rows_t<true, OUT_ACT_F32>(p, ma, mb, grid, idesc)
+                                    : bind_rows_t<false, OUT_ACT_F32>(p, ma, mb, grid, idesc);
+        case OUT_ACT_F16: return km ? bind_rows_t<true, OUT_ACT_F16>(p, ma, mb, grid, idesc)
+                                    : bind_rows_t<false, OUT_ACT_F16>(p, ma, mb, grid, idesc);
         case OUT_U8: return km ? bind_rows_t<true, OUT_U8>(p, ma, mb, grid, idesc)
                                : bind_rows_t<false, OUT_U8>(p, ma, mb, grid, idesc);
         default: return km ? bind_rows_t<true, OUT_S8>(p, ma, mb, grid, idesc)

@@ -31,6 +31,8 @@ __device__ __forceinline__ void simt_store(const Epilogue& e, int b, int m, int 
         static_cast<int32_t*>(e.c)[idx] = static_cast<int32_t>(sum);
     } else if constexpr (OUT == OUT_F32) {
         static_cast<float*>(e.c)[idx] = finish_float(e, n, sum);
+    } else if constexpr (out_activated(OUT)) {
+        store_activated<OUT>(e, idx, m, n, sum);
     } else {
         static_cast<uint8_t*>(e.c)[idx] = finish_byte(e, n, sum, OUT == OUT_U8);
     }
@@ -129,6 +131,12 @@ cudaError_t launch_gemm_simt(const GemmLaunch& L, cudaStream_t stream) {
         case OUT_I32: int8_gemm_simt_kernel<OUT_I32><<<grid, simt::THREADS, 0, stream>>>(L, tiles_m, tiles_n); break;
         case OUT_F32: int8_gemm_simt_kernel<OUT_F32><<<grid, simt::THREADS, 0, stream>>>(L, tiles_m, tiles_n); break;
         case OUT_U8: int8_gemm_simt_kernel<OUT_U8><<<grid, simt::THREADS, 0, stream>>>(L, tiles_m, tiles_n); break;
+        case OUT_ACT_F32:
+            int8_gemm_simt_kernel<OUT_ACT_F32><<<grid, simt::THREADS, 0, stream>>>(L, tiles_m, tiles_n);
+            break;
+        case OUT_ACT_F16:
+            int8_gemm_simt_kernel<OUT_ACT_F16><<<grid, simt::THREADS, 0, stream>>>(L, tiles_m, tiles_n);
+            break;
         default: int8_gemm_simt_kernel<OUT_S8><<<grid, simt::THREADS, 0, stream>>>(L, tiles_m, tiles_n); break;
     }
     return cudaGetLastError();

@@ -82,6 +82,7 @@ struct TcParams {
     Epilogue epi;
     int* error_flag;
     int tma_store;  // int32 / float results leave through shared memory and TMA stores (C rows 16-byte aligned)
+    int residual_vec;  // activated form: 16-byte loads of the residual (its rows 16-byte aligned)
     // Stream-K: the workers split the total_tiles * k_blocks (tile, K block) units into equal contiguous ranges. A
     // tile cut by a range boundary is finished by the worker holding its K-block-0 segment (the end of its range),
     // after the next worker has handed over the sums of the later segment (the start of its range) through
@@ -375,6 +376,91 @@ __device__ __forceinline__ void stage_half(const ColTerms& t, const Epilogue& e,
     }
 }
 
+// The activated form of N consecutive sums of one row (tile columns j0.., output element idx of the first; the first
+// `cols` of them inside the output).
+template <int OUT, int N>
+__device__ __forceinline__ void finish_activated(const ColTerms& t, const Epilogue& e, bool za_per_row, uint32_t za,
+                                                 uint32_t rt, float row_scale, int j0, int64_t idx, int cols,
+                                                 bool res_vec, const uint32_t* r, float (&f)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; q++)
+        f[q] = scaled_sum(tile_sum(t, za_per_row, za, rt, j0 + q, r[q]), row_scale, t.scale[j0 + q],
+                          e.float_bias != nullptr, t.fbias[j0 + q]);
+    activate_all(f, e.activation);
+    if (e.residual == nullptr) return;
+    if (res_vec && cols >= N) {
+        if constexpr (OUT == OUT_ACT_F16) {
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __half*>(e.residual) + idx);
+#pragma unroll
+            for (int q = 0; q < N; q += 8) {
+                const uint4 w = src[q / 8];
+                const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[u]));
+                    f[q + 2 * u] = __fadd_rn(f[q + 2 * u], v.x);
+                    f[q + 2 * u + 1] = __fadd_rn(f[q + 2 * u + 1], v.y);
+                }
+            }
+        } else {
+            const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(e.residual) + idx);
+#pragma unroll
+            for (int q = 0; q < N; q += 4) {
+                const float4 v = src[q / 4];
+                f[q] = __fadd_rn(f[q], v.x);
+                f[q + 1] = __fadd_rn(f[q + 1], v.y);
+                f[q + 2] = __fadd_rn(f[q + 2], v.z);
+                f[q + 3] = __fadd_rn(f[q + 3], v.w);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < N; q++)
+        if (q < cols) f[q] = __fadd_rn(f[q], residual_at<OUT>(e, idx + q));
+}
+
+// Two results as one word of float16.
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One 64-byte row of a store box: 16 words in the 64-byte swizzle (see stage_half).
+__device__ __forceinline__ void stage_words(const uint32_t (&w)[16], uint8_t* box, int lane) {
+    const uint32_t row = smem_u32(box) + lane * 64;
+    const uint32_t sw = (lane >> 1) & 3;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t addr = row + ((j ^ sw) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[4 * j]), "r"(w[4 * j + 1]),
+                     "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                     : "memory");
+    }
+}
+
+// Stores 32 consecutive activated results of one row (output element idx, tile column j0, `cols` of them inside the
+// output) when the output's rows do not allow TMA stores.
+template <int OUT>
+__device__ __forceinline__ void store_chunk_activated(const ColTerms& t, const Epilogue& e, bool za_per_row, uint32_t za,
+                                                      uint32_t rt, float row_scale, int64_t idx, int j0, int cols,
+                                                      const uint32_t (&r)[32]) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float f[16];
+        finish_activated<OUT>(t, e, za_per_row, za, rt, row_scale, j0 + 16 * h, idx + 16 * h, cols - 16 * h, false,
+                              r + 16 * h, f);
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+            if (16 * h + q >= cols) break;
+            if constexpr (OUT == OUT_ACT_F16)
+                static_cast<__half*>(e.c)[idx + 16 * h + q] = __float2half_rn(f[q]);
+            else
+                static_cast<float*>(e.c)[idx + 16 * h + q] = f[q];
+        }
+    }
+}
+
 // Stores 32 consecutive results of row m (columns n0.. of the output; j0 is n0's column within the tile).
 template <int OUT>
 __device__ __forceinline__ void store_chunk(const ColTerms& t, const Epilogue& e, bool terms, bool za_per_row,
@@ -472,8 +558,9 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
     }
-    constexpr bool WORDS = OUT == OUT_I32 || OUT == OUT_F32;
-    const bool tma_store = WORDS && p.tma_store;
+    constexpr bool ACT = out_activated(OUT);
+    constexpr bool BOXED = OUT == OUT_I32 || OUT == OUT_F32 || ACT;  // results that can leave through store boxes
+    const bool tma_store = BOXED && p.tma_store;
     if (tma_store && warp == 2 && lane == 0) prefetch_tmap(&tmap_c);
     pdl_wait();  // the preceding grid is done: its outputs are readable and its TMEM is free
     // This launch's stream-K generation: flags set to it belong to this launch.
@@ -706,6 +793,12 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                 const uint32_t rsa = e.row_sum_a ? row_sum_of(e, b, m) : 0u;
                 rt = static_cast<uint32_t>(p.k) * za - rsa;
             }
+            float row_scale = 0.0f;  // activated form: the scale of this row of A, and the row's place in the output
+            int64_t row_at = 0;
+            if constexpr (ACT) {
+                if (row_ok) row_scale = row_scale_of(e, m);
+                row_at = b * e.batch_stride_c + static_cast<int64_t>(m) * e.ldc;
+            }
             if (tma_store) {
                 // Each 32 x 32 chunk leaves as two TMA stores of 32 x 16 words (64-byte row segments) through this
                 // warp's boxes in turn (with two boxes, staging one half never waits for the store just issued);
@@ -719,6 +812,29 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                     tmem_ld_32x32b_x32(t_row + c * 32, r);
                     tmem_ld_wait();
                     if (sk_in != nullptr) sk_add(sk_in, c, row_in_cta, r);
+                    if constexpr (OUT == OUT_ACT_F16) {  // 32 float16 results fill one box
+                        uint8_t* box = staging + ew * C::BOXES * C::BOX_BYTES;
+                        uint32_t w[16];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            float f[16];
+                            finish_activated<OUT>(terms_smem, e, za_per_row, za, rt, row_scale, c * 32 + 16 * h,
+                                                  row_at + n0 + 16 * h, row_ok ? p.n - n0 - 16 * h : 0, p.residual_vec,
+                                                  r + 16 * h, f);
+#pragma unroll
+                            for (int q = 0; q < 8; q++) w[8 * h + q] = half_pair(f[2 * q], f[2 * q + 1]);
+                        }
+                        if (lane == 0) bulk_wait_group_read<0>();
+                        __syncwarp();
+                        stage_words(w, box, lane);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&tmap_c, box, n0, box_row, b);
+                            bulk_commit_group();
+                        }
+                        continue;
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         if (n0 + 16 * h >= p.n) break;
@@ -726,8 +842,19 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                         uint8_t* box = staging + (ew * C::BOXES + h % C::BOXES) * C::BOX_BYTES;
                         if (lane == 0) bulk_wait_group_read<C::BOXES - 1>();
                         __syncwarp();
-                        stage_half<OUT>(terms_smem, e, with_terms, za_per_row, za, rt, c * 32 + 16 * h, r + 16 * h,
-                                        box, lane);
+                        if constexpr (OUT == OUT_ACT_F32) {
+                            float f[16];
+                            uint32_t w[16];
+                            finish_activated<OUT>(terms_smem, e, za_per_row, za, rt, row_scale, c * 32 + 16 * h,
+                                                  row_at + n0 + 16 * h, row_ok ? p.n - n0 - 16 * h : 0, p.residual_vec,
+                                                  r + 16 * h, f);
+#pragma unroll
+                            for (int q = 0; q < 16; q++) w[q] = __float_as_uint(f[q]);
+                            stage_words(w, box, lane);
+                        } else {
+                            stage_half<OUT>(terms_smem, e, with_terms, za_per_row, za, rt, c * 32 + 16 * h, r + 16 * h,
+                                            box, lane);
+                        }
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
@@ -748,7 +875,13 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                     tmem_ld_32x32b_x32(t_row + c * 32, r);
                     tmem_ld_wait();
                     if (sk_in != nullptr) sk_add(sk_in, c, row_in_cta, r);
-                    if (row_ok) store_chunk<OUT>(terms_smem, e, terms, za_per_row, za, rt, b, m, n0, c * 32, r);
+                    if constexpr (ACT) {
+                        if (row_ok)
+                            store_chunk_activated<OUT>(terms_smem, e, za_per_row, za, rt, row_scale, row_at + n0, c * 32,
+                                                       min(32, p.n - n0), r);
+                    } else {
+                        if (row_ok) store_chunk<OUT>(terms_smem, e, terms, za_per_row, za, rt, b, m, n0, c * 32, r);
+                    }
                 }
             }
             tc_fence_before();
@@ -839,16 +972,16 @@ static bool make_map(CUtensorMap* map, const void* base, uint64_t x, uint64_t y,
 }
 
 // The output C as a 3-D tensor of 4-byte words (columns innermost) stored in 32-row x 16-word boxes from 64-byte-swizzled
-// shared memory.
+// shared memory; float16 results (half) as 2-byte elements in 32 x 32 boxes of the same size.
 static bool make_store_map(CUtensorMap* map, void* base, uint64_t n, uint64_t m, uint64_t batch, uint64_t row_bytes,
-                           uint64_t batch_bytes) {
+                           uint64_t batch_bytes, bool half) {
     auto fn = encode_fn();
     if (fn == nullptr) return false;
     cuuint64_t dims[3] = {n, m, batch};
     cuuint64_t strides[2] = {row_bytes, batch_bytes};
-    cuuint32_t box[3] = {16, 32, 1};
+    cuuint32_t box[3] = {half ? 32u : 16u, 32, 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    CUresult r = fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_INT32, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }
@@ -1046,12 +1179,15 @@ static LaunchFn prepare_cg(const GemmLaunch& L, cudaError_t* err) {
     // int32 / float results go out through TMA stores when C's rows (and batches) start on 16-byte boundaries.
     CUtensorMap mc;
     std::memset(&mc, 0, sizeof(mc));
-    const bool words = L.epi.out_kind == OUT_I32 || L.epi.out_kind == OUT_F32;
-    const bool c_aligned = (reinterpret_cast<uintptr_t>(L.epi.c) & 15) == 0 && (L.epi.ldc & 3) == 0 &&
-                           (L.batch == 1 || (L.epi.batch_stride_c & 3) == 0);
-    p.tma_store = words && c_aligned &&
-                  make_store_map(&mc, L.epi.c, L.n, L.m, L.batch, uint64_t(L.epi.ldc) * 4,
-                                 L.batch > 1 ? uint64_t(L.epi.batch_stride_c) * 4 : round16(uint64_t(L.epi.ldc) * 4 * L.m));
+    const uint64_t out_size = out_bytes(L.epi.out_kind);
+    const bool boxed = out_size > 1;
+    const uint64_t row_bytes = uint64_t(L.epi.ldc) * out_size, batch_bytes = uint64_t(L.epi.batch_stride_c) * out_size;
+    const bool rows_aligned = (row_bytes & 15) == 0 && (L.batch == 1 || (batch_bytes & 15) == 0);
+    const bool c_aligned = (reinterpret_cast<uintptr_t>(L.epi.c) & 15) == 0 && rows_aligned;
+    p.tma_store = boxed && c_aligned &&
+                  make_store_map(&mc, L.epi.c, L.n, L.m, L.batch, row_bytes,
+                                 L.batch > 1 ? batch_bytes : round16(row_bytes * L.m), out_size == 2);
+    p.residual_vec = (reinterpret_cast<uintptr_t>(L.epi.residual) & 15) == 0 && rows_aligned;
     const int64_t workers = L.num_sms / CG;
     int grid = static_cast<int>((total < workers ? total : workers) * CG);
     // Stream-K when it pays (sk_worthwhile) and the caller gave the hand-over buffers.
@@ -1087,6 +1223,10 @@ static LaunchFn prepare_cg(const GemmLaunch& L, cudaError_t* err) {
                                  : bind_tc_s<CG, false, OUT_I32>(L, p, ma, mb, mc, grid);
         case OUT_F32: return bmn ? bind_tc_s<CG, true, OUT_F32>(L, p, ma, mb, mc, grid)
                                  : bind_tc_s<CG, false, OUT_F32>(L, p, ma, mb, mc, grid);
+        case OUT_ACT_F32: return bmn ? bind_tc_s<CG, true, OUT_ACT_F32>(L, p, ma, mb, mc, grid)
+                                     : bind_tc_s<CG, false, OUT_ACT_F32>(L, p, ma, mb, mc, grid);
+        case OUT_ACT_F16: return bmn ? bind_tc_s<CG, true, OUT_ACT_F16>(L, p, ma, mb, mc, grid)
+                                     : bind_tc_s<CG, false, OUT_ACT_F16>(L, p, ma, mb, mc, grid);
         case OUT_U8: return bmn ? bind_tc_s<CG, true, OUT_U8>(L, p, ma, mb, mc, grid)
                                 : bind_tc_s<CG, false, OUT_U8>(L, p, ma, mb, mc, grid);
         default: return bmn ? bind_tc_s<CG, true, OUT_S8>(L, p, ma, mb, mc, grid)

@@ -3,11 +3,21 @@
 #pragma once
 
 #include <cstdint>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include "og_act.cuh"
 
 namespace og {
 
-enum OutKind : int { OUT_I32 = 0, OUT_F32 = 1, OUT_U8 = 2, OUT_S8 = 3 };
+// OUT_ACT_F32 / OUT_ACT_F16: the float form with a scale per row of A, an activation and a residual
+// (og_int8_gemm_encode_activated), stored as float32 or float16.
+enum OutKind : int { OUT_I32 = 0, OUT_F32 = 1, OUT_U8 = 2, OUT_S8 = 3, OUT_ACT_F32 = 4, OUT_ACT_F16 = 5 };
+
+__host__ __device__ constexpr bool out_activated(int out) { return out == OUT_ACT_F32 || out == OUT_ACT_F16; }
+__host__ __device__ constexpr int out_bytes(int out) {
+    return out == OUT_U8 || out == OUT_S8 ? 1 : out == OUT_ACT_F16 ? 2 : 4;
+}
 
 // What a product kernel needs to finish and store C[b, m, n]. Zero points: mode 0 absent, 1 one value, 2 one per row
 // (A) or per column (B). The correction uses the byte sums of the other operand:
@@ -37,6 +47,12 @@ struct Epilogue {
     const float* float_bias;      // per column, or null
     int zero_point_y;
     int vec_ok;                   // every output row starts on a 16-byte boundary
+    // Activated form: the scale of A (one, or one per row), the activation, and the residual (laid out like the output
+    // and of its type, possibly the output itself) or null.
+    const float* row_scale;
+    int row_scale_vector;
+    int activation;
+    const void* residual;
 };
 
 __device__ __forceinline__ int32_t zp_value(const uint8_t* z, int vector, int is_signed, int idx) {
@@ -73,6 +89,41 @@ __device__ __forceinline__ float finish_float(const Epilogue& e, int n, uint32_t
     float f = __fmul_rn(__int2float_rn(static_cast<int32_t>(s)), sc);
     if (e.float_bias != nullptr) f = __fadd_rn(f, __ldg(e.float_bias + n));
     return f;
+}
+
+// The scale of row m of A in the activated form.
+__device__ __forceinline__ float row_scale_of(const Epilogue& e, int m) {
+    return __ldg(e.row_scale + (e.row_scale_vector ? m : 0));
+}
+
+// The activated form before its activation: float(sum) * (aScale * bScale[n]), then + float bias, each step rounded
+// on its own as in the dequantize form.
+__device__ __forceinline__ float scaled_sum(uint32_t s, float row_scale, float scale, bool biased, float bias) {
+    const float f = __fmul_rn(__int2float_rn(static_cast<int32_t>(s)), __fmul_rn(row_scale, scale));
+    return biased ? __fadd_rn(f, bias) : f;
+}
+
+// Element idx of the residual, as float32. A plain load: the residual may be the output itself, whose element idx is
+// written by the thread that has read it here.
+template <int OUT>
+__device__ __forceinline__ float residual_at(const Epilogue& e, int64_t idx) {
+    if constexpr (OUT == OUT_ACT_F16)
+        return __half2float(static_cast<const __half*>(e.residual)[idx]);
+    else
+        return static_cast<const float*>(e.residual)[idx];
+}
+
+// One result of the activated form at element idx of the output (row m, column n), stored.
+template <int OUT>
+__device__ __forceinline__ void store_activated(const Epilogue& e, int64_t idx, int m, int n, uint32_t s) {
+    float f[1] = {scaled_sum(s, row_scale_of(e, m), __ldg(e.scale + (e.scale_vector ? n : 0)), e.float_bias != nullptr,
+                             e.float_bias != nullptr ? __ldg(e.float_bias + n) : 0.0f)};
+    activate_all(f, e.activation);
+    if (e.residual != nullptr) f[0] = __fadd_rn(f[0], residual_at<OUT>(e, idx));
+    if constexpr (OUT == OUT_ACT_F16)
+        static_cast<__half*>(e.c)[idx] = __float2half_rn(f[0]);
+    else
+        static_cast<float*>(e.c)[idx] = f[0];
 }
 
 // clamp(round_half_even(float(sum) * multiplier) + zeroPointY) to the output type, NaN to the smallest value

@@ -45,6 +45,8 @@ _NP = {U8: np.uint8, S8: np.int8, I32: np.int32, F32: np.float32, F16: np.float1
 _FROM_NP = {np.dtype(v): k for k, v in _NP.items()}
 
 KERNEL_AUTO, KERNEL_TENSOR_CORE, KERNEL_PORTABLE = 0, 1, 2
+# og_activation
+ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_GELU, ACTIVATION_GELU_TANH, ACTIVATION_SILU = 0, 1, 2, 3, 4
 
 
 class og_error_info(ctypes.Structure):
@@ -83,6 +85,10 @@ _PP = ctypes.POINTER(ctypes.c_void_p)
 _BUF = ctypes.POINTER(og_buffer)
 _OPD = ctypes.POINTER(og_operand)
 _PROB = ctypes.POINTER(og_int8_gemm_problem)
+
+# x, offset, rows, columns, row stride, y, offset, scale, offset, zero point, offset
+_ROWS_ARGS = [_BUF, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _BUF, ctypes.c_int32, _BUF,
+              ctypes.c_int32, _BUF, ctypes.c_int32]
 
 # x, offset, shape, rank, axis, per_axis, scale, offset, zero point, offset, output, offset
 _QUANT_ARGS = [_BUF, ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
@@ -131,6 +137,9 @@ EXPORTS = {
                                         _OPD],
     "og_int8_gemm_encode_dequantize": [_P, _P, _PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD, _OPD, _OPD, _OPD],
     "og_int8_gemm_check_dequantize": [_PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD, _OPD, _OPD, _OPD],
+    "og_int8_gemm_encode_activated": [_P, _P, _PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD, _OPD, _OPD, _OPD,
+                                      ctypes.c_int32, _OPD],
+    "og_int8_gemm_check_activated": [_PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD, _OPD, _OPD, _OPD, ctypes.c_int32, _OPD],
     "og_int8_gemm_int32_noalloc": [_P, _PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD],
     "og_int8_gemm_noalloc_status": [_P],
     "og_int8_gemm_noalloc_watchdog_selftest": [_P, ctypes.c_uint32],
@@ -143,6 +152,8 @@ EXPORTS = {
                                    ctypes.c_int32, _BUF, ctypes.c_int32],
     "og_dynamic_quantize_check": [_BUF, ctypes.c_int32, ctypes.c_int32, _BUF, ctypes.c_int32, _BUF, ctypes.c_int32,
                                   _BUF, ctypes.c_int32],
+    "og_dynamic_quantize_encode_rows": [_P, _P] + _ROWS_ARGS,
+    "og_dynamic_quantize_check_rows": _ROWS_ARGS,
     "og_buffer_write_async": [_P, _P, _P, ctypes.c_uint64],
     "og_buffer_read_async": [_P, _P, _P, ctypes.c_uint64, _PP],
     "og_readback_wait": [_P],
@@ -694,6 +705,20 @@ class Int8Gemm:
                                                    _opd(zero_point_a), _opd(zero_point_b), _opd(float_bias),
                                                    _opd(int_bias)))
 
+    def encode_activated(self, encoder: GpuCommandEncoder, problem: Int8GemmProblem, a: GpuBuffer, b: GpuBuffer,
+                         c: GpuBuffer, a_scale: Int8Operand, b_scale: Int8Operand,
+                         zero_point_a: Optional[Int8Operand] = None, zero_point_b: Optional[Int8Operand] = None,
+                         float_bias: Optional[Int8Operand] = None, int_bias: Optional[Int8Operand] = None,
+                         activation: int = ACTIVATION_NONE, residual: Optional[Int8Operand] = None) -> None:
+        """activation(float(sum + intBias) * (aScale[m] * bScale[n]) + floatBias[n]) + residual[m, n] in one call, with
+        float32 or float16 results: a_scale is one value or one per row (``DynamicQuantizeKernels.encode_rows``), the
+        residual has c's type and layout and may be c itself. No counterpart in the reference."""
+        p = problem.c_struct()
+        _check(_lib.og_int8_gemm_encode_activated(self.handle, encoder.handle if encoder else None, ctypes.byref(p),
+                                                  _buf(a), _buf(b), _buf(c), _opd(a_scale), _opd(b_scale),
+                                                  _opd(zero_point_a), _opd(zero_point_b), _opd(float_bias),
+                                                  _opd(int_bias), int(activation), _opd(residual)))
+
     # The reference's member names.
     EncodeInt32 = encode_int32
     EncodeFloat = encode_float
@@ -776,6 +801,15 @@ def check_dequantize(problem, a, b, c, a_scale, b_scale, zero_point_a=None, zero
                                               _opd(float_bias), _opd(int_bias)))
 
 
+def check_activated(problem, a, b, c, a_scale, b_scale, zero_point_a=None, zero_point_b=None, float_bias=None,
+                    int_bias=None, activation=ACTIVATION_NONE, residual=None) -> None:
+    """The argument checks of Int8Gemm.encode_activated alone (no device needed)."""
+    p = problem.c_struct()
+    _check(_lib.og_int8_gemm_check_activated(ctypes.byref(p), _buf(a), _buf(b), _buf(c), _opd(a_scale), _opd(b_scale),
+                                             _opd(zero_point_a), _opd(zero_point_b), _opd(float_bias),
+                                             _opd(int_bias), int(activation), _opd(residual)))
+
+
 def check_requantized(problem, a, b, y, multiplier, zero_point_y, zero_point_a=None, zero_point_b=None,
                       int_bias=None, scratch=None) -> None:
     p = problem.c_struct()
@@ -788,6 +822,13 @@ def check_dynamic_quantize(x, offset_x, count, y, offset_y, scale, offset_scale,
                            offset_zero_point) -> None:
     _check(_lib.og_dynamic_quantize_check(_buf(x), offset_x, count, _buf(y), offset_y, _buf(scale), offset_scale,
                                           _buf(zero_point), offset_zero_point))
+
+
+def check_dynamic_quantize_rows(x, offset_x, rows, columns, row_stride_x, y, offset_y, scale, offset_scale, zero_point,
+                                offset_zero_point) -> None:
+    """The argument checks of DynamicQuantizeKernels.encode_rows alone (no device needed)."""
+    _check(_lib.og_dynamic_quantize_check_rows(_buf(x), offset_x, rows, columns, row_stride_x, _buf(y), offset_y,
+                                               _buf(scale), offset_scale, _buf(zero_point), offset_zero_point))
 
 
 def _shape(shape):
@@ -1004,6 +1045,16 @@ class DynamicQuantizeKernels:
         _check(_lib.og_dynamic_quantize_encode(self.handle, encoder.handle if encoder else None, _buf(x), offset_x,
                                                count, _buf(y), offset_y, _buf(scale), offset_scale, _buf(zero_point),
                                                offset_zero_point))
+
+    def encode_rows(self, encoder: GpuCommandEncoder, x: GpuBuffer, offset_x: int, rows: int, columns: int,
+                    row_stride_x: int, y: GpuBuffer, offset_y: int, scale: GpuBuffer, offset_scale: int,
+                    zero_point: GpuBuffer, offset_zero_point: int) -> None:
+        """DynamicQuantizeLinear of every row (token) of a rows x columns tensor on its own: x float32 or float16 with
+        rows row_stride_x elements apart (0: dense), y dense, one scale and zero point per row. No counterpart in the
+        reference."""
+        _check(_lib.og_dynamic_quantize_encode_rows(self.handle, encoder.handle if encoder else None, _buf(x), offset_x,
+                                                    rows, columns, row_stride_x, _buf(y), offset_y, _buf(scale),
+                                                    offset_scale, _buf(zero_point), offset_zero_point))
 
     Encode = encode
 
