@@ -415,6 +415,49 @@ OG_API og_status og_dequantize_check_quantize(const og_buffer* x, int32_t offset
                                               int32_t offset_zero_point, const og_buffer* output,
                                               int32_t offset_output);
 
+/* ---- Int8MoeKernels: a mixture-of-experts layer on int8 weights (no counterpart in the reference) ------------------
+ * For a few tokens (a decode step), float activations that are not quantized:
+ *   logits[t][e] = sum_d x[t][d] router[e][d];  p = softmax of a token's logits over the experts
+ *   a token's top_k experts by p (equal ones: the lowest index first; a NaN logit ranks below every number);
+ *   w = p, or p / (the sum of the chosen p) when `normalize` is set
+ *   u[j] = w_in_scale[e][j] sum_d w_in[e][j][d] x[t][d]
+ *   h[j] = activation(u[j]) * u[expert_size + j] when `gated` is set (w_in holds the activated half's expert_size rows,
+ *          then the other half's), activation(u[j]) otherwise
+ *   y[t][d] = residual[t][d] + sum over the chosen experts of w w_out_scale[e][d] sum_j w_out[e][d][j] h[j]
+ * All sums are held in float32. */
+
+/* tokens 0 .. 128; model_size and expert_size 1 .. 65536; experts 1 .. 512; top_k 1 .. min(experts, 16); activation an
+ * og_activation; gated and normalize 0 or 1; offsets in elements. */
+typedef struct og_moe_problem {
+    int32_t tokens, model_size, expert_size, experts, top_k;
+    int32_t activation, gated, normalize;
+    int32_t offset_x, offset_router, offset_in, offset_in_scale, offset_out, offset_out_scale, offset_y;
+    int32_t offset_residual, offset_ids, offset_weights;
+} og_moe_problem;
+
+typedef struct og_int8_moe og_int8_moe;
+
+OG_API og_status og_int8_moe_create(og_device* device, og_int8_moe** out);
+/* Waits for the device, releases the instance's workspace. */
+OG_API og_status og_int8_moe_destroy(og_int8_moe* moe);
+/* The kernel the last encode call recorded: "portable" or "none". */
+OG_API og_status og_int8_moe_last_kernel(og_int8_moe* moe, char* buffer, uint64_t capacity);
+/* x, y and residual are float32 or float16 (one type), [tokens][model_size]; router float32 or float16,
+ * [experts][model_size]; w_in int8 [experts][(gated ? 2 : 1) * expert_size][model_size] and w_out int8
+ * [experts][model_size][expert_size], a float32 scale per row of each; expert_ids int32 and expert_weights float32,
+ * [tokens][top_k] by falling p, receive the routing. residual, expert_ids and expert_weights may be NULL; y may be x,
+ * and residual may be y or x (the same elements). */
+OG_API og_status og_int8_moe_encode(og_int8_moe* moe, og_encoder* encoder, const og_moe_problem* problem,
+                                    const og_buffer* x, const og_buffer* router, const og_buffer* w_in,
+                                    const og_buffer* w_in_scale, const og_buffer* w_out, const og_buffer* w_out_scale,
+                                    const og_buffer* y, const og_buffer* residual, const og_buffer* expert_ids,
+                                    const og_buffer* expert_weights);
+/* Its argument checks alone (no device needed). */
+OG_API og_status og_int8_moe_check(const og_moe_problem* problem, const og_buffer* x, const og_buffer* router,
+                                   const og_buffer* w_in, const og_buffer* w_in_scale, const og_buffer* w_out,
+                                   const og_buffer* w_out_scale, const og_buffer* y, const og_buffer* residual,
+                                   const og_buffer* expert_ids, const og_buffer* expert_weights);
+
 /* ---- ConvIntegerKernels (src/RecursiveAI.OneGpu.Kernels/ConvIntegerKernels.cs:25-351) --------------------------- */
 
 /* ConvProblem (src/RecursiveAI.OneGpu.Kernels/ConvProblem.cs): NCHW input, OIHW weights, strides, dilations,

@@ -33,6 +33,14 @@ internal struct OgConvProblem                                                   
 }
 
 [StructLayout(LayoutKind.Sequential)]
+internal struct OgMoeProblem                                                                   // og_moe_problem
+{
+    public int Tokens, ModelSize, ExpertSize, Experts, TopK, Activation, Gated, Normalize;
+    public int OffsetX, OffsetRouter, OffsetIn, OffsetInScale, OffsetOut, OffsetOutScale, OffsetY;
+    public int OffsetResidual, OffsetIds, OffsetWeights;
+}
+
+[StructLayout(LayoutKind.Sequential)]
 internal unsafe struct OgErrorInfo                                                             // og_error_info
 {
     public int Status;
@@ -157,6 +165,16 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int og_dequantize_check_quantize(OgBuffer* x, int offsetX,
         int* shape, int rank, int axis, int perAxis, OgBuffer* scale, int offsetScale, OgBuffer* zeroPoint,
         int offsetZeroPoint, OgBuffer* output, int offsetOutput);
+
+    [LibraryImport(Lib)] internal static partial int og_int8_moe_create(nint device, nint* moe);
+    [LibraryImport(Lib)] internal static partial int og_int8_moe_destroy(nint moe);
+    [LibraryImport(Lib)] internal static partial int og_int8_moe_last_kernel(nint moe, byte* buffer, ulong capacity);
+    [LibraryImport(Lib)] internal static partial int og_int8_moe_encode(nint moe, nint encoder, OgMoeProblem* p,
+        OgBuffer* x, OgBuffer* router, OgBuffer* wIn, OgBuffer* wInScale, OgBuffer* wOut, OgBuffer* wOutScale, OgBuffer* y,
+        OgBuffer* residual, OgBuffer* expertIds, OgBuffer* expertWeights);
+    [LibraryImport(Lib)] internal static partial int og_int8_moe_check(OgMoeProblem* p, OgBuffer* x, OgBuffer* router,
+        OgBuffer* wIn, OgBuffer* wInScale, OgBuffer* wOut, OgBuffer* wOutScale, OgBuffer* y, OgBuffer* residual,
+        OgBuffer* expertIds, OgBuffer* expertWeights);
 
     [LibraryImport(Lib)] internal static partial int og_conv_integer_create(nint device, OgOptions* options, nint* conv);
     [LibraryImport(Lib)] internal static partial int og_conv_integer_destroy(nint conv);

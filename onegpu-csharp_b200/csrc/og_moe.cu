@@ -1,0 +1,381 @@
+// A whole mixture-of-experts layer for a few tokens on int8 weights, with its argument checks and C ABI.
+//
+//   logits[t][e] = sum_d x[t][d] router[e][d],  p = softmax over the experts
+//   the top_k experts of a token by p (ties to the lowest index), w = p, or p / (sum of the chosen p) when normalized
+//   u = scale_in[e][j] sum_d w_in[e][j][d] x[t][d];   h[j] = activation(u[j]) u[F + j]  (gated), activation(u[j])
+//   y[t][d] = residual[t][d] + sum over the chosen e of w_e scale_out[e][d] sum_j w_out[e][d][j] h[j]
+//
+// Everything is accumulated in float32; the activations are not quantized. A NaN logit ranks below every number.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "og_act.cuh"
+#include "og_gemm.h"
+#include "og_host.h"
+#include "og_moe.h"
+#include "og_ptx.cuh"
+
+namespace og {
+
+__device__ __forceinline__ float moe_value(const void* p, int half, int64_t i) {
+    return half ? __half2float(__ldg(static_cast<const __half*>(p) + i)) : __ldg(static_cast<const float*>(p) + i);
+}
+
+__device__ __forceinline__ float moe_warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+// The top_k experts of one token by a warp: logits in shared memory (NaN already replaced by -infinity for the
+// ranking; `sum` is the softmax's denominator over the true logits, `top` its maximum). Each round takes the largest
+// remaining logit, the lowest index among equals.
+__device__ __forceinline__ void moe_top_k(float* rank, const MoeLaunch& L, int t, float top, float sum) {
+    const int lane = threadIdx.x & 31;
+    float chosen_sum = 0.0f;
+    float weight = 0.0f;  // lane k: the k-th chosen weight
+    int id = 0;
+    for (int k = 0; k < L.top_k; k++) {
+        float best = -INFINITY;
+        int at = MOE_MAX_EXPERTS;
+        for (int e = lane; e < L.experts; e += 32)
+            if (rank[e] > best || (at == MOE_MAX_EXPERTS && rank[e] == best)) {
+                // strictly larger, or the first candidate of this lane (a taken expert is NaN and never compares)
+                best = rank[e];
+                at = e;
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float b2 = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+            const int a2 = __shfl_xor_sync(0xFFFFFFFFu, at, o);
+            if (b2 > best || (b2 == best && a2 < at)) {
+                best = b2;
+                at = a2;
+            }
+        }
+        const float w = expf(best - top) / sum;
+        chosen_sum += w;
+        if (lane == k) {
+            weight = w;
+            id = at;
+        }
+        if (lane == 0) rank[at] = NAN;
+        __syncwarp();
+    }
+    if (lane < L.top_k) {
+        if (L.normalize) weight = weight / chosen_sum;
+        const int i = t * L.top_k + lane;
+        L.ids[i] = id;
+        L.weights[i] = weight;
+        if (L.ids_out != nullptr) L.ids_out[i] = id;
+        if (L.weights_out != nullptr) L.weights_out[i] = weight;
+    }
+}
+
+// Portable kernels: any sizes and alignment.
+
+// One block per token: its logits (a warp per expert), then the softmax and the top k.
+__global__ void __launch_bounds__(256) moe_router_kernel(const MoeLaunch L) {
+    __shared__ float logits[MOE_MAX_EXPERTS];
+    __shared__ float rank[MOE_MAX_EXPERTS];
+    pdl_trigger();
+    pdl_wait();
+    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int e = warp; e < L.experts; e += 8) {
+        double sum = 0.0;
+        for (int d = lane; d < L.model; d += 32)
+            sum += static_cast<double>(moe_value(L.x, L.x_half, static_cast<int64_t>(t) * L.model + d)) *
+                   moe_value(L.router, L.router_half, static_cast<int64_t>(e) * L.model + d);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (lane == 0) {
+            logits[e] = static_cast<float>(sum);
+            rank[e] = isnan(logits[e]) ? -INFINITY : logits[e];
+        }
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    float top = -INFINITY;
+    bool nan = false;
+    for (int e = lane; e < L.experts; e += 32) {
+        nan |= isnan(logits[e]);
+        top = fmaxf(top, logits[e]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (__any_sync(0xFFFFFFFFu, nan)) top = NAN;  // the softmax of a row with a NaN is NaN
+    float sum = 0.0f;
+    for (int e = lane; e < L.experts; e += 32) sum += expf(logits[e] - top);
+    moe_top_k(rank, L, t, top, moe_warp_sum(sum));
+}
+
+// One warp per (token, choice, hidden unit).
+__global__ void __launch_bounds__(256) moe_up_kernel(const MoeLaunch L) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    if (unit >= static_cast<int64_t>(L.tokens) * L.top_k * L.expert) return;
+    const int pair = static_cast<int>(unit / L.expert), j = static_cast<int>(unit % L.expert);
+    const int t = pair / L.top_k, e = __ldcg(L.ids + pair);
+    const int64_t rows = static_cast<int64_t>(L.gated ? 2 : 1) * L.expert;
+    float u[2] = {0.0f, 0.0f};
+    for (int g = 0; g < (L.gated ? 2 : 1); g++) {
+        const int64_t row = e * rows + static_cast<int64_t>(g) * L.expert + j;
+        const int8_t* w = L.w_in + row * L.model;
+        float sum = 0.0f;
+        for (int d = lane; d < L.model; d += 32)
+            sum = fmaf(static_cast<float>(__ldg(w + d)), moe_value(L.x, L.x_half, static_cast<int64_t>(t) * L.model + d),
+                       sum);
+        u[g] = moe_warp_sum(sum) * __ldg(L.in_scale + row);
+    }
+    if (lane != 0) return;
+    float h[1] = {u[0]};
+    activate_all(h, L.activation);
+    L.hidden[unit] = L.gated ? h[0] * u[1] : h[0];
+}
+
+// One warp per (token, output).
+__global__ void __launch_bounds__(256) moe_down_kernel(const MoeLaunch L) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    if (unit >= static_cast<int64_t>(L.tokens) * L.model) return;
+    const int t = static_cast<int>(unit / L.model), d = static_cast<int>(unit % L.model);
+    float out = 0.0f;
+    for (int k = 0; k < L.top_k; k++) {
+        const int pair = t * L.top_k + k;
+        const int64_t row = static_cast<int64_t>(__ldcg(L.ids + pair)) * L.model + d;
+        const int8_t* w = L.w_out + row * L.expert;
+        const float* h = L.hidden + static_cast<int64_t>(pair) * L.expert;
+        float sum = 0.0f;
+        for (int j = lane; j < L.expert; j += 32) sum = fmaf(static_cast<float>(__ldg(w + j)), __ldcg(h + j), sum);
+        out = fmaf(__ldcg(L.weights + pair), moe_warp_sum(sum) * __ldg(L.out_scale + row), out);
+    }
+    if (lane != 0) return;
+    if (L.x_half) {
+        if (L.residual != nullptr) out += __half2float(static_cast<const __half*>(L.residual)[unit]);
+        static_cast<__half*>(L.y)[unit] = __float2half_rn(out);
+    } else {
+        if (L.residual != nullptr) out += static_cast<const float*>(L.residual)[unit];
+        static_cast<float*>(L.y)[unit] = out;
+    }
+}
+
+static cudaError_t launch_moe_portable(const MoeLaunch& L, cudaStream_t s) {
+    cudaError_t e = launch_pdl(moe_router_kernel, dim3(L.tokens), dim3(256), 0, s, L);
+    if (e != cudaSuccess) return e;
+    const int64_t up = static_cast<int64_t>(L.tokens) * L.top_k * L.expert, down = static_cast<int64_t>(L.tokens) * L.model;
+    e = launch_pdl(moe_up_kernel, dim3(static_cast<unsigned>((up + 7) / 8)), dim3(256), 0, s, L);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(moe_down_kernel, dim3(static_cast<unsigned>((down + 7) / 8)), dim3(256), 0, s, L);
+}
+
+}  // namespace og
+
+// ---- host layer ------------------------------------------------------------------------------------------------------
+
+using namespace og_host;
+
+struct og_int8_moe {
+    og_device* device = nullptr;
+    std::string last = "none";
+    std::vector<void*> buffers;  // workspaces, the latest last; older ones live until destroy (recorded work names them)
+    int64_t bytes = 0;
+};
+
+namespace {
+
+const char* kMoe = "Int8Moe";
+
+void require_float(const og_buffer* b, const char* arg) {
+    if (b->type != OG_F32 && b->type != OG_F16)
+        shape(kMoe, arg, std::string("element type ") + type_name(b->type) + " is not supported; use Single or Half");
+}
+
+void require(const og_buffer* b, const char* arg, int32_t type) {
+    if (b->type != type)
+        shape(kMoe, arg, std::string("element type ") + type_name(b->type) + " is not supported; use " + type_name(type));
+}
+
+void between(const char* arg, int32_t v, int32_t low, int32_t high) {
+    if (v < low || v > high)
+        shape(kMoe, arg, std::to_string(v) + " is outside " + std::to_string(low) + ".." + std::to_string(high));
+}
+
+void need(const og_buffer* b, const char* arg) {
+    if (b == nullptr || b->ptr == nullptr) null_arg(kMoe, arg);
+}
+
+template <class T>
+T* at(const og_buffer* b, int32_t offset) {
+    return reinterpret_cast<T*>(static_cast<uint8_t*>(b->ptr) + static_cast<int64_t>(offset) * elem_size(b->type));
+}
+
+// The checks; false when there is nothing to do (no tokens).
+bool check_moe(const og_moe_problem* p, const og_buffer* x, const og_buffer* router, const og_buffer* w_in,
+               const og_buffer* w_in_scale, const og_buffer* w_out, const og_buffer* w_out_scale, const og_buffer* y,
+               const og_buffer* residual, const og_buffer* ids, const og_buffer* weights) {
+    need(x, "x");
+    need(router, "router");
+    need(w_in, "wIn");
+    need(w_in_scale, "wInScale");
+    need(w_out, "wOut");
+    need(w_out_scale, "wOutScale");
+    need(y, "y");
+    if (p == nullptr) null_arg(kMoe, "problem");
+    require_float(x, "x");
+    require_float(router, "router");
+    require(w_in, "wIn", OG_S8);
+    require(w_in_scale, "wInScale", OG_F32);
+    require(w_out, "wOut", OG_S8);
+    require(w_out_scale, "wOutScale", OG_F32);
+    require(y, "y", x->type);
+    between("Tokens", p->tokens, 0, og::MOE_MAX_TOKENS);
+    between("ModelSize", p->model_size, 1, og::MOE_MAX_SIZE);
+    between("ExpertSize", p->expert_size, 1, og::MOE_MAX_SIZE);
+    between("Experts", p->experts, 1, og::MOE_MAX_EXPERTS);
+    between("TopK", p->top_k, 1, std::min(p->experts, og::MOE_MAX_TOP_K));
+    between("Activation", p->activation, OG_ACTIVATION_NONE, OG_ACTIVATION_SILU);
+    const int64_t t = p->tokens, d = p->model_size, e = p->experts;
+    const int64_t up = static_cast<int64_t>(p->gated ? 2 : 1) * p->expert_size, f = p->expert_size;
+    range(kMoe, "x", x->length, p->offset_x, t * d);
+    range(kMoe, "router", router->length, p->offset_router, e * d);
+    range(kMoe, "wIn", w_in->length, p->offset_in, e * up * d);
+    range(kMoe, "wInScale", w_in_scale->length, p->offset_in_scale, e * up);
+    range(kMoe, "wOut", w_out->length, p->offset_out, e * d * f);
+    range(kMoe, "wOutScale", w_out_scale->length, p->offset_out_scale, e * d);
+    range(kMoe, "y", y->length, p->offset_y, t * d);
+    if (residual != nullptr) {
+        need(residual, "residual");
+        require(residual, "residual", y->type);
+        range(kMoe, "residual", residual->length, p->offset_residual, t * d);
+        const uint8_t* r0 = at<uint8_t>(residual, p->offset_residual);
+        const uint8_t* y0 = at<uint8_t>(y, p->offset_y);
+        const int64_t bytes = t * d * elem_size(y->type);
+        if (r0 != y0 && r0 < y0 + bytes && y0 < r0 + bytes)
+            shape(kMoe, "residual", "overlaps y without being the same elements");
+    }
+    if (ids != nullptr) {
+        need(ids, "expertIds");
+        require(ids, "expertIds", OG_I32);
+        range(kMoe, "expertIds", ids->length, p->offset_ids, t * p->top_k);
+    }
+    if (weights != nullptr) {
+        need(weights, "expertWeights");
+        require(weights, "expertWeights", OG_F32);
+        range(kMoe, "expertWeights", weights->length, p->offset_weights, t * p->top_k);
+    }
+    return p->tokens > 0;
+}
+
+int64_t round256(int64_t v) { return (v + 255) & ~int64_t(255); }
+
+// Carves the layer's workspace out of the instance's, growing it geometrically.
+void bind_workspace(og_int8_moe* m, og::MoeLaunch& L) {
+    const int64_t pairs = static_cast<int64_t>(L.tokens) * L.top_k;
+    const int64_t ids = round256(pairs * 4), weights = round256(pairs * 4), hidden = round256(pairs * L.expert * 4);
+    const int64_t bytes = ids + weights + hidden;
+    if (m->bytes < bytes) {
+        const int64_t len = std::max(bytes, std::max<int64_t>(int64_t(1) << 20, 2 * m->bytes));
+        void* p = nullptr;
+        check_cuda(cudaMalloc(&p, static_cast<size_t>(len)), "Int8Moe workspace");
+        m->buffers.push_back(p);
+        m->bytes = len;
+    }
+    uint8_t* base = static_cast<uint8_t*>(m->buffers.back());
+    L.ids = reinterpret_cast<int32_t*>(base);
+    L.weights = reinterpret_cast<float*>(base + ids);
+    L.hidden = reinterpret_cast<float*>(base + ids + weights);
+}
+
+}  // namespace
+
+extern "C" {
+
+OG_API og_status og_int8_moe_create(og_device* d, og_int8_moe** out) {
+    return guard([&] {
+        if (d == nullptr) null_arg(kMoe, "device");
+        if (out == nullptr) null_arg(kMoe, "out");
+        auto* m = new og_int8_moe();
+        m->device = d;
+        *out = m;
+    });
+}
+
+OG_API og_status og_int8_moe_destroy(og_int8_moe* m) {
+    return guard([&] {
+        if (m == nullptr) return;
+        use(m->device);
+        cudaStreamSynchronize(m->device->stream);
+        for (void* p : m->buffers) cudaFree(p);
+        delete m;
+    });
+}
+
+OG_API og_status og_int8_moe_last_kernel(og_int8_moe* m, char* buffer, uint64_t capacity) {
+    return guard([&] {
+        if (m == nullptr) throw OgError{OG_ERROR_INVALID_HANDLE, kMoe, "moe", "null handle", "", "", ""};
+        if (buffer == nullptr || capacity == 0) return;
+        const size_t n = std::min(static_cast<size_t>(capacity) - 1, m->last.size());
+        m->last.copy(buffer, n);
+        buffer[n] = 0;
+    });
+}
+
+OG_API og_status og_int8_moe_check(const og_moe_problem* p, const og_buffer* x, const og_buffer* router,
+                                   const og_buffer* w_in, const og_buffer* w_in_scale, const og_buffer* w_out,
+                                   const og_buffer* w_out_scale, const og_buffer* y, const og_buffer* residual,
+                                   const og_buffer* ids, const og_buffer* weights) {
+    return guard([&] { check_moe(p, x, router, w_in, w_in_scale, w_out, w_out_scale, y, residual, ids, weights); });
+}
+
+OG_API og_status og_int8_moe_encode(og_int8_moe* m, og_encoder* enc, const og_moe_problem* p, const og_buffer* x,
+                                    const og_buffer* router, const og_buffer* w_in, const og_buffer* w_in_scale,
+                                    const og_buffer* w_out, const og_buffer* w_out_scale, const og_buffer* y,
+                                    const og_buffer* residual, const og_buffer* ids, const og_buffer* weights) {
+    return guard([&] {
+        if (m == nullptr) throw OgError{OG_ERROR_INVALID_HANDLE, kMoe, "moe", "null handle", "", "", ""};
+        if (enc == nullptr) null_arg(kMoe, "encoder");
+        if (enc->device != m->device)
+            throw OgError{OG_ERROR_INVALID_HANDLE, kMoe, "encoder", "the encoder belongs to another device", "", "", ""};
+        if (!check_moe(p, x, router, w_in, w_in_scale, w_out, w_out_scale, y, residual, ids, weights)) {
+            m->last = "none";
+            return;
+        }
+        use(m->device);
+        og::MoeLaunch L = {};
+        L.tokens = p->tokens;
+        L.model = p->model_size;
+        L.expert = p->expert_size;
+        L.experts = p->experts;
+        L.top_k = p->top_k;
+        L.activation = p->activation;
+        L.gated = p->gated != 0;
+        L.normalize = p->normalize != 0;
+        L.x_half = x->type == OG_F16;
+        L.router_half = router->type == OG_F16;
+        L.x = at<void>(x, p->offset_x);
+        L.router = at<void>(router, p->offset_router);
+        L.w_in = at<int8_t>(w_in, p->offset_in);
+        L.in_scale = at<float>(w_in_scale, p->offset_in_scale);
+        L.w_out = at<int8_t>(w_out, p->offset_out);
+        L.out_scale = at<float>(w_out_scale, p->offset_out_scale);
+        L.y = at<void>(y, p->offset_y);
+        L.residual = residual != nullptr ? at<void>(residual, p->offset_residual) : nullptr;
+        L.ids_out = ids != nullptr ? at<int32_t>(ids, p->offset_ids) : nullptr;
+        L.weights_out = weights != nullptr ? at<float>(weights, p->offset_weights) : nullptr;
+        bind_workspace(m, L);
+        m->last = "portable";
+        enc->ops.push_back([L](cudaStream_t s) { return og::launch_moe_portable(L, s); });
+        enc->dispatches += 3;
+    });
+}
+
+}  // extern "C"

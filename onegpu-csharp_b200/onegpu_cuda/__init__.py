@@ -163,6 +163,11 @@ EXPORTS = {
     "og_dequantize_encode_quantize": [_P, _P] + _QUANT_ARGS,
     "og_dequantize_check": _QUANT_ARGS,
     "og_dequantize_check_quantize": _QUANT_ARGS,
+    "og_int8_moe_create": [_P, _PP],
+    "og_int8_moe_destroy": [_P],
+    "og_int8_moe_last_kernel": [_P, ctypes.c_char_p, ctypes.c_uint64],
+    "og_int8_moe_encode": [_P, _P, _P] + [_BUF] * 10,
+    "og_int8_moe_check": [_P] + [_BUF] * 10,
     "og_conv_integer_create": [_P, _P, _PP],
     "og_conv_integer_destroy": [_P],
     "og_conv_integer_variant": [_P, ctypes.c_char_p, ctypes.c_uint64],
@@ -1019,6 +1024,90 @@ class ConvIntegerKernels:
     def dispose(self) -> None:
         if self.handle:
             _check(_lib.og_conv_integer_destroy(self.handle))
+            self.handle = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.dispose()
+
+
+# ---- Int8MoeKernels ---------------------------------------------------------------------------------------------------
+
+class og_moe_problem(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in
+                ("tokens", "model_size", "expert_size", "experts", "top_k", "activation", "gated", "normalize", "offset_x",
+                 "offset_router", "offset_in", "offset_in_scale", "offset_out", "offset_out_scale", "offset_y",
+                 "offset_residual", "offset_ids", "offset_weights")]
+
+
+@dataclass
+class MoeProblem:
+    """og_moe_problem: a mixture-of-experts layer for up to 128 tokens, offsets in elements. `gated`: the hidden values
+    are activation(first half) * second half of the expert's input product; `normalize`: the chosen experts' weights sum
+    to one."""
+    tokens: int
+    model_size: int
+    expert_size: int
+    experts: int
+    top_k: int
+    activation: int = ACTIVATION_SILU
+    gated: bool = True
+    normalize: bool = True
+    offset_x: int = 0
+    offset_router: int = 0
+    offset_in: int = 0
+    offset_in_scale: int = 0
+    offset_out: int = 0
+    offset_out_scale: int = 0
+    offset_y: int = 0
+    offset_residual: int = 0
+    offset_ids: int = 0
+    offset_weights: int = 0
+
+    def c_struct(self) -> og_moe_problem:
+        return og_moe_problem(*[int(getattr(self, name)) for name, _ in og_moe_problem._fields_])
+
+
+def check_moe(problem: MoeProblem, x, router, w_in, w_in_scale, w_out, w_out_scale, y, residual=None, expert_ids=None,
+              expert_weights=None) -> None:
+    """The argument checks of Int8MoeKernels.encode alone (no device needed)."""
+    p = problem.c_struct()
+    _check(_lib.og_int8_moe_check(ctypes.byref(p), _buf(x), _buf(router), _buf(w_in), _buf(w_in_scale), _buf(w_out),
+                                  _buf(w_out_scale), _buf(y), _buf(residual), _buf(expert_ids), _buf(expert_weights)))
+
+
+class Int8MoeKernels:
+    """A whole mixture-of-experts layer for a few tokens on int8 weights: the router, the choice of each token's experts,
+    their feed-forward products and the weighted sum. No counterpart in the reference."""
+
+    def __init__(self, device: GpuDevice):
+        self.device = device
+        h = ctypes.c_void_p()
+        _check(_lib.og_int8_moe_create(device.handle, ctypes.byref(h)))
+        self.handle = h.value
+
+    @property
+    def last_kernel(self) -> str:
+        s = ctypes.create_string_buffer(64)
+        _check(_lib.og_int8_moe_last_kernel(self.handle, s, 64))
+        return s.value.decode()
+
+    def encode(self, encoder: GpuCommandEncoder, problem: MoeProblem, x: GpuBuffer, router: GpuBuffer, w_in: GpuBuffer,
+               w_in_scale: GpuBuffer, w_out: GpuBuffer, w_out_scale: GpuBuffer, y: GpuBuffer,
+               residual: Optional[GpuBuffer] = None, expert_ids: Optional[GpuBuffer] = None,
+               expert_weights: Optional[GpuBuffer] = None) -> None:
+        p = problem.c_struct()
+        _check(_lib.og_int8_moe_encode(self.handle, encoder.handle if encoder else None, ctypes.byref(p), _buf(x),
+                                       _buf(router), _buf(w_in), _buf(w_in_scale), _buf(w_out), _buf(w_out_scale),
+                                       _buf(y), _buf(residual), _buf(expert_ids), _buf(expert_weights)))
+
+    Encode = encode
+
+    def dispose(self) -> None:
+        if self.handle:
+            _check(_lib.og_int8_moe_destroy(self.handle))
             self.handle = None
 
     def __enter__(self):

@@ -75,3 +75,54 @@ def test_quantize_rows():
     assert argument_of(chk, x, 0, 5, 8, 0, y, 0, s, 1, z, 0) == (shape, "scale")
     assert argument_of(chk, x, 0, 5, 8, 0, y, 0, s, 0, z, 1) == (shape, "zeroPoint")
     assert argument_of(chk, x, 0, 65536, 65536, 0, y, 0, s, 0, z, 0) == (shape, "rows")
+
+
+def _moe(**change):
+    """Buffers of a small layer (5 tokens of 8, 4 experts of 6, 2 chosen), some of them replaced."""
+    b = dict(x=spec(F16, 40), router=spec(F32, 32), w_in=spec(S8, 4 * 12 * 8), w_in_scale=spec(F32, 48),
+             w_out=spec(S8, 4 * 8 * 6), w_out_scale=spec(F32, 32), y=og._BufferSpec(F16, 48, 0x9000))
+    b.update(change)
+    return b
+
+
+def test_moe():
+    chk, M = og.check_moe, og.MoeProblem
+    p = M(5, 8, 6, 4, 2)
+    chk(p, **_moe())
+    chk(p, **_moe(residual=_moe()["y"], expert_ids=spec(I32, 10), expert_weights=spec(F32, 10), router=spec(F16, 32)))
+    chk(p, **_moe(residual=_moe()["x"], y=_moe()["x"]))
+    chk(M(0, 8, 6, 4, 2), **_moe())
+    chk(M(5, 8, 12, 4, 2, gated=False, offset_y=8), **_moe(w_out=spec(S8, 384)))
+    chk(M(5, 8, 6, 4, 4), **_moe())
+    names = dict(x="x", router="router", w_in="wIn", w_in_scale="wInScale", w_out="wOut", w_out_scale="wOutScale", y="y")
+    for key, name in names.items():
+        assert argument_of(chk, p, **_moe(**{key: None})) == (null, name)
+        full = _moe()[key]
+        assert argument_of(chk, p, **_moe(**{key: spec(np.int16, full.length)})) == (shape, name)
+        short = {"y": 39}.get(key, full.length - 1)
+        assert argument_of(chk, p, **_moe(**{key: spec(full.dtype, short)})) == (shape, name)
+    assert argument_of(chk, p, **_moe(y=spec(F32, 40))) == (shape, "y")
+    assert argument_of(chk, p, **_moe(w_in=spec(U8, 384))) == (shape, "wIn")
+    for bad, name in [(M(-1, 8, 6, 4, 2), "Tokens"), (M(129, 8, 6, 4, 2), "Tokens"), (M(5, 0, 6, 4, 2), "ModelSize"),
+                      (M(5, 65537, 6, 4, 2), "ModelSize"), (M(5, 8, 0, 4, 2), "ExpertSize"),
+                      (M(5, 8, 65537, 4, 2), "ExpertSize"), (M(5, 8, 6, 0, 1), "Experts"),
+                      (M(5, 8, 6, 513, 2), "Experts"), (M(5, 8, 6, 4, 0), "TopK"), (M(5, 8, 6, 4, 5), "TopK"),
+                      (M(5, 8, 6, 100, 17), "TopK"), (M(5, 8, 6, 4, 2, activation=5), "Activation"),
+                      (M(5, 8, 6, 4, 2, activation=-1), "Activation")]:
+        assert argument_of(chk, bad, **_moe()) == (shape, name)
+    for field, name in [("offset_x", "x"), ("offset_router", "router"), ("offset_in", "wIn"),
+                        ("offset_in_scale", "wInScale"), ("offset_out", "wOut"), ("offset_out_scale", "wOutScale"),
+                        ("offset_y", "y")]:
+        assert argument_of(chk, M(5, 8, 6, 4, 2, **{field: 9}), **_moe()) == (shape, name)
+        assert argument_of(chk, M(5, 8, 6, 4, 2, **{field: -1}), **_moe()) == (shape, name + "Offset")
+    far = og._BufferSpec(F16, 48, 0x20000)
+    chk(M(5, 8, 6, 4, 2, offset_residual=8), **_moe(residual=far))
+    assert argument_of(chk, M(5, 8, 6, 4, 2, offset_residual=9), **_moe(residual=far)) == (shape, "residual")
+    assert argument_of(chk, p, **_moe(residual=spec(F32, 40))) == (shape, "residual")
+    assert argument_of(chk, p, **_moe(residual=spec(F16, 40, null=True))) == (null, "residual")
+    assert argument_of(chk, M(5, 8, 6, 4, 2, offset_residual=1), **_moe(residual=_moe()["y"])) == (shape, "residual")
+    assert argument_of(chk, p, **_moe(expert_ids=spec(F32, 10))) == (shape, "expertIds")
+    assert argument_of(chk, p, **_moe(expert_ids=spec(I32, 9))) == (shape, "expertIds")
+    assert argument_of(chk, p, **_moe(expert_weights=spec(F16, 10))) == (shape, "expertWeights")
+    assert argument_of(chk, M(5, 8, 6, 4, 2, offset_weights=1), **_moe(expert_weights=spec(F32, 10))) == (
+        shape, "expertWeights")
