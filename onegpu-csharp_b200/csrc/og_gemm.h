@@ -96,9 +96,9 @@ int64_t rows_part_ints(const GemmLaunch& L, int workers);
 int64_t rows_tickets(const GemmLaunch& L);
 cudaError_t launch_gemm_rows(const GemmLaunch& L, cudaStream_t stream);
 
-// A 3-D byte tensor map (x innermost) with 128-byte swizzled box_x x box_y boxes (og_gemm_tc.cu).
+// A 3-D byte tensor map (x innermost) with 128-byte swizzled box_x x box_y x box_z boxes (og_gemm_tc.cu).
 bool make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t x, uint64_t y, uint64_t z, uint64_t stride_y,
-                        uint64_t stride_z, uint32_t box_x, uint32_t box_y);
+                        uint64_t stride_z, uint32_t box_x, uint32_t box_y, uint32_t box_z = 1);
 
 // Portable SIMT product (og_gemm_simt.cu): any alignment, subtracts the zero points while staging, so it needs no
 // byte sums; its epilogue ignores row_sum_a / col_sum_b.

@@ -699,9 +699,6 @@ done:
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-bool make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t x, uint64_t y, uint64_t z, uint64_t stride_y,
-                        uint64_t stride_z, uint32_t box_x, uint32_t box_y);
-
 bool rows_eligible(const GemmLaunch& L) {
     return L.m >= 1 && L.m <= rows::MAXM && L.batch <= 65535 && tc_eligible(L);
 }

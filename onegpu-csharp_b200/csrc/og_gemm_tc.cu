@@ -956,14 +956,14 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// A 3-D byte tensor (x innermost) with 128-byte swizzled boxes of box_x x box_y.
+// A 3-D byte tensor (x innermost) with 128-byte swizzled boxes of box_x x box_y x box_z.
 static bool make_map(CUtensorMap* map, const void* base, uint64_t x, uint64_t y, uint64_t z, uint64_t stride_y,
-                     uint64_t stride_z, uint32_t box_x, uint32_t box_y) {
+                     uint64_t stride_z, uint32_t box_x, uint32_t box_y, uint32_t box_z = 1) {
     auto fn = encode_fn();
     if (fn == nullptr) return false;
     cuuint64_t dims[3] = {x, y, z};
     cuuint64_t strides[2] = {stride_y, stride_z};
-    cuuint32_t box[3] = {box_x, box_y, 1};
+    cuuint32_t box[3] = {box_x, box_y, box_z};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -987,8 +987,8 @@ static bool make_store_map(CUtensorMap* map, void* base, uint64_t n, uint64_t m,
 }
 
 bool make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t x, uint64_t y, uint64_t z, uint64_t stride_y,
-                        uint64_t stride_z, uint32_t box_x, uint32_t box_y) {
-    return make_map(map, base, x, y, z, stride_y, stride_z, box_x, box_y);
+                        uint64_t stride_z, uint32_t box_x, uint32_t box_y, uint32_t box_z) {
+    return make_map(map, base, x, y, z, stride_y, stride_z, box_x, box_y, box_z);
 }
 
 static uint64_t round16(uint64_t v) { return (v + 15) & ~uint64_t(15); }

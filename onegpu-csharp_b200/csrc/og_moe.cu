@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(256) moe_down_kernel(const MoeLaunch L) {
     }
 }
 
-static cudaError_t launch_moe_portable(const MoeLaunch& L, cudaStream_t s) {
+cudaError_t launch_moe_portable(const MoeLaunch& L, cudaStream_t s) {
     cudaError_t e = launch_pdl(moe_router_kernel, dim3(L.tokens), dim3(256), 0, s, L);
     if (e != cudaSuccess) return e;
     const int64_t up = static_cast<int64_t>(L.tokens) * L.top_k * L.expert, down = static_cast<int64_t>(L.tokens) * L.model;
@@ -188,6 +188,7 @@ struct og_int8_moe {
     std::string last = "none";
     std::vector<void*> buffers;  // workspaces, the latest last; older ones live until destroy (recorded work names them)
     int64_t bytes = 0;
+    unsigned long long* arrivals = nullptr;  // the fused kernel's grid barrier
 };
 
 namespace {
@@ -277,22 +278,36 @@ bool check_moe(const og_moe_problem* p, const og_buffer* x, const og_buffer* rou
 
 int64_t round256(int64_t v) { return (v + 255) & ~int64_t(255); }
 
-// Carves the layer's workspace out of the instance's, growing it geometrically.
-void bind_workspace(og_int8_moe* m, og::MoeLaunch& L) {
+// Carves the layer's workspace out of the instance's, growing it geometrically. The portable kernels' part is always
+// there (the fused launch falls back to them).
+void bind_workspace(og_int8_moe* m, og::MoeLaunch& L, bool fused) {
     const int64_t pairs = static_cast<int64_t>(L.tokens) * L.top_k;
-    const int64_t ids = round256(pairs * 4), weights = round256(pairs * 4), hidden = round256(pairs * L.expert * 4);
-    const int64_t bytes = ids + weights + hidden;
-    if (m->bytes < bytes) {
-        const int64_t len = std::max(bytes, std::max<int64_t>(int64_t(1) << 20, 2 * m->bytes));
+    const og::MoeFusedSizes s = fused ? og::moe_fused_sizes(L) : og::MoeFusedSizes{};
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += round256(bytes);
+        return here;
+    };
+    const int64_t ids = take(pairs * 4), weights = take(pairs * 4), hidden = take(pairs * L.expert * 4);
+    const int64_t logits = take(s.logits), x = take(s.x_pieces), h = take(s.h_pieces), outputs = take(s.outputs);
+    const int64_t segments = take(s.segments);
+    if (m->bytes < at) {
+        const int64_t len = std::max(at, std::max<int64_t>(int64_t(1) << 20, 2 * m->bytes));
         void* p = nullptr;
         check_cuda(cudaMalloc(&p, static_cast<size_t>(len)), "Int8Moe workspace");
         m->buffers.push_back(p);
         m->bytes = len;
     }
     uint8_t* base = static_cast<uint8_t*>(m->buffers.back());
-    L.ids = reinterpret_cast<int32_t*>(base);
-    L.weights = reinterpret_cast<float*>(base + ids);
-    L.hidden = reinterpret_cast<float*>(base + ids + weights);
+    L.ids = reinterpret_cast<int32_t*>(base + ids);
+    L.weights = reinterpret_cast<float*>(base + weights);
+    L.hidden = reinterpret_cast<float*>(base + hidden);
+    L.logits = reinterpret_cast<float*>(base + logits);
+    L.x_pieces = base + x;
+    L.h_pieces = base + h;
+    L.outputs = reinterpret_cast<float*>(base + outputs);
+    L.segments = reinterpret_cast<float*>(base + segments);
 }
 
 }  // namespace
@@ -303,8 +318,15 @@ OG_API og_status og_int8_moe_create(og_device* d, og_int8_moe** out) {
     return guard([&] {
         if (d == nullptr) null_arg(kMoe, "device");
         if (out == nullptr) null_arg(kMoe, "out");
+        use(d);
+        void* p = nullptr;
+        check_cuda(cudaMalloc(&p, sizeof(unsigned long long)), "Int8Moe barrier");
+        const cudaError_t e = cudaMemset(p, 0, sizeof(unsigned long long));
+        if (e != cudaSuccess) cudaFree(p);
+        check_cuda(e, "Int8Moe barrier");
         auto* m = new og_int8_moe();
         m->device = d;
+        m->arrivals = static_cast<unsigned long long*>(p);
         *out = m;
     });
 }
@@ -315,6 +337,7 @@ OG_API og_status og_int8_moe_destroy(og_int8_moe* m) {
         use(m->device);
         cudaStreamSynchronize(m->device->stream);
         for (void* p : m->buffers) cudaFree(p);
+        cudaFree(m->arrivals);
         delete m;
     });
 }
@@ -371,7 +394,20 @@ OG_API og_status og_int8_moe_encode(og_int8_moe* m, og_encoder* enc, const og_mo
         L.residual = residual != nullptr ? at<void>(residual, p->offset_residual) : nullptr;
         L.ids_out = ids != nullptr ? at<int32_t>(ids, p->offset_ids) : nullptr;
         L.weights_out = weights != nullptr ? at<float>(weights, p->offset_weights) : nullptr;
-        bind_workspace(m, L);
+        L.arrivals = m->arrivals;
+        L.error_flag = m->device->status;
+        L.num_sms = m->device->sm_count;
+        const bool fused = og::moe_fused_eligible(L);
+        bind_workspace(m, L, fused);
+        if (fused) {
+            cudaError_t err;
+            auto fn = og::prepare_moe_fused(L, &err);  // tensor maps built now, at record time
+            check_cuda(err, "Int8Moe tensor maps");
+            m->last = "fused";
+            enc->ops.push_back(std::move(fn));
+            enc->dispatches += 1;
+            return;
+        }
         m->last = "portable";
         enc->ops.push_back([L](cudaStream_t s) { return og::launch_moe_portable(L, s); });
         enc->dispatches += 3;

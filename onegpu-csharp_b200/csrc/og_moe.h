@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <functional>
 
 namespace og {
 
@@ -33,6 +34,26 @@ struct MoeLaunch {
     int32_t* ids;    // [tokens][top_k]
     float* weights;  // [tokens][top_k]
     float* hidden;   // [tokens * top_k][expert]
+    // Fused kernel (og_moe_fused.cu).
+    float* logits;                 // [tokens][experts]
+    uint8_t* x_pieces;             // [tokens][chunks of model][pieces][128] 16-bit pieces of x
+    uint8_t* h_pieces;             // [tokens * top_k][chunks of expert][pieces][128] of the hidden values
+    float* outputs;                // [tokens * top_k][model] weighted outputs of the chosen experts
+    float* segments;               // partial sums of units cut between warps
+    unsigned long long* arrivals;  // grid barrier: arrivals of all launches so far
+    int* error_flag;
+    int num_sms;
 };
+
+// Whether the fused kernel can run the layer: weight rows on 16-byte boundaries (what TMA loads).
+bool moe_fused_eligible(const MoeLaunch& L);
+// The workspace sizes of the fused kernel, in bytes.
+struct MoeFusedSizes {
+    int64_t logits, x_pieces, h_pieces, outputs, segments;
+};
+MoeFusedSizes moe_fused_sizes(const MoeLaunch& L);
+// Builds the tensor maps; the returned launch runs the portable kernels when the device refuses the cooperative launch.
+std::function<cudaError_t(cudaStream_t)> prepare_moe_fused(const MoeLaunch& L, cudaError_t* err);
+cudaError_t launch_moe_portable(const MoeLaunch& L, cudaStream_t s);
 
 }  // namespace og
