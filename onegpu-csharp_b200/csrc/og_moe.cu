@@ -194,6 +194,8 @@ struct og_int8_moe {
 namespace {
 
 const char* kMoe = "Int8Moe";
+// The fused kernel's barrier count, then its tickets.
+constexpr size_t kBarrierBytes = sizeof(unsigned long long) + og::MOE_MAX_TOKENS / 8 * sizeof(unsigned int);
 
 void require_float(const og_buffer* b, const char* arg) {
     if (b->type != OG_F32 && b->type != OG_F16)
@@ -290,8 +292,8 @@ void bind_workspace(og_int8_moe* m, og::MoeLaunch& L, bool fused) {
         return here;
     };
     const int64_t ids = take(pairs * 4), weights = take(pairs * 4), hidden = take(pairs * L.expert * 4);
-    const int64_t logits = take(s.logits), x = take(s.x_pieces), h = take(s.h_pieces), outputs = take(s.outputs);
-    const int64_t segments = take(s.segments);
+    const int64_t logits = take(s.logits), x = take(s.x_digits), h = take(s.h_digits), outputs = take(s.outputs);
+    const int64_t x_most = take(s.x_most), h_most = take(s.h_most), segments = take(s.segments);
     if (m->bytes < at) {
         const int64_t len = std::max(at, std::max<int64_t>(int64_t(1) << 20, 2 * m->bytes));
         void* p = nullptr;
@@ -304,10 +306,12 @@ void bind_workspace(og_int8_moe* m, og::MoeLaunch& L, bool fused) {
     L.weights = reinterpret_cast<float*>(base + weights);
     L.hidden = reinterpret_cast<float*>(base + hidden);
     L.logits = reinterpret_cast<float*>(base + logits);
-    L.x_pieces = base + x;
-    L.h_pieces = base + h;
+    L.x_digits = base + x;
+    L.h_digits = base + h;
+    L.x_most = reinterpret_cast<uint32_t*>(base + x_most);
+    L.h_most = reinterpret_cast<uint32_t*>(base + h_most);
     L.outputs = reinterpret_cast<float*>(base + outputs);
-    L.segments = reinterpret_cast<float*>(base + segments);
+    L.segments = reinterpret_cast<long long*>(base + segments);
 }
 
 }  // namespace
@@ -320,8 +324,8 @@ OG_API og_status og_int8_moe_create(og_device* d, og_int8_moe** out) {
         if (out == nullptr) null_arg(kMoe, "out");
         use(d);
         void* p = nullptr;
-        check_cuda(cudaMalloc(&p, sizeof(unsigned long long)), "Int8Moe barrier");
-        const cudaError_t e = cudaMemset(p, 0, sizeof(unsigned long long));
+        check_cuda(cudaMalloc(&p, kBarrierBytes), "Int8Moe barrier");
+        const cudaError_t e = cudaMemset(p, 0, kBarrierBytes);
         if (e != cudaSuccess) cudaFree(p);
         check_cuda(e, "Int8Moe barrier");
         auto* m = new og_int8_moe();
@@ -395,6 +399,7 @@ OG_API og_status og_int8_moe_encode(og_int8_moe* m, og_encoder* enc, const og_mo
         L.ids_out = ids != nullptr ? at<int32_t>(ids, p->offset_ids) : nullptr;
         L.weights_out = weights != nullptr ? at<float>(weights, p->offset_weights) : nullptr;
         L.arrivals = m->arrivals;
+        L.tickets = reinterpret_cast<unsigned int*>(m->arrivals + 1);
         L.error_flag = m->device->status;
         L.num_sms = m->device->sm_count;
         const bool fused = og::moe_fused_eligible(L);

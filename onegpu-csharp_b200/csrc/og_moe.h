@@ -36,11 +36,14 @@ struct MoeLaunch {
     float* hidden;   // [tokens * top_k][expert]
     // Fused kernel (og_moe_fused.cu).
     float* logits;                 // [tokens][experts]
-    uint8_t* x_pieces;             // [tokens][chunks of model][pieces][128] 16-bit pieces of x
-    uint8_t* h_pieces;             // [tokens * top_k][chunks of expert][pieces][128] of the hidden values
+    uint8_t* x_digits;             // [tokens][chunks of model][digits][128] of x
+    uint8_t* h_digits;             // [tokens * top_k][chunks of expert][digits][128] of the hidden values
+    uint32_t* x_most;              // [tokens] the bits of a token's largest magnitude
+    uint32_t* h_most;              // [tokens * top_k] and of a pair's hidden values
     float* outputs;                // [tokens * top_k][model] weighted outputs of the chosen experts
-    float* segments;               // partial sums of units cut between warps
+    long long* segments;           // partial sums of units cut between warps
     unsigned long long* arrivals;  // grid barrier: arrivals of all launches so far
+    unsigned int* tickets;         // [MOE_MAX_TOKENS / 8] logits finished of each block of 8 tokens, 0 between launches
     int* error_flag;
     int num_sms;
 };
@@ -49,7 +52,7 @@ struct MoeLaunch {
 bool moe_fused_eligible(const MoeLaunch& L);
 // The workspace sizes of the fused kernel, in bytes.
 struct MoeFusedSizes {
-    int64_t logits, x_pieces, h_pieces, outputs, segments;
+    int64_t logits, x_digits, h_digits, x_most, h_most, outputs, segments;
 };
 MoeFusedSizes moe_fused_sizes(const MoeLaunch& L);
 // Builds the tensor maps; the returned launch runs the portable kernels when the device refuses the cooperative launch.

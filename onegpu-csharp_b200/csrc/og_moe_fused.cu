@@ -2,28 +2,33 @@
 //
 // For a few tokens the layer is bound by reading the touched experts' weights once (3 x model x expert bytes each when
 // gated), so everything is arranged around keeping those reads in flight:
-//  0. Router: logits (a CTA per expert and 8 tokens, its warps splitting the sum), and x rewritten as 16-bit pieces in
-//     the order the matrix instructions take them. Grid barrier.
-//     Every CTA then finds all tokens' experts itself (a warp per token) and sorts the (token, choice) pairs by expert
-//     into groups of one expert and up to 8 NT pairs: cheaper than another barrier.
+//  0. Router: logits (an expert and 8 tokens at a time, shared by warps of a CTA), and x rewritten as digits (below).
+//     Grid barrier. Every CTA then finds all tokens' experts itself, a warp per token: cheaper than another barrier; of more
+//     tokens than warps, each block of 8 has been ranked by the CTA that completed its logits, before the barrier. Every CTA
+//     sorts the (token, choice) pairs by expert into groups of one expert and up to 8 NT pairs.
 //  1. Input products: units of one group and 16 rows of w_in (8 of each half when gated, so that a lane holds both
-//     factors of a hidden value), K in chunks of 128 bytes. Hidden values leave as pieces. Grid barrier.
+//     factors of a hidden value), K in chunks of 128 bytes. Grid barrier, the hidden values rewritten as digits, grid
+//     barrier.
 //  2. Output products: units of one group and 16 rows of w_out; weighted results per pair. Grid barrier.
 //  3. The sum over each token's pairs, in the order of their rank: the result does not depend on the schedule.
 // A CTA owns a contiguous range of units and its warps equal contiguous ranges of the units' chunks; a unit cut between
-// warps meets through partial sums (`segments`), added in order by the warp that holds its start. Each warp
-// feeds itself: a ring of SLOTS 2 KB boxes loaded by TMA (128-byte swizzle, no multicast), the next box issued as soon as
-// one is in registers. The ring runs on into phase 2's weights, which do not depend on the barrier: DRAM stays busy
-// while the hidden values are exchanged.
+// warps meets through partial sums (`segments`), added by the warp that holds its start. Each warp feeds itself: a ring of
+// SLOTS 2 KB boxes loaded by TMA (128-byte swizzle, no multicast), the next box issued as soon as one is in registers. The
+// ring runs on into phase 2's weights, which do not depend on the barriers: DRAM stays busy while the hidden values
+// are exchanged.
 //
-// Arithmetic: int8 weights are exact in 16 bits. float16 x multiplies as it is; float32 values are cut into three
-// bfloat16 pieces of 8 bits (exact), hidden values of a float16 layer into two (16 bits, 2^-17 relative, the range of
-// float32). mma.sync m16n8k16 with the weights as the 16-row operand and 8 tokens as its columns: the tensor
-// cores' rate does not matter here (one token per expert uses an eighth of a tile), the fragments come straight from
-// the swizzled rows, and 128-row tcgen05 tiles would cut the work too coarsely for one token. Every chunk's sums start
-// at zero and are added in float32, so that no more than 128 products are accumulated inside the matrix instructions.
+// Arithmetic: the int8 weights multiply as they are (mma.sync m16n8k32 s8, weights as the 16-row operand, 8 pairs as its
+// columns). The other operand is a row of x or of hidden values in fixed point, q = rint(v 2^s) with the row's own s, cut
+// into D balanced base-256 digits that are int8 operands too: every digit's sum is an exact int32 (65536 x 128 x 128 stays
+// below 2^31) and the digits' sums together an exact int64, whatever the order. Held are 23 bits below the row's largest
+// value for float16 layers (D = 3) and 31 bits for float32 ones (D = 4), float32's own precision for values down to 2^-7
+// of the largest. Measured against converting
+// the weights to bfloat16 in registers and multiplying two or three bfloat16 pieces: 239 instructions per 2 KB of
+// weights became about 100, 8 tokens through 2 of 8 experts (4096 x 8192) went from 163 to 149 us (4.9 TB/s over the whole
+// launch, 6 TB/s while the weights stream), 64 tokens through 6 of 64 experts (2048 x 1408) from 199 to 164 us. The tensor cores' rate does not matter here (one token per expert uses an eighth of
+// a tile), and 128-row tcgen05 tiles would cut the work too coarsely for one token.
+// A token with an infinite or NaN value, or such a hidden value, gets NaN.
 #include <cuda.h>
-#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -39,20 +44,33 @@
 namespace og {
 
 namespace moe {
-constexpr int WARPS = 16;
-constexpr int THREADS = 32 * WARPS;
-constexpr int ROWS = 16;                      // weight rows of a unit
 constexpr int CHUNK = 128;                    // bytes of K of a box
-constexpr int BOX = ROWS * CHUNK;             // 2 KB
-constexpr int SLOTS = 4;                      // boxes in flight per warp: 128 KB per SM
+constexpr int SLOTS = 4;                      // boxes in flight per warp
 constexpr int MAX_PAIRS = MOE_MAX_TOKENS * MOE_MAX_TOP_K;
-constexpr int PIECE_BYTES = 2 * CHUNK;        // one piece of one row's chunk
+
+// MT matrix tiles of 16 weight rows in a unit, NT tiles of 8 columns in a group. MT = 1: 16 warps (of at most 128
+// registers), the finest units, for one or two tokens, whose columns are all the same few rows. MT = 2: 8 warps, each
+// column digit read from L1 for 32 weight rows instead of 16: with 8 different rows a load touches 8 lines, and from
+// some 4 columns on these loads, not DRAM, set the time.
+template <int NT_, int MT_>
+struct Shape {
+    static constexpr int NT = NT_, MT = MT_;
+    static constexpr int WARPS = MT == 1 ? 16 : 8;
+    static constexpr int THREADS = 32 * WARPS;
+    static constexpr int ROWS = 16 * MT;
+    static constexpr int BOX = ROWS * CHUNK;              // 2 or 4 KB; 128 KB of boxes in flight per SM
+    static constexpr int SUMS = ROWS * 8 * NT;            // of a unit
+    static constexpr int WHOLE_FROM = WARPS * 3 / 4;      // warps with a whole unit each: 96 KB in flight are enough
+    static constexpr int RING = WARPS * SLOTS * BOX;
+};
 }  // namespace moe
 
 struct MoeFusedParams {
     MoeLaunch L;
     int chunks_in, chunks_out;  // K chunks of the two products
     int blocks_in, blocks_out;  // units per group
+    int router_split;           // warps that share one (expert, 8 tokens) of the router
+    int vec;                    // rows of x and of the router allow loads of four elements
 };
 
 // A group: one expert and a run of the pairs sorted by expert.
@@ -60,94 +78,104 @@ struct MoeGroup {
     uint16_t expert, first, count, pad;
 };
 
-template <int NT>
+template <class S>
 struct MoeShared {
-    static constexpr int GROUPS = MOE_MAX_EXPERTS + moe::MAX_PAIRS / (8 * NT);
-    uint64_t full[moe::WARPS][moe::SLOTS];
-    double logit_part[2][moe::WARPS][8];
+    static constexpr int GROUPS = MOE_MAX_EXPERTS + moe::MAX_PAIRS / (8 * S::NT);
+    uint64_t full[S::WARPS][moe::SLOTS];
+    double logit_part[2][S::WARPS][8];
+    int count[MOE_MAX_EXPERTS];        // pairs of each expert, then the place of its first one in `order`
     float weight[moe::MAX_PAIRS];      // by pair (token * top_k + rank)
-    uint16_t id[moe::MAX_PAIRS];       // by pair
+    uint32_t most[moe::MAX_PAIRS];     // by pair: the bits of its largest hidden value seen by this CTA
+    int16_t shift[moe::MAX_PAIRS];     // by pair: the shift of its token's x, later of its hidden values
+    alignas(16) uint16_t id[moe::MAX_PAIRS];  // by pair
     uint16_t order[moe::MAX_PAIRS];    // pairs sorted by expert
     MoeGroup group[GROUPS];
-    int warp_total[2][moe::WARPS];
+    int warp_total[2][S::WARPS];
+    unsigned complete;                 // token blocks whose logits this CTA completed
     int groups;
     int abort;
     int failed;
 };
 
-template <int NT>
-__host__ __device__ constexpr int moe_segment_floats() { return moe::ROWS * 8 * NT; }
-
-template <int NT>
+template <class S>
 constexpr size_t moe_smem_bytes() {
-    return 1024 + size_t(moe::WARPS) * moe::SLOTS * moe::BOX + sizeof(MoeShared<NT>);
+    return 1024 + size_t(S::RING) + sizeof(MoeShared<S>);
 }
 
-// ---- pieces ---------------------------------------------------------------------------------------------------------
+// ---- digits ---------------------------------------------------------------------------------------------------------
 
-// A float32 as P 16-bit pieces whose sum it is: for P = 1 the float16 it came from; for P = 3 three bfloat16 of 8 bits,
-// cut off rather than rounded so that no piece overflows; for P = 2 the second one rounded. An infinity or NaN is its
-// first piece alone.
-template <int P>
-__device__ __forceinline__ void to_pieces(float v, uint16_t (&out)[P]) {
-    if constexpr (P == 1) {
-        out[0] = __half_as_ushort(__float2half_rn(v));
-    } else {
-        const uint32_t bits = __float_as_uint(v);
-        if ((bits & 0x7F800000u) == 0x7F800000u) {
-            out[0] = static_cast<uint16_t>((bits & 0x007FFFFFu) ? 0x7FC0u : bits >> 16);
+// v * 2^n, by two factors so that every n that occurs (below 2 * 126 in size) can be formed.
+__device__ __forceinline__ float times_pow2(float v, int n) {
+    const int a = n / 2;
+    return v * __int_as_float((127 + a) << 23) * __int_as_float((127 + n - a) << 23);
+}
+
+// The shift s of a row whose largest magnitude has the bits `most`: v 2^s rounds to D balanced digits, the largest one's
+// to nearly all their range. A row of zeros shifts by 0.
+template <int D>
+__device__ __forceinline__ int row_shift(uint32_t most) {
+    if (most == 0) return 0;
+    const int exponent = most >= 0x00800000u ? static_cast<int>(most >> 23) - 127 : -118 - __clz(most);
+    const int s = 8 * D - 2 - exponent;  // the largest in [2^(8 D - 2), 2^(8 D - 1))
+    const float limit = D == 3 ? 8355711.0f : 2139062016.0f;  // 127 (256^D - 1) / 255, rounded down to a float32
+    return times_pow2(__uint_as_float(most), s) > limit ? s - 1 : s;
+}
+
+constexpr int NOT_FINITE = 0x7FFF;  // in place of the shift of a row that holds an infinity or NaN
+
+template <int D>
+__device__ __forceinline__ int16_t shift_or_not(uint32_t most) {
+    return static_cast<int16_t>(most < 0x7F800000u ? row_shift<D>(most) : NOT_FINITE);
+}
+
+// A digits' sum as the value it stands for.
+__device__ __forceinline__ float shifted_back(long long sum, int shift) {
+    return shift == NOT_FINITE ? NAN : times_pow2(__ll2float_rn(sum), -shift);
+}
+
+__device__ __forceinline__ bool finite_bits(uint32_t most) { return most < 0x7F800000u; }
+
+// Four values of a row as D words of digits, the lowest digit first, at `to`, `to` + 128 ..
+template <int D>
+__device__ __forceinline__ void put_digits(const float4& v, int shift, uint8_t* to) {
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    uint32_t word[D] = {};
 #pragma unroll
-            for (int p = 1; p < P; p++) out[p] = 0;
-            return;
-        }
+    for (int i = 0; i < 4; i++) {
+        int q = __float2int_rn(times_pow2(f[i], shift));
 #pragma unroll
-        for (int p = 0; p < P; p++) {
-            if (P == 2 && p == 1) {
-                out[p] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
-            } else {
-                const uint32_t top = __float_as_uint(v) & 0xFFFF0000u;
-                out[p] = static_cast<uint16_t>(top >> 16);
-                v = v - __uint_as_float(top);  // exact
-            }
+        for (int d = 0; d < D; d++) {
+            const int digit = static_cast<int8_t>(q);
+            word[d] |= static_cast<uint32_t>(digit & 0xFF) << (8 * i);
+            q = (q - digit) >> 8;
         }
     }
+#pragma unroll
+    for (int d = 0; d < D; d++) *reinterpret_cast<uint32_t*>(to + d * moe::CHUNK) = word[d];
 }
 
-// Two bytes of a word of int8 weights as a pair of 16-bit floats, exactly. float16: 0x6400 | u is 1024 + u for the byte
-// u = w + 128. bfloat16 holds 7 mantissa bits: 0x4300 | (w & 0x7F) is 128 + those bits, and 0x4300 | (w & 0x80) is 128, or
-// 256 for a negative w.
-template <bool BF16, bool HIGH>
-__device__ __forceinline__ uint32_t weight_pair(uint32_t w) {
-    uint32_t r;
-    if constexpr (BF16) {
-        const uint32_t p = __byte_perm(w, 0x43434343u, HIGH ? 0x4342 : 0x4140);
-        const uint32_t a = p & 0xFF7FFF7Fu, b = p & 0xFF80FF80u;
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
-                                         *reinterpret_cast<const __nv_bfloat162*>(&b));
-        r = *reinterpret_cast<const uint32_t*>(&d);
-    } else {
-        const uint32_t p = __byte_perm(w, 0x64646464u, HIGH ? 0x4342 : 0x4140);  // w: bytes + 128
-        const uint32_t b = 0x64806480u;                                          // 1152
-        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&b));
-        r = *reinterpret_cast<const uint32_t*>(&d);
-    }
-    return r;
+// Where value k (a multiple of 4) of a row chunk's digits lies. In step i of the chunk's four, lane q of a matrix column
+// needs k = 32 i + 4 q .. and k = 32 i + 16 + 4 q ..; the words of steps 2 j and 2 j + 1 form its 16-byte unit (j, q), so
+// that a column's four lanes read 64 consecutive bytes.
+__device__ __forceinline__ int digit_place(int k) {
+    return (k >> 6) * 64 + ((k >> 2) & 3) * 16 + ((k >> 5) & 1) * 8 + ((k >> 4) & 1) * 4;
 }
 
-template <bool BF16>
-__device__ __forceinline__ void moe_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void moe_mma(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The 16 x 32 byte operand of one step: lane l gives the address of one of the four 8 x 16 byte parts' rows (rows 0-7 and
+// 8-15 of the first 16 bytes, then of the second), every lane gets its four words in the order the instruction takes them.
+__device__ __forceinline__ void load_rows(uint32_t (&a)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                 : "r"(addr)
+                 : "memory");
 }
 
 // ---- grid barrier ---------------------------------------------------------------------------------------------------
@@ -173,16 +201,29 @@ __device__ __forceinline__ bool grid_arrive(unsigned long long* arrivals, bool w
     return true;
 }
 
-// The whole CTA meets the grid; false (for every thread) when this CTA has failed or gives up here.
-template <class S>
-__device__ __forceinline__ bool grid_barrier(S& sh, unsigned long long* arrivals) {
+// The whole CTA meets the grid; false (for every thread) when this CTA has failed or gives up here. Out of line: the
+// kernel runs each of its parts once or twice, so instructions that are fetched a second time are what it waits for.
+static __device__ __noinline__ bool grid_barrier(unsigned long long* arrivals, const int* abort, int* failed) {
     __syncthreads();
     if (threadIdx.x == 0) {
-        const bool ok = sh.abort == 0;
-        if (!grid_arrive(arrivals, ok) || !ok) sh.failed = 1;
+        const bool ok = *abort == 0;
+        if (!grid_arrive(arrivals, ok) || !ok) *failed = 1;
     }
     __syncthreads();
-    return sh.failed == 0;
+    return *failed == 0;
+}
+
+// The counts of finished logits, for the next launch; by CTA 0, once every CTA is past the first barrier.
+__device__ __forceinline__ void clear_tickets(const MoeLaunch& L) {
+    for (int i = 0; i < MOE_MAX_TOKENS / 8; i++) atomicExch(L.tickets + i, 0u);
+}
+
+// A CTA that gives up: the launch's failure is raised and the barriers it will not wait at still count it.
+__device__ __forceinline__ void leave_early(const MoeLaunch& L, int barriers_left) {
+    if (threadIdx.x != 0) return;
+    if (blockIdx.x == 0) clear_tickets(L);
+    for (int i = 0; i < barriers_left; i++) grid_arrive(L.arrivals, false);
+    atomicExch(L.error_flag, 1);
 }
 
 // ---- phase 0 --------------------------------------------------------------------------------------------------------
@@ -191,69 +232,130 @@ __device__ __forceinline__ float moe_load(const void* p, int half, int64_t i) {
     return half ? __half2float(__ldg(static_cast<const __half*>(p) + i)) : __ldg(static_cast<const float*>(p) + i);
 }
 
-// x as pieces: 16-byte unit (j, q) of a chunk's piece holds the eight values k = 32 q + 8 j ..; and zeros in the part of
-// the hidden values' last chunk that lies past the expert's size.
-template <int PX, int PH>
-__device__ __forceinline__ void moe_split_x(const MoeFusedParams& p) {
+// Four consecutive elements; VEC when they may be loaded as one.
+template <bool HALF, bool VEC>
+__device__ __forceinline__ float4 moe_load4(const void* p, int64_t i) {
+    if constexpr (!VEC)
+        return make_float4(moe_load(p, HALF, i), moe_load(p, HALF, i + 1), moe_load(p, HALF, i + 2), moe_load(p, HALF, i + 3));
+    if constexpr (!HALF) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(p) + i));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// The start of part `part` of `total` things in `parts` nearly equal parts.
+__device__ __forceinline__ int moe_split(int total, int part, int parts) {
+    return static_cast<int>(static_cast<int64_t>(total) * part / parts);
+}
+
+// x as digits, row chunk by row chunk [D][128]. A warp finds its token's largest value and converts a part of four chunks.
+template <class S, bool HALF, bool VEC>
+__device__ __forceinline__ void moe_digits_x(const MoeFusedParams& p) {
+    constexpr int D = HALF ? 3 : 4;
     const MoeLaunch& L = p.L;
-    const int thread = blockIdx.x * moe::THREADS + threadIdx.x, threads = gridDim.x * moe::THREADS;
-    const int units = L.tokens * p.chunks_in * 16;
-    for (int u = thread; u < units; u += threads) {
-        const int t = u / (p.chunks_in * 16), c = (u >> 4) % p.chunks_in, j = (u >> 2) & 3, q = u & 3;
-        const int k0 = c * moe::CHUNK + 32 * q + 8 * j;
-        uint16_t piece[PX][8];
+    const int lane = threadIdx.x & 31;
+    const int parts = (p.chunks_in + 3) / 4;
+    // Spread over the CTAs, from the last one down: the first ones hold the router's units.
+    for (int u = (threadIdx.x >> 5) * gridDim.x + gridDim.x - 1 - blockIdx.x; u < L.tokens * parts;
+         u += gridDim.x * S::WARPS) {
+        const int t = u / parts, part = u - t * parts;
+        const int64_t x0 = static_cast<int64_t>(t) * L.model;
+        const int vectors = L.model / 4;  // model is a multiple of 16
+        uint32_t most = 0;
+#pragma unroll 1
+        for (int v0 = lane; v0 < vectors; v0 += 256) {
+            float4 x[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            uint16_t v[PX];
-            to_pieces<PX>(k0 + i < L.model ? moe_load(L.x, L.x_half, static_cast<int64_t>(t) * L.model + k0 + i) : 0.0f, v);
+            for (int i = 0; i < 8; i++)  // all in flight; past the end, the last vector again
+                x[i] = moe_load4<HALF, VEC>(L.x, x0 + 4 * min(v0 + 32 * i, vectors - 1));
 #pragma unroll
-            for (int s = 0; s < PX; s++) piece[s][i] = v[s];
+            for (int i = 0; i < 8; i++)
+                most = max(max(most, max(__float_as_uint(x[i].x) & 0x7FFFFFFFu, __float_as_uint(x[i].y) & 0x7FFFFFFFu)),
+                           max(__float_as_uint(x[i].z) & 0x7FFFFFFFu, __float_as_uint(x[i].w) & 0x7FFFFFFFu));
         }
-        uint8_t* to = L.x_pieces + (static_cast<int64_t>(t) * p.chunks_in + c) * PX * moe::PIECE_BYTES + j * 64 + q * 16;
-#pragma unroll
-        for (int s = 0; s < PX; s++)
-            *reinterpret_cast<uint4*>(to + s * moe::PIECE_BYTES) =
-                make_uint4(piece[s][0] | piece[s][1] << 16, piece[s][2] | piece[s][3] << 16,
-                           piece[s][4] | piece[s][5] << 16, piece[s][6] | piece[s][7] << 16);
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
+        if (part == 0 && lane == 0) L.x_most[t] = most;
+        const int shift = finite_bits(most) ? row_shift<D>(most) : 0;
+#pragma unroll 1
+        for (int c = part * 4; c < min(part * 4 + 4, p.chunks_in); c++) {
+            const int k = c * moe::CHUNK + lane * 4;
+            const float4 x = k < L.model ? moe_load4<HALF, VEC>(L.x, x0 + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            put_digits<D>(x, shift, L.x_digits + (static_cast<int64_t>(t) * p.chunks_in + c) * D * moe::CHUNK +
+                                        digit_place(lane * 4));
+        }
     }
-    const int used = (L.expert % moe::CHUNK) / 8;  // units of the last chunk that hold values (expert is a multiple of 8)
-    if (used != 0) {
-        const int pairs = L.tokens * L.top_k, empty = 16 - used;
-        for (int u = thread; u < pairs * empty * PH; u += threads) {
-            const int pair = u / (empty * PH), s = (u / empty) % PH, k = 8 * (used + u % empty);
-            uint8_t* to = L.h_pieces +
-                          ((static_cast<int64_t>(pair) * p.chunks_out + p.chunks_out - 1) * PH + s) * moe::PIECE_BYTES +
-                          (k % 32) / 8 * 64 + k / 32 * 16;
-            *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
-        }
+    for (int i = blockIdx.x * S::THREADS + threadIdx.x; i < L.tokens * L.top_k; i += gridDim.x * S::THREADS)
+        L.h_most[i] = 0;
+}
+
+// The hidden values as digits, in the same layout; zeros past the expert's size. A warp converts a chunk at a time.
+template <class S, int D>
+__device__ __forceinline__ void moe_digits_h(const MoeFusedParams& p) {
+    const MoeLaunch& L = p.L;
+    const int lane = threadIdx.x & 31;
+    const int units = L.tokens * L.top_k * p.chunks_out;
+#pragma unroll 1
+    for (int u = (threadIdx.x >> 5) * gridDim.x + blockIdx.x; u < units; u += gridDim.x * S::WARPS) {
+        const int pair = u / p.chunks_out, k = (u - pair * p.chunks_out) * moe::CHUNK + lane * 4;
+        const uint32_t most = __ldcg(L.h_most + pair);
+        float4 h = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k < L.expert)  // expert is a multiple of 16
+            h = __ldcg(reinterpret_cast<const float4*>(L.hidden + static_cast<int64_t>(pair) * L.expert + k));
+        put_digits<D>(h, finite_bits(most) ? row_shift<D>(most) : 0,
+                      L.h_digits + static_cast<int64_t>(u) * D * moe::CHUNK + digit_place(lane * 4));
     }
 }
 
-// Logits: a CTA per (expert, 8 tokens), lanes striding over the sum; eight products at a time in float32, the rest in
-// float64, so that near-equal logits rank as their exact values do.
-template <class S>
-__device__ __forceinline__ void moe_logits(const MoeLaunch& L, S& sh) {
+// Logits: units of one expert and 8 tokens, each shared by router_split warps of a CTA (so that a few units still occupy
+// the SMs). Eight products at a time in float32, the rest in float64, so that near-equal logits rank as their exact
+// values do.
+template <class S, bool HALF, bool VEC, bool ROUTER_HALF>
+__device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>& sh) {
+    const MoeLaunch& L = p.L;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int token_blocks = (L.tokens + 7) / 8;
+    const int split = p.router_split, per_cta = S::WARPS / split, part = warp % split;
+    const int token_blocks = (L.tokens + 7) / 8, units = L.experts * token_blocks;
+    const int vectors = L.model / 4;  // of four elements (model is a multiple of 16); this warp's share of them
+    const int v0 = moe_split(vectors, part, split), v1 = moe_split(vectors, part + 1, split);
     int buffer = 0;
-    for (int unit = blockIdx.x; unit < L.experts * token_blocks; unit += gridDim.x, buffer ^= 1) {
-        const int e = unit / token_blocks, t0 = (unit % token_blocks) * 8, n = min(8, L.tokens - t0);
+    for (int first = blockIdx.x * per_cta; first < units; first += gridDim.x * per_cta, buffer ^= 1) {
+        const int unit = first + warp / split;
+        const int block = unit / L.experts, e = unit - block * L.experts, t0 = block * 8;  // a block's units lie together:
+                                                                                          // blocks end on different CTAs
+        const int n = unit < units ? min(8, L.tokens - t0) : 0;
         double sum[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) sum[i] = 0.0;
-        for (int d0 = threadIdx.x; d0 < L.model; d0 += 8 * moe::THREADS) {
-            float part[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (n > 0) {
+            const int64_t r0 = static_cast<int64_t>(e) * L.model, x0 = static_cast<int64_t>(t0) * L.model;
+            // Past the tokens or the share, the last one again (its sums are dropped): every load of a step is in flight
+            // at once.
+            for (int v = v0 + lane; v < v1; v += 64) {
+                float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                float4 r[2], x[2][8];
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
-                const int d = d0 + s * moe::THREADS;
-                if (d >= L.model) break;
-                const float r = moe_load(L.router, L.router_half, static_cast<int64_t>(e) * L.model + d);
+                for (int u = 0; u < 2; u++) {
+                    const int d = 4 * min(v + 32 * u, v1 - 1);
+                    r[u] = moe_load4<ROUTER_HALF, VEC>(L.router, r0 + d);
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (i < n) part[i] = fmaf(moe_load(L.x, L.x_half, static_cast<int64_t>(t0 + i) * L.model + d), r, part[i]);
+                    for (int i = 0; i < 8; i++)
+                        x[u][i] = moe_load4<HALF, VEC>(L.x, x0 + static_cast<int64_t>(min(i, n - 1)) * L.model + d);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    if (u == 1 && v + 32 >= v1) break;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        f[i] = fmaf(x[u][i].x, r[u].x, f[i]);
+                        f[i] = fmaf(x[u][i].y, r[u].y, f[i]);
+                        f[i] = fmaf(x[u][i].z, r[u].z, f[i]);
+                        f[i] = fmaf(x[u][i].w, r[u].w, f[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) sum[i] += f[i];
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) sum[i] += part[i];
         }
         // Lane bits 4, 3 and 2 choose the token: 4 + 2 + 1 exchanges, then two more within each token's four lanes.
         double a[4], b[2], c;
@@ -272,10 +374,17 @@ __device__ __forceinline__ void moe_logits(const MoeLaunch& L, S& sh) {
         c += __shfl_xor_sync(0xFFFFFFFFu, c, 1);
         if ((lane & 3) == 0) sh.logit_part[buffer][warp][lane >> 2] = c;
         __syncthreads();
-        if (static_cast<int>(threadIdx.x) < n) {
+        if (part == 0 && lane < n) {
             double total = 0.0;
-            for (int w = 0; w < moe::WARPS; w++) total += sh.logit_part[buffer][w][threadIdx.x];
-            L.logits[static_cast<int64_t>(t0 + threadIdx.x) * L.experts + e] = static_cast<float>(total);
+            for (int w = 0; w < split; w++) total += sh.logit_part[buffer][warp + w][lane];
+            L.logits[static_cast<int64_t>(t0 + lane) * L.experts + e] = static_cast<float>(total);
+        }
+        if (L.tokens > S::WARPS && part == 0 && n > 0) {
+            __syncwarp();
+            if (lane == 0) {
+                __threadfence();
+                if (atomicAdd(L.tickets + t0 / 8, 1u) == static_cast<unsigned>(L.experts) - 1) atomicOr(&sh.complete, 1u << (t0 / 8));
+            }
         }
     }
 }
@@ -288,81 +397,147 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;  // -infinity is 0x007FFFFF: 0 marks a taken expert
 }
 
-// A token's experts by one warp: the largest key, the lowest expert among equals, top_k times.
-template <class S>
-__device__ __forceinline__ void moe_choose(const MoeLaunch& L, S& sh, int t, bool publish) {
+// A token's experts by one warp: the largest key, the lowest expert among equals, top_k times. PER_LANE logits per lane.
+template <class S, int D, int PER_LANE>
+__device__ __forceinline__ void moe_choose(const MoeLaunch& L, MoeShared<S>& sh, int t, float (&v)[PER_LANE], uint32_t x_most,
+                                           bool publish) {
     const int lane = threadIdx.x & 31;
-    constexpr int PER_LANE = MOE_MAX_EXPERTS / 32;
-    const float* logits = L.logits + static_cast<int64_t>(t) * L.experts;
     uint32_t key[PER_LANE];
     float top = -INFINITY;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < PER_LANE; i++) {
-        key[i] = 0;
-        if (32 * i < L.experts && lane + 32 * i < L.experts) {
-            const float v = __ldcg(logits + lane + 32 * i);
-            key[i] = rank_key(v);
-            nan |= isnan(v);
-            top = fmaxf(top, v);
-        }
+        key[i] = lane + 32 * i < L.experts ? rank_key(v[i]) : 0u;
+        nan |= isnan(v[i]);
+        top = fmaxf(top, v[i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     if (__any_sync(0xFFFFFFFFu, nan)) top = NAN;  // the softmax of a row with a NaN is NaN
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER_LANE; i++)
-        if (32 * i < L.experts && lane + 32 * i < L.experts) sum += expf(__ldcg(logits + lane + 32 * i) - top);
+    for (int i = 0; i < PER_LANE; i++) {
+        v[i] = lane + 32 * i < L.experts ? expf(v[i] - top) : 0.0f;
+        sum += v[i];
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     float weight = 0.0f, chosen = 0.0f;
     int id = 0;
+#pragma unroll 1
     for (int k = 0; k < L.top_k; k++) {
         uint32_t best = 0;
-#pragma unroll
-        for (int i = 0; i < PER_LANE; i++)
-            if (32 * i < L.experts) best = max(best, key[i]);
-        best = __reduce_max_sync(0xFFFFFFFFu, best);
+        float share = 0.0f;
         int at = MOE_MAX_EXPERTS;
 #pragma unroll
-        for (int i = PER_LANE - 1; i >= 0; i--)
-            if (32 * i < L.experts && key[i] == best) at = lane + 32 * i;
-        at = __reduce_min_sync(0xFFFFFFFFu, at);
+        for (int i = 0; i < PER_LANE; i++)
+            if (key[i] > best) {
+                best = key[i];
+                at = lane + 32 * i;
+                share = v[i];
+            }
+        const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, best);
+        const int chosen_at = __reduce_min_sync(0xFFFFFFFFu, best == most ? at : MOE_MAX_EXPERTS);
+        share = __shfl_sync(0xFFFFFFFFu, share, chosen_at & 31);
+        chosen += share;
+        if (lane == k) {
+            weight = share;
+            id = chosen_at;
+        }
 #pragma unroll
         for (int i = 0; i < PER_LANE; i++)
-            if (at == lane + 32 * i) key[i] = 0;
-        const float w = expf(__ldcg(logits + at) - top) / sum;
-        chosen += w;
-        if (lane == k) {
-            weight = w;
-            id = at;
-        }
+            if (chosen_at == lane + 32 * i) key[i] = 0;
     }
     if (lane < L.top_k) {
-        if (L.normalize) weight = weight / chosen;
+        weight = weight / (L.normalize ? chosen : sum);
         const int i = t * L.top_k + lane;
         sh.id[i] = static_cast<uint16_t>(id);
         sh.weight[i] = weight;
+        sh.shift[i] = shift_or_not<D>(x_most);
         if (publish) {
+            L.ids[i] = id;
+            L.weights[i] = weight;
             if (L.ids_out != nullptr) L.ids_out[i] = id;
             if (L.weights_out != nullptr) L.weights_out[i] = weight;
         }
     }
 }
 
-// The pairs sorted by expert and cut into groups of at most 8 NT pairs: thread e counts, places and lists expert e.
-template <int NT>
-__device__ __forceinline__ void moe_group(const MoeLaunch& L, MoeShared<NT>& sh) {
-    const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
-    const int pairs = L.tokens * L.top_k;
-    int count = 0;
-    if (e < L.experts)
-        for (int i = 0; i < pairs; i++) count += sh.id[i] == e;
-    const int groups = (count + 8 * NT - 1) / (8 * NT);
-    int first = count, group = groups;  // inclusive sums over the experts
+// Tokens first .. first + count - 1, a warp each.
+template <class S, int D, int PER_LANE>
+__device__ __forceinline__ void moe_choose_some(const MoeLaunch& L, MoeShared<S>& sh, int first, int count, bool publish) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int t = first + warp; t < first + count; t += S::WARPS) {
+        float v[PER_LANE];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+        for (int i = 0; i < PER_LANE; i++)
+            v[i] = lane + 32 * i < L.experts ? __ldcg(L.logits + static_cast<int64_t>(t) * L.experts + lane + 32 * i)
+                                             : -INFINITY;
+        moe_choose<S, D, PER_LANE>(L, sh, t, v, L.tokens > S::WARPS ? 0u : __ldcg(L.x_most + t), publish);
+    }
+}
+
+template <class S, int D>
+__device__ __forceinline__ void moe_choose_tokens(const MoeLaunch& L, MoeShared<S>& sh, int first, int count, bool publish) {
+    if (L.experts <= 128)
+        moe_choose_some<S, D, 4>(L, sh, first, count, publish);
+    else
+        moe_choose_some<S, D, MOE_MAX_EXPERTS / 32>(L, sh, first, count, publish);
+}
+
+// The pairs sorted by expert and cut into groups of at most 8 NT pairs; each thread lists its experts'. Within a group the
+// pairs stand in the order the threads come in, which changes no result (a pair's sums do not depend on its column). Where
+// an expert has more than one group, every CTA must cut its pairs alike: they are put in order first.
+template <class S>
+__device__ __forceinline__ void moe_group(const MoeLaunch& L, MoeShared<S>& sh) {
+    constexpr int PER_THREAD = moe::MAX_PAIRS / S::THREADS, EXPERTS = MOE_MAX_EXPERTS / S::THREADS, FULL = 8 * S::NT;
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    const int pairs = L.tokens * L.top_k;
+#pragma unroll
+    for (int i = 0; i < EXPERTS; i++) sh.count[thread * EXPERTS + i] = 0;
+    __syncthreads();  // the choices are in, the counts are clear
+    int rank[PER_THREAD];
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; i++) {
+        const int pair = thread + i * S::THREADS;
+        if (pair >= pairs) break;
+        rank[i] = atomicAdd(&sh.count[sh.id[pair]], 1);
+    }
+    __syncthreads();
+    int count[EXPERTS], first = 0, group = 0;
+    bool many = false;
+#pragma unroll
+    for (int i = 0; i < EXPERTS; i++) {
+        count[i] = sh.count[thread * EXPERTS + i];
+        first += count[i];
+        group += (count[i] + FULL - 1) / FULL;
+        many |= count[i] > FULL;
+    }
+    if (__syncthreads_or(many)) {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; i++) {
+            const int pair = thread + i * S::THREADS;
+            if (pair >= pairs || sh.count[sh.id[pair]] <= FULL) continue;
+            const uint32_t same = sh.id[pair];
+            int less = 0;
+#pragma unroll 1
+            for (int j = 0; j < pair; j += 8) {  // ids past the pairs are never counted: they lie past `pair`
+                const uint4 v = *reinterpret_cast<const uint4*>(&sh.id[j]);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    less += j + 2 * u < pair && (w[u] & 0xFFFFu) == same;
+                    less += j + 2 * u + 1 < pair && (w[u] >> 16) == same;
+                }
+            }
+            rank[i] = less;
+        }
+        __syncthreads();  // the counts have been read
+    }
+    const int own = first, own_groups = group;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {  // inclusive sums over the experts
         const int a = __shfl_up_sync(0xFFFFFFFFu, first, o), b = __shfl_up_sync(0xFFFFFFFFu, group, o);
         if (lane >= o) {
             first += a;
@@ -374,303 +549,454 @@ __device__ __forceinline__ void moe_group(const MoeLaunch& L, MoeShared<NT>& sh)
         sh.warp_total[1][warp] = group;
     }
     __syncthreads();
-    for (int w = 0; w < warp; w++) {
-        first += sh.warp_total[0][w];
-        group += sh.warp_total[1][w];
+#pragma unroll
+    for (int w = 0; w < S::WARPS; w++)
+        if (w < warp) {
+            first += sh.warp_total[0][w];
+            group += sh.warp_total[1][w];
+        }
+    if (thread == S::THREADS - 1) sh.groups = group;
+    first -= own;
+    group -= own_groups;
+#pragma unroll
+    for (int i = 0; i < EXPERTS; i++) {
+        const int e = thread * EXPERTS + i;
+        sh.count[e] = first;
+        for (int done = 0; done < count[i]; done += FULL)
+            sh.group[group++] = MoeGroup{static_cast<uint16_t>(e), static_cast<uint16_t>(first + done),
+                                         static_cast<uint16_t>(min(FULL, count[i] - done)), 0};
+        first += count[i];
     }
-    if (e == moe::THREADS - 1) sh.groups = group;
-    first -= count;
-    group -= groups;
-    if (count > 0) {
-        int at = first;
-        for (int i = 0; i < pairs; i++)
-            if (sh.id[i] == e) sh.order[at++] = static_cast<uint16_t>(i);
-        for (int g = 0; g < groups; g++)
-            sh.group[group + g] = MoeGroup{static_cast<uint16_t>(e), static_cast<uint16_t>(first + g * 8 * NT),
-                                           static_cast<uint16_t>(min(8 * NT, count - g * 8 * NT)), 0};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; i++) {
+        const int pair = thread + i * S::THREADS;
+        if (pair >= pairs) break;
+        sh.order[sh.count[sh.id[pair]] + rank[i]] = static_cast<uint16_t>(pair);
     }
     __syncthreads();
 }
 
 // ---- phases 1 and 2 -------------------------------------------------------------------------------------------------
 
-// One phase's work of this warp: chunks [at, end) of the CTA's units, unit u0 + i / chunks, chunk i % chunks.
+// One phase's work of this warp. The CTA owns units [u0, u0 + units). Its warps take whole units in turn, walking K
+// together, so that they find the columns' digits in L1; the units left over after the full rounds go to a warp each if
+// there are many, and are otherwise cut into equal runs of chunks, so that every warp keeps boxes in flight to the end.
+// Position i of a warp's work: chunk i % chunks of its unit i / chunks for i < rounds * chunks, then the run
+// [at, end) of the chunks of units u0 + tail ..
 struct MoeRange {
-    int u0, units;  // the CTA's units
-    int at, end;
+    int u0, units;
+    int rounds;   // whole units of this warp
+    int tail;     // units before the cut ones
+    int at, end;  // the warp's run of the cut units' chunks
 };
 
-__device__ __forceinline__ int moe_split(int total, int part, int parts) {
-    return static_cast<int>(static_cast<int64_t>(total) * part / parts);
-}
-
+template <class S>
 __device__ __forceinline__ MoeRange moe_range(int units, int chunks, int warp) {
     MoeRange r;
     r.u0 = moe_split(units, blockIdx.x, gridDim.x);
     r.units = moe_split(units, blockIdx.x + 1, gridDim.x) - r.u0;
-    r.at = moe_split(r.units * chunks, warp, moe::WARPS);
-    r.end = moe_split(r.units * chunks, warp + 1, moe::WARPS);
+    r.rounds = r.units / S::WARPS;
+    r.tail = r.rounds * S::WARPS;
+    int left = r.units - r.tail;
+    if (left >= S::WHOLE_FROM) {
+        r.rounds += warp < left;
+        r.tail = r.units;
+        left = 0;
+    }
+    r.at = moe_split(left * chunks, warp, S::WARPS);
+    r.end = moe_split(left * chunks, warp + 1, S::WARPS);
     return r;
 }
 
 // The warp that holds chunk i of `total`.
+template <class S>
 __device__ __forceinline__ int moe_owner(int i, int total) {
-    return static_cast<int>((static_cast<int64_t>(i + 1) * moe::WARPS - 1) / total);
+    return static_cast<int>((static_cast<int64_t>(i + 1) * S::WARPS - 1) / total);
 }
 
-// What the warp's ring loads next: phase 1's range, then phase 2's.
+// What the warp's ring loads next: phase 1's work, then phase 2's.
 struct MoeFeed {
-    int phase, at, end;
-    uint32_t issued;  // boxes so far
+    int phase;
+    int rounds;        // whole units still to begin
+    int unit;          // the unit being loaded
+    int left;          // boxes left of this run of boxes (a unit, or the run over the cut units)
+    int x, x_end;      // byte of K of the next box, and past the last one
+    int y, e;          // row and expert (gate half) of the next box
+    uint32_t issued;   // boxes so far
 };
 
-template <int NT>
+template <class S, int D>
 struct MoeWarp {
+    static constexpr int NT = S::NT, MT = S::MT;
     const MoeFusedParams& p;
-    MoeShared<NT>& sh;
-    const CUtensorMap* maps[2];
+    MoeShared<S>& sh;
+    const CUtensorMap* map_in;
+    const CUtensorMap* map_out;
     uint8_t* ring;
     uint64_t* full;
-    int lane;
-    MoeRange range[2];
+    int warp, lane;
+    MoeRange range_in, range_out;
     MoeFeed feed;
     uint32_t taken;  // boxes read so far
+    float2 scale[MT];  // of the unit at hand
 
     __device__ __forceinline__ int chunks(int phase) const { return phase == 0 ? p.chunks_in : p.chunks_out; }
     __device__ __forceinline__ int blocks(int phase) const { return phase == 0 ? p.blocks_in : p.blocks_out; }
 
-    // Issues the next box, if any is left and a slot is free.
-    __device__ __forceinline__ void issue() {
-        while (feed.phase < 2 && feed.at >= feed.end) {
-            feed.phase++;
-            if (feed.phase < 2) {
-                feed.at = range[1].at;
-                feed.end = range[1].end;
-            }
-        }
-        if (feed.phase >= 2 || feed.issued - taken >= moe::SLOTS) return;
-        const int c = chunks(feed.phase), b = blocks(feed.phase);
-        const int local = feed.at / c, chunk = feed.at - local * c;
-        const int unit = range[feed.phase].u0 + local, g = unit / b, block = unit - g * b;
-        if (lane == 0) {
-            const int slot = feed.issued % moe::SLOTS;
-            const int e = sh.group[g].expert;
-            const bool halves = feed.phase == 0 && p.L.gated;
-            mbar_arrive_expect_tx(&full[slot], moe::BOX);
-            tma_load_3d(ring + slot * moe::BOX, maps[feed.phase], &full[slot], chunk * moe::CHUNK,
-                        block * (halves ? 8 : 16), halves ? 2 * e : e);
-        }
-        feed.at++;
-        feed.issued++;
+    // Points the feed at a unit of its phase.
+    __device__ __forceinline__ void aim(int unit) {
+        const int b = blocks(feed.phase), group = unit / b;
+        const bool halves = feed.phase == 0 && p.L.gated;
+        feed.unit = unit;
+        feed.y = (unit - group * b) * (halves ? 8 * MT : 16 * MT);
+        feed.e = sh.group[group].expert * (halves ? 2 : 1);
     }
 
-    // The sums of one unit's chunks [c0, c1) for the group's columns: row g (and g + 8) of the unit, columns 2 q and
-    // 2 q + 1 of n-tile t in acc[t]. BF16 and P: the pieces of the columns' values at `values`, `row` by column.
-    template <bool BF16, int P>
-    __device__ __forceinline__ bool products(const uint8_t* values, const uint32_t (&row)[NT], int tiles, int c0, int c1,
-                                             float (&acc)[NT][4]) {
-        const int g = lane >> 2, q = lane & 3;
+    // The next run of boxes; false when there is none.
+    __device__ __forceinline__ bool next_run() {
+        while (true) {
+            const MoeRange& r = feed.phase == 0 ? range_in : range_out;
+            const int c = chunks(feed.phase);
+            if (feed.rounds < r.rounds) {
+                aim(r.u0 + feed.rounds * S::WARPS + warp);
+                feed.x = 0;
+                feed.x_end = c * moe::CHUNK;
+                feed.left = c;
+                feed.rounds++;
+                return true;
+            }
+            if (feed.rounds == r.rounds && r.at < r.end) {
+                feed.rounds++;
+                const int local = r.at / c;
+                aim(r.u0 + r.tail + local);
+                feed.x = (r.at - local * c) * moe::CHUNK;
+                feed.x_end = c * moe::CHUNK;
+                feed.left = r.end - r.at;
+                return true;
+            }
+            if (feed.phase == 1) return false;
+            feed.phase = 1;
+            feed.rounds = 0;
+        }
+    }
+
+    // Issues the next box if any is left; the caller has freed a slot.
+    __device__ __forceinline__ void issue() {
+        if (feed.left == 0 && !next_run()) return;
+        if (lane == 0) {
+            const int slot = feed.issued % moe::SLOTS;
+            mbar_arrive_expect_tx(&full[slot], S::BOX);
+            tma_load_3d(ring + slot * S::BOX, feed.phase == 0 ? map_in : map_out, &full[slot], feed.x, feed.y, feed.e);
+        }
+        feed.issued++;
+        feed.left--;
+        feed.x += moe::CHUNK;
+        if (feed.x == feed.x_end && feed.left > 0) {
+            feed.x = 0;
+            aim(feed.unit + 1);
+        }
+    }
+
+    // The digits of n-tile t's columns in one chunk: v points at the chunk of row 0 (this lane's 16 bytes).
+    __device__ __forceinline__ static void load_digits(uint4 (&b)[D][2], const uint8_t* v) {
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int d = 0; d < D; d++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[t][i] = 0.0f;
+            for (int j = 0; j < 2; j++) b[d][j] = *reinterpret_cast<const uint4*>(v + d * moe::CHUNK + j * 64);
+    }
+
+    // The digits' sums of one unit's chunks [c0, c1): rows g and g + 8 of matrix tile i, columns 2 q and 2 q + 1 of n-tile
+    // t in acc[i][t][digit]. The columns' digits start at values + row[t] (column g of the tile). `halves`: the box holds
+    // the gate's rows, then the other half's, and a tile 8 of each.
+    __device__ __forceinline__ bool products(const uint8_t* values, const uint32_t (&row)[NT], int tiles, bool halves,
+                                             int c0, int c1, int (&acc)[MT][NT][D][4]) {
+        // Where registers allow, the next chunk's digits are on their way while one is multiplied (64 tokens through 6 of
+        // 64 experts 172 -> 165 us); elsewhere tile 0's are asked for before the wait for the box and the other tiles' when
+        // their turn comes (with NT = 4 or at 16 warps the earlier loads only spill).
+        constexpr bool AHEAD = MT == 2 && NT * D <= 6;
+        constexpr int EARLY = AHEAD ? NT : 1;
+        const int q = lane & 3;
+        // This lane's row of the parts of a step: part lane / 8 is rows 0-7 or 8-15 (odd) of the first or second (2, 3)
+        // 16 bytes. A box's 16-byte units are swizzled by the row (its low three bits are lane % 8 in every part), so eight
+        // lanes of a part touch eight different units of 128 bytes: no bank conflict.
+        const int tile_step = (halves ? 8 : 16) * moe::CHUNK, half_step = (halves ? 8 * MT : 8) * moe::CHUNK;
+        const uint32_t my_row = smem_u32(ring) + (lane & 7) * moe::CHUNK + ((lane >> 3) & 1) * half_step;
+        const uint32_t my_unit = lane >> 4, my_swizzle = lane & 7;
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int d = 0; d < D; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[m][t][d][i] = 0;
+        const uint8_t* v = values + c0 * D * moe::CHUNK + q * 16;
+        uint4 next[EARLY][D][2];
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int t = 0; t < EARLY; t++)
+                if (t < tiles) load_digits(next[t], v + row[t]);
+        }
 #pragma unroll 1
-        for (int c = c0; c < c1; c++) {
+        for (int c = c0; c < c1; c++, v += D * moe::CHUNK) {
             const int slot = taken % moe::SLOTS;
+            uint4 b[EARLY][D][2];
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int t = 0; t < EARLY; t++)
+#pragma unroll
+                    for (int d = 0; d < D; d++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) b[t][d][j] = next[t][d][j];
+                if (c + 1 < c1) {
+#pragma unroll
+                    for (int t = 0; t < EARLY; t++)
+                        if (t < tiles) load_digits(next[t], v + D * moe::CHUNK + row[t]);
+                }
+            } else {
+                load_digits(b[0], v + row[0]);
+            }
             const bool ok = mbar_wait(&full[slot], (taken / moe::SLOTS) & 1, &sh.abort);
             if (!__all_sync(0xFFFFFFFFu, ok)) return false;
-            // Bytes 32 q .. 32 q + 31 of rows g and g + 8: 16-byte units 2 q and 2 q + 1, swizzled by the row. Eight
-            // consecutive lanes touch eight different units of 128 bytes: no bank conflict.
-            const uint8_t* box = ring + slot * moe::BOX + g * moe::CHUNK;
-            uint4 w[2][2];
+            uint32_t a[MT][4][4];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-                    w[h][u] = *reinterpret_cast<const uint4*>(box + h * 8 * moe::CHUNK + (((2 * q + u) ^ g) << 4));
+                for (int i = 0; i < 4; i++)
+                    load_rows(a[m][i], my_row + slot * S::BOX + m * tile_step + (((2 * i + my_unit) ^ my_swizzle) << 4));
             taken++;
-            __syncwarp();  // the slot is in registers
-            issue();
-            uint32_t a[8][4];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t lo[4] = {w[0][u].x, w[0][u].y, w[0][u].z, w[0][u].w};
-                const uint32_t hi[4] = {w[1][u].x, w[1][u].y, w[1][u].z, w[1][u].w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t x = BF16 ? lo[i] : lo[i] ^ 0x80808080u, y = BF16 ? hi[i] : hi[i] ^ 0x80808080u;
-                    a[4 * u + i][0] = weight_pair<BF16, false>(x);
-                    a[4 * u + i][1] = weight_pair<BF16, false>(y);
-                    a[4 * u + i][2] = weight_pair<BF16, true>(x);
-                    a[4 * u + i][3] = weight_pair<BF16, true>(y);
-                }
-            }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 if (t >= tiles) break;
-                const uint8_t* v = values + row[t] + c * P * moe::PIECE_BYTES + q * 16;
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint4 (&bt)[D][2] = b[t % EARLY];
+                if (t >= EARLY) load_digits(bt, v + row[t]);
 #pragma unroll
-                for (int piece = P - 1; piece >= 0; piece--) {  // the smallest first
-                    uint4 b[4];
+                for (int j = 0; j < 2; j++) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        b[j] = *reinterpret_cast<const uint4*>(v + piece * moe::PIECE_BYTES + j * 64);
+                    for (int m = 0; m < MT; m++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        moe_mma<BF16>(s, a[2 * j], b[j].x, b[j].y);
-                        moe_mma<BF16>(s, a[2 * j + 1], b[j].z, b[j].w);
-                    }
+                        for (int d = 0; d < D; d++) moe_mma(acc[m][t][d], a[m][2 * j], bt[d][j].x, bt[d][j].y);
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int d = 0; d < D; d++) moe_mma(acc[m][t][d], a[m][2 * j + 1], bt[d][j].z, bt[d][j].w);
                 }
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[t][i] += s[i];
+                // Every row part has been an operand, so the slot's reads are done: a box loaded over it any earlier could
+                // overtake reads that still wait in line behind the digits' loads.
+                if (t == 0) {
+                    __syncwarp();
+                    issue();
+                }
             }
         }
         return true;
     }
 
-    // Phase 1's results: rows g and g + 8 of the unit times their scales; the hidden values as pieces.
-    template <int PH>
-    __device__ __forceinline__ void finish_in(int unit, const float (&acc)[NT][4]) {
+    // The digits' sums as one exact sum.
+    __device__ __forceinline__ static long long whole(const int (&acc)[D][4], int i) {
+        long long sum = acc[D - 1][i];
+#pragma unroll
+        for (int d = D - 2; d >= 0; d--) sum = sum * 256 + acc[d][i];
+        return sum;
+    }
+
+    // The scales of rows g and g + 8 of a unit's tiles. Asked for before its products and (volatile) not later: behind the
+    // weights queued in DRAM such a load takes some 3 us.
+    __device__ __forceinline__ void scales(int phase, const MoeGroup& grp, int block) {
+        const MoeLaunch& L = p.L;
+        const bool halves = phase == 0 && L.gated;
+        const int size = phase == 0 ? L.expert : L.model;
+        const int other = halves ? size : 8;
+        const float* s = (phase == 0 ? L.in_scale : L.out_scale) + static_cast<int64_t>(grp.expert) * (halves ? 2 : 1) * size;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const int r = (block * MT + m) * (halves ? 8 : 16) + (lane >> 2);
+            scale[m] = make_float2(0.0f, 0.0f);
+            if (r < size) asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(scale[m].x) : "l"(s + r));
+            if (halves ? r < size : r + 8 < size) asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(scale[m].y) : "l"(s + r + other));
+        }
+    }
+
+    // Phase 1's results: the hidden values and each pair's largest.
+    __device__ __forceinline__ void finish_in(const MoeGroup& grp, int block, const long long (&sum)[MT][NT][4]) {
         const MoeLaunch& L = p.L;
         const int g = lane >> 2, q = lane & 3;
-        const MoeGroup grp = sh.group[unit / p.blocks_in];
-        const int block = unit % p.blocks_in;
-        const int j0 = L.gated ? block * 8 + g : block * 16 + g;
-        const int64_t rows = static_cast<int64_t>(L.gated ? 2 : 1) * L.expert;
-        const float* scale = L.in_scale + grp.expert * rows;
-        const float s0 = j0 < L.expert ? __ldg(scale + j0) : 0.0f;
-        const int j1 = L.gated ? j0 + L.expert : j0 + 8;
-        const float s1 = (L.gated ? j0 < L.expert : j1 < L.expert) ? __ldg(scale + j1) : 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
+            if (8 * t >= grp.count) break;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int n = 8 * t + 2 * q + i;
+                const int pair = sh.order[grp.first + min(n, grp.count - 1)];
+                const int shift = sh.shift[pair];
+                float* hidden = L.hidden + static_cast<int64_t>(pair) * L.expert;
+                uint32_t most = 0;
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const int j0 = (block * MT + m) * (L.gated ? 8 : 16) + g;
+                    float h[2] = {shifted_back(sum[m][t][i], shift) * scale[m].x,
+                                  shifted_back(sum[m][t][2 + i], shift) * scale[m].y};
+                    if (L.gated) {
+                        float f[1] = {h[0]};
+                        activate_all(f, L.activation);
+                        h[0] = f[0] * h[1];
+                    } else {
+                        activate_all(h, L.activation);
+                        if (n < grp.count && j0 + 8 < L.expert) {
+                            hidden[j0 + 8] = h[1];
+                            most = max(most, __float_as_uint(h[1]) & 0x7FFFFFFFu);
+                        }
+                    }
+                    if (n < grp.count && j0 < L.expert) {
+                        hidden[j0] = h[0];
+                        most = max(most, __float_as_uint(h[0]) & 0x7FFFFFFFu);
+                    }
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+                if (g == 0 && n < grp.count) atomicMax(&sh.most[pair], most);
+            }
+        }
+    }
+
+    // Phase 2's results: the pair's weight times the row's scale times the sum.
+    __device__ __forceinline__ void finish_out(const MoeGroup& grp, int block, const long long (&sum)[MT][NT][4]) {
+        const MoeLaunch& L = p.L;
+        const int g = lane >> 2, q = lane & 3;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (8 * t >= grp.count) break;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int n = 8 * t + 2 * q + i;
                 if (n >= grp.count) continue;
                 const int pair = sh.order[grp.first + n];
-                float h[2] = {acc[t][i] * s0, acc[t][2 + i] * s1};
-                if (L.gated) {
-                    float f[1] = {h[0]};
-                    activate_all(f, L.activation);
-                    if (j0 < L.expert) put_hidden<PH>(pair, j0, f[0] * h[1]);
-                } else {
-                    activate_all(h, L.activation);
-                    if (j0 < L.expert) put_hidden<PH>(pair, j0, h[0]);
-                    if (j1 < L.expert) put_hidden<PH>(pair, j1, h[1]);
+                const int shift = sh.shift[pair];
+                const float weight = sh.weight[pair];
+                float* to = L.outputs + static_cast<int64_t>(pair) * L.model;
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const int d0 = (block * MT + m) * 16 + g;
+                    if (d0 < L.model) to[d0] = weight * (shifted_back(sum[m][t][i], shift) * scale[m].x);
+                    if (d0 + 8 < L.model) to[d0 + 8] = weight * (shifted_back(sum[m][t][2 + i], shift) * scale[m].y);
                 }
             }
         }
     }
 
-    template <int PH>
-    __device__ __forceinline__ void put_hidden(int pair, int j, float v) {
-        uint16_t piece[PH];
-        to_pieces<PH>(v, piece);
-        const int k = j % moe::CHUNK;
-        uint8_t* to = p.L.h_pieces + (static_cast<int64_t>(pair) * p.chunks_out + j / moe::CHUNK) * PH * moe::PIECE_BYTES +
-                      (k % 32) / 8 * 64 + k / 32 * 16 + (k % 8) * 2;
-#pragma unroll
-        for (int s = 0; s < PH; s++) *reinterpret_cast<uint16_t*>(to + s * moe::PIECE_BYTES) = piece[s];
+    __device__ __forceinline__ long long* segment(int warp, int which) const {
+        return p.L.segments + (static_cast<int64_t>(blockIdx.x * S::WARPS + warp) * 2 + which) * S::SUMS;
     }
 
-    // Phase 2's results: the pair's weight times the row's scale times the sum.
-    __device__ __forceinline__ void finish_out(int unit, const float (&acc)[NT][4]) {
-        const MoeLaunch& L = p.L;
-        const int g = lane >> 2, q = lane & 3;
-        const MoeGroup grp = sh.group[unit / p.blocks_out];
-        const int d0 = (unit % p.blocks_out) * 16 + g;
-        const float* scale = L.out_scale + static_cast<int64_t>(grp.expert) * L.model;
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int d = d0 + 8 * r;
-            if (d >= L.model) continue;
-            const float s = __ldg(scale + d);
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int n = 8 * t + 2 * q + i;
-                    if (n >= grp.count) continue;
-                    const int pair = sh.order[grp.first + n];
-                    L.outputs[static_cast<int64_t>(pair) * L.model + d] = sh.weight[pair] * (acc[t][2 * r + i] * s);
-                }
-        }
-    }
-
-    __device__ __forceinline__ float* segment(int warp, int which) const {
-        return p.L.segments + (static_cast<int64_t>(blockIdx.x * moe::WARPS + warp) * 2 + which) * moe_segment_floats<NT>();
-    }
-
-    // The warp's range of one phase. False when a wait gave up.
-    template <int PHASE, bool BF16, int P, int PH>
-    __device__ __forceinline__ bool run(int warp) {
-        const MoeRange r = range[PHASE];
-        const int c = chunks(PHASE), total = r.units * c;
-        const uint8_t* values = PHASE == 0 ? p.L.x_pieces : p.L.h_pieces;
-        const uint32_t row_bytes = static_cast<uint32_t>(c) * P * moe::PIECE_BYTES;
+    // The warp's range of one phase. False (for the whole CTA) when a wait gave up.
+    __device__ __forceinline__ bool run(int phase) {
+        const MoeRange r = phase == 0 ? range_in : range_out;
+        const int c = chunks(phase), per_group = blocks(phase), total = (r.units - r.tail) * c;
+        const uint8_t* values = phase == 0 ? p.L.x_digits : p.L.h_digits;
+        const uint32_t row_bytes = static_cast<uint32_t>(c) * D * moe::CHUNK;
         const int g = lane >> 2;
-        for (int at = r.at; at < r.end;) {
-            const int local = at / c, c0 = at - local * c, c1 = min(c, c0 + r.end - at);
-            const int unit = r.u0 + local;
-            const MoeGroup grp = sh.group[unit / blocks(PHASE)];
-            const int tiles = (grp.count + 7) / 8;
-            uint32_t row[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {  // columns past the group's pairs repeat its last one and are not stored
-                const int pair = sh.order[grp.first + min(8 * t + g, grp.count - 1)];
-                row[t] = static_cast<uint32_t>(PHASE == 0 ? pair / p.L.top_k : pair) * row_bytes;
-            }
-            float acc[NT][4];
-            if (!products<BF16, P>(values, row, tiles, c0, c1, acc)) break;  // the abort flag is up
-            if (c0 == 0 && c1 == c) {
-                if constexpr (PHASE == 0)
-                    finish_in<PH>(unit, acc);
-                else
-                    finish_out(unit, acc);
+        // The unit that this warp's run cuts at its end, if the run holds its start: finished after the others.
+        int local = (r.end - 1) / c;
+        const int cut = r.at < r.end && local * c >= r.at && local * c + c > r.end ? local : -1;
+        int round = 0, at = r.at;
+        bool last_pass = false;
+#pragma unroll 1
+        while (true) {
+            // A pass: a segment of a unit (its sums, to be finished or left in `segments`), then, once all warps are
+            // through theirs, the cut unit.
+            int c0 = 0, c1 = c, unit;
+            const bool in_round = round < r.rounds;
+            if (in_round) {
+                unit = r.u0 + round * S::WARPS + warp;
+            } else if (at < r.end) {
+                local = at / c;
+                c0 = at - local * c;
+                c1 = min(c, c0 + r.end - at);
+                unit = r.u0 + r.tail + local;
             } else {
-                float4* to = reinterpret_cast<float4*>(segment(warp, at == r.at ? 0 : 1)) + lane;
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-                    if (t < tiles) to[32 * t] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+                if (last_pass) break;
+                last_pass = true;
+                __syncthreads();
+                if (sh.abort || cut < 0) break;
+                unit = r.u0 + r.tail + cut;
             }
-            at += c1 - c0;
-        }
-        __syncthreads();
-        if (sh.abort) return false;
-        // A cut unit is finished by the warp that holds its start: its own segment is its last one (or, starting at its
-        // range's start, its first), the others' are their first.
-        if (r.at < r.end) {
-            const int local = (r.end - 1) / c, i0 = local * c;
-            if (i0 >= r.at && i0 + c > r.end) {
-                const int unit = r.u0 + local;
-                const int tiles = (sh.group[unit / blocks(PHASE)].count + 7) / 8;
-                const int last = moe_owner(i0 + c - 1, total);
-                float acc[NT][4];
+            const int group = unit / per_group, block = unit - group * per_group;
+            const MoeGroup grp = sh.group[group];
+            const int tiles = (grp.count + 7) / 8;
+            const bool is_whole = c1 - c0 == c;
+            if (!last_pass && (is_whole || (!in_round && local == cut))) scales(phase, grp, block);  // a cut one's is kept
+            long long sum[MT][NT][4];
+            if (!last_pass) {
+                uint32_t row[NT];
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                for (int t = 0; t < NT; t++) {  // columns past the group's pairs repeat its last one and are not stored
+                    const int pair = sh.order[grp.first + min(8 * t + g, grp.count - 1)];
+                    row[t] = static_cast<uint32_t>(phase == 0 ? pair / p.L.top_k : pair) * row_bytes;
+                }
+                int acc[MT][NT][D][4];
+                if (!products(values, row, tiles, phase == 0 && p.L.gated, c0, c1, acc)) {  // the abort flag is up
+                    round = r.rounds;
+                    at = r.end;
+                    continue;
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][i] = 0.0f;
-                for (int w = warp; w <= last; w++) {
-                    if (moe_split(total, w, moe::WARPS) == moe_split(total, w + 1, moe::WARPS)) continue;  // no share
-                    const float4* from = reinterpret_cast<const float4*>(segment(w, w == warp && i0 != r.at ? 1 : 0)) + lane;
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sum[m][t][i] = whole(acc[m][t], i);
+                if (!is_whole) {
+                    longlong2* to = reinterpret_cast<longlong2*>(segment(warp, at == r.at ? 0 : 1)) + lane;
 #pragma unroll
                     for (int t = 0; t < NT; t++)
                         if (t < tiles) {
-                            const float4 v = from[32 * t];
-                            acc[t][0] += v.x;
-                            acc[t][1] += v.y;
-                            acc[t][2] += v.z;
-                            acc[t][3] += v.w;
+#pragma unroll
+                            for (int m = 0; m < MT; m++) {
+                                to[64 * (MT * t + m)] = make_longlong2(sum[m][t][0], sum[m][t][1]);
+                                to[64 * (MT * t + m) + 32] = make_longlong2(sum[m][t][2], sum[m][t][3]);
+                            }
                         }
                 }
-                if constexpr (PHASE == 0)
-                    finish_in<PH>(unit, acc);
+                if (in_round)
+                    round++;
                 else
-                    finish_out(unit, acc);
+                    at += c1 - c0;
+                if (!is_whole) continue;
+            } else {
+                // Its own segment is its last one (or, starting at its range's start, its first), the others' their first.
+                const int i0 = cut * c, last = moe_owner<S>(i0 + c - 1, total);
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sum[m][t][i] = 0;
+#pragma unroll 1
+                for (int w = warp; w <= last; w++) {
+                    if (moe_split(total, w, S::WARPS) == moe_split(total, w + 1, S::WARPS)) continue;  // no share
+                    const longlong2* from =
+                        reinterpret_cast<const longlong2*>(segment(w, w == warp && i0 != r.at ? 1 : 0)) + lane;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+                        if (t < tiles) {
+#pragma unroll
+                            for (int m = 0; m < MT; m++) {
+                                const longlong2 u = from[64 * (MT * t + m)], v = from[64 * (MT * t + m) + 32];
+                                sum[m][t][0] += u.x;
+                                sum[m][t][1] += u.y;
+                                sum[m][t][2] += v.x;
+                                sum[m][t][3] += v.y;
+                            }
+                        }
+                }
             }
+            if (phase == 0)
+                finish_in(grp, block, sum);
+            else
+                finish_out(grp, block, sum);
         }
-        return true;
+        return sh.abort == 0;
     }
 
     // Waits (bounded) for boxes still in flight: none may land after the CTA has gone.
@@ -683,64 +1009,98 @@ struct MoeWarp {
     }
 };
 
-template <bool HALF, int NT>
-__global__ void __launch_bounds__(moe::THREADS, 1)
+template <bool HALF, class S>
+__global__ void __launch_bounds__(S::THREADS, 1)
     moe_fused_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_out,
                      const __grid_constant__ MoeFusedParams p) {
-    constexpr int PX = HALF ? 1 : 3, PH = HALF ? 2 : 3;
+    constexpr int D = HALF ? 3 : 4;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    MoeShared<NT>& sh = *reinterpret_cast<MoeShared<NT>*>(smem + moe::WARPS * moe::SLOTS * moe::BOX);
+    MoeShared<S>& sh = *reinterpret_cast<MoeShared<S>*>(smem + S::RING);
     const MoeLaunch& L = p.L;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_trigger();
     if (threadIdx.x == 0) {
-        for (int w = 0; w < moe::WARPS; w++)
+        for (int w = 0; w < S::WARPS; w++)
             for (int s = 0; s < moe::SLOTS; s++) mbar_init(&sh.full[w][s], 1);
         sh.abort = 0;
         sh.failed = 0;
+        sh.complete = 0;
         fence_mbar_init();
         prefetch_tmap(&map_in);
         prefetch_tmap(&map_out);
     }
     pdl_wait();
-    moe_split_x<PX, PH>(p);
-    moe_logits(L, sh);
-    if (!grid_barrier(sh, L.arrivals)) {
-        if (threadIdx.x == 0) {
-            grid_arrive(L.arrivals, false);
-            grid_arrive(L.arrivals, false);
-            atomicExch(L.error_flag, 1);
+    for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS) sh.most[i] = 0;
+    if (p.vec)
+        moe_digits_x<S, HALF, true>(p);
+    else
+        moe_digits_x<S, HALF, false>(p);
+    if (!p.vec)
+        L.router_half ? moe_logits<S, HALF, false, true>(p, sh) : moe_logits<S, HALF, false, false>(p, sh);
+    else
+        L.router_half ? moe_logits<S, HALF, true, true>(p, sh) : moe_logits<S, HALF, true, false>(p, sh);
+    if (L.tokens > S::WARPS) {
+        __syncthreads();
+        __threadfence();  // the other CTAs' logits of the blocks completed here
+        for (unsigned left = sh.complete; left != 0; left &= left - 1) {
+            const int t0 = 8 * (__ffs(left) - 1);
+            moe_choose_tokens<S, D>(L, sh, t0, min(8, L.tokens - t0), true);
         }
+    }
+    // Four grid barriers; a CTA that leaves early still arrives at the ones it skips.
+    if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
+        leave_early(L, 3);
         return;
     }
-    for (int t = warp; t < L.tokens; t += moe::WARPS) moe_choose(L, sh, t, blockIdx.x == 0);
-    __syncthreads();
-    moe_group<NT>(L, sh);
+    if (L.tokens <= S::WARPS) {
+        moe_choose_tokens<S, D>(L, sh, 0, L.tokens, blockIdx.x == 0);
+    } else {
+        for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS) {
+            sh.id[i] = static_cast<uint16_t>(__ldcg(L.ids + i));
+            sh.weight[i] = __ldcg(L.weights + i);
+            sh.shift[i] = shift_or_not<D>(__ldcg(L.x_most + i / L.top_k));
+        }
+    }
+    moe_group(L, sh);
 
-    MoeWarp<NT> me{p, sh, {&map_in, &map_out}, smem + warp * moe::SLOTS * moe::BOX, sh.full[warp], lane, {}, {}, 0};
-    me.range[0] = moe_range(sh.groups * p.blocks_in, p.chunks_in, warp);
-    me.range[1] = moe_range(sh.groups * p.blocks_out, p.chunks_out, warp);
-    me.feed = MoeFeed{0, me.range[0].at, me.range[0].end, 0};
+    MoeWarp<S, D> me{p, sh, &map_in, &map_out, smem + warp * moe::SLOTS * S::BOX, sh.full[warp], warp, lane, {}, {}, {}, 0, {}};
+    me.range_in = moe_range<S>(sh.groups * p.blocks_in, p.chunks_in, warp);
+    me.range_out = moe_range<S>(sh.groups * p.blocks_out, p.chunks_out, warp);
     for (int s = 0; s < moe::SLOTS; s++) me.issue();
 
-    bool ok = me.template run<0, !HALF, PX, PH>(warp);
-    ok = grid_barrier(sh, L.arrivals) && ok;
-    if (ok) ok = me.template run<1, true, PH, PH>(warp);
-    me.drain();
-    if (sh.failed) {  // the same for every thread
-        if (threadIdx.x == 0) {
-            grid_arrive(L.arrivals, false);
-            atomicExch(L.error_flag, 1);
+#pragma unroll 1
+    for (int phase = 0; phase < 2; phase++) {
+        const bool ok = me.run(phase);
+        if (phase == 1) break;
+        if (ok) {
+            __syncthreads();  // every warp's largest values are in
+            for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS)
+                if (sh.most[i] != 0) atomicMax(L.h_most + i, sh.most[i]);
         }
+        if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
+            me.drain();
+            leave_early(L, 2);
+            return;
+        }
+        moe_digits_h<S, D>(p);
+        if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
+            me.drain();
+            leave_early(L, 1);
+            return;
+        }
+        for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS)
+            sh.shift[i] = shift_or_not<D>(__ldcg(L.h_most + i));
+        __syncthreads();
+    }
+    me.drain();
+    if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
+        leave_early(L, 0);
         return;
     }
-    if (!grid_barrier(sh, L.arrivals)) {
-        if (threadIdx.x == 0) atomicExch(L.error_flag, 1);
-        return;
-    }
+    if (blockIdx.x == 0 && threadIdx.x == 0 && L.tokens > S::WARPS) clear_tickets(L);
     const int total = L.tokens * L.model / 4;  // model is a multiple of 16
-    for (int i = blockIdx.x * moe::THREADS + threadIdx.x; i < total; i += gridDim.x * moe::THREADS) {
+    for (int i = blockIdx.x * S::THREADS + threadIdx.x; i < total; i += gridDim.x * S::THREADS) {
         const int t = i / (L.model / 4), d = (i - t * (L.model / 4)) * 4;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k = 0; k < L.top_k; k++) {
@@ -768,7 +1128,18 @@ __global__ void __launch_bounds__(moe::THREADS, 1)
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 
-static int moe_tiles(const MoeLaunch& L) { return L.tokens <= 8 ? 1 : 4; }
+// The shape of a launch: NT and MT.
+struct MoeChoice {
+    int nt, mt, warps;
+};
+
+// Groups of 8 columns hold all of an expert's tokens up to 8 tokens; groups of 16 most of them while the experts see 10
+// on average at most.
+static MoeChoice moe_choice(const MoeLaunch& L) {
+    if (L.tokens <= 2) return {1, 1, moe::Shape<1, 1>::WARPS};
+    const int nt = L.tokens <= 8 ? 1 : L.tokens * L.top_k <= 10 * L.experts ? 2 : 4;
+    return {nt, 2, moe::Shape<1, 2>::WARPS};
+}
 
 static int chunks_of(int size) { return (size + moe::CHUNK - 1) / moe::CHUNK; }
 
@@ -781,20 +1152,24 @@ MoeFusedSizes moe_fused_sizes(const MoeLaunch& L) {
     const int64_t pairs = int64_t(L.tokens) * L.top_k;
     MoeFusedSizes s;
     s.logits = int64_t(L.tokens) * L.experts * 4;
-    s.x_pieces = int64_t(L.tokens) * chunks_of(L.model) * (L.x_half ? 1 : 3) * moe::PIECE_BYTES;
-    s.h_pieces = pairs * chunks_of(L.expert) * (L.x_half ? 2 : 3) * moe::PIECE_BYTES;
+    const int digits = L.x_half ? 3 : 4;
+    s.x_digits = int64_t(L.tokens) * chunks_of(L.model) * digits * moe::CHUNK;
+    s.h_digits = pairs * chunks_of(L.expert) * digits * moe::CHUNK;
+    s.x_most = int64_t(L.tokens) * 4;
+    s.h_most = pairs * 4;
     s.outputs = pairs * L.model * 4;
-    s.segments = int64_t(L.num_sms) * moe::WARPS * 2 * moe::ROWS * 8 * moe_tiles(L) * 4;
+    const MoeChoice shape = moe_choice(L);
+    s.segments = int64_t(L.num_sms) * shape.warps * 2 * (16 * shape.mt) * (8 * shape.nt) * int64_t(sizeof(long long));
     return s;
 }
 
-template <bool HALF, int NT>
+template <bool HALF, class S>
 static std::function<cudaError_t(cudaStream_t)> bind_moe(const MoeFusedParams& p, const CUtensorMap& in,
                                                          const CUtensorMap& out) {
     return [=](cudaStream_t stream) -> cudaError_t {
         static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
-        auto kern = moe_fused_kernel<HALF, NT>;
-        constexpr size_t smem = moe_smem_bytes<NT>();
+        auto kern = moe_fused_kernel<HALF, S>;
+        constexpr size_t smem = moe_smem_bytes<S>();
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
@@ -806,7 +1181,7 @@ static std::function<cudaError_t(cudaStream_t)> bind_moe(const MoeFusedParams& p
         }
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(p.L.num_sms));
-        cfg.blockDim = dim3(moe::THREADS);
+        cfg.blockDim = dim3(S::THREADS);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = stream;
         cudaLaunchAttribute attr[1];
@@ -826,18 +1201,30 @@ std::function<cudaError_t(cudaStream_t)> prepare_moe_fused(const MoeLaunch& L, c
     p.L = L;
     p.chunks_in = chunks_of(L.model);
     p.chunks_out = chunks_of(L.expert);
-    p.blocks_in = L.gated ? (L.expert + 7) / 8 : (L.expert + 15) / 16;
-    p.blocks_out = (L.model + 15) / 16;
+    const MoeChoice shape = moe_choice(L);
+    const int rows_in = (L.gated ? 8 : 16) * shape.mt, rows_out = 16 * shape.mt;
+    p.blocks_in = (L.expert + rows_in - 1) / rows_in;
+    p.blocks_out = (L.model + rows_out - 1) / rows_out;
+    const int64_t router_units = int64_t(L.experts) * ((L.tokens + 7) / 8);
+    p.router_split = 1;
+    while (p.router_split < shape.warps && router_units * p.router_split * 2 <= int64_t(L.num_sms) * shape.warps)
+        p.router_split *= 2;
+    auto four = [](const void* q, int half) { return (reinterpret_cast<uintptr_t>(q) & (half ? 7 : 15)) == 0; };
+    p.vec = four(L.x, L.x_half) && four(L.router, L.router_half);  // model is a multiple of 16
     const uint64_t d = L.model, f = L.expert, e = L.experts;
     CUtensorMap in, out;
-    const bool ok = make_tensor_map_u8(&in, L.w_in, d, f, (L.gated ? 2 : 1) * e, d, d * f, moe::CHUNK, L.gated ? 8 : 16,
+    const bool ok = make_tensor_map_u8(&in, L.w_in, d, f, (L.gated ? 2 : 1) * e, d, d * f, moe::CHUNK, rows_in,
                                        L.gated ? 2 : 1) &&
-                    make_tensor_map_u8(&out, L.w_out, f, d, e, f, d * f, moe::CHUNK, 16);
+                    make_tensor_map_u8(&out, L.w_out, f, d, e, f, d * f, moe::CHUNK, rows_out);
     *err = ok ? cudaSuccess : cudaErrorInvalidValue;
     if (!ok) return nullptr;
-    const bool one = moe_tiles(L) == 1;
-    if (L.x_half) return one ? bind_moe<true, 1>(p, in, out) : bind_moe<true, 4>(p, in, out);
-    return one ? bind_moe<false, 1>(p, in, out) : bind_moe<false, 4>(p, in, out);
+    using moe::Shape;
+    if (shape.mt == 1) return L.x_half ? bind_moe<true, Shape<1, 1>>(p, in, out) : bind_moe<false, Shape<1, 1>>(p, in, out);
+    switch (shape.nt) {
+        case 1: return L.x_half ? bind_moe<true, Shape<1, 2>>(p, in, out) : bind_moe<false, Shape<1, 2>>(p, in, out);
+        case 2: return L.x_half ? bind_moe<true, Shape<2, 2>>(p, in, out) : bind_moe<false, Shape<2, 2>>(p, in, out);
+        default: return L.x_half ? bind_moe<true, Shape<4, 2>>(p, in, out) : bind_moe<false, Shape<4, 2>>(p, in, out);
+    }
 }
 
 }  // namespace og

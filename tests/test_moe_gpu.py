@@ -304,3 +304,49 @@ def test_captured_replayed_and_repeated(device):
             g.dispose()
         for layer in layers:
             layer.dispose()
+
+
+@pytest.mark.parametrize("tokens,model,expert,experts,top_k,half", [(40, 2048, 1408, 48, 6, True),
+                                                                    (1, 4096, 4096, 12, 8, True),
+                                                                    (6, 2048, 2048, 24, 4, False)])
+def test_layers_that_keep_dram_busy(device, tokens, model, expert, experts, top_k, half):
+    """Weights far larger than L2, so that every load waits behind others: some tokens against the formula, and the same
+    bits in every run."""
+    rng = np.random.default_rng(tokens)
+    kind = np.float16 if half else np.float32
+    x = rng.standard_normal((tokens, model)).astype(kind)
+    router = (rng.standard_normal((experts, model)) * 2 / np.sqrt(model)).astype(np.float32)
+    w_in = rng.integers(-128, 128, (experts, 2 * expert, model), dtype=np.int8)
+    w_out = rng.integers(-128, 128, (experts, model, expert), dtype=np.int8)
+    in_scale = (rng.uniform(0.5, 1.5, (experts, 2 * expert)) / (74 * np.sqrt(model))).astype(np.float32)
+    out_scale = (rng.uniform(0.5, 1.5, (experts, model)) / (74 * np.sqrt(expert))).astype(np.float32)
+    bufs = [device.create_buffer(a.dtype, a.reshape(-1)) for a in (x, router, w_in, in_scale, w_out, out_scale)]
+    y, ids = device.create_buffer(kind, tokens * model), device.create_buffer(np.int32, tokens * top_k)
+    with og.Int8MoeKernels(device) as moe:
+        first = None
+        for _ in range(12):
+            y.fill(0xFF)
+            enc = device.begin_commands()
+            moe.encode(enc, og.MoeProblem(tokens, model, expert, experts, top_k), *bufs, y, expert_ids=ids)
+            device.submit(enc)
+            got = y.read()
+            first = got if first is None else first
+            assert np.array_equal(first.view(np.uint8), got.view(np.uint8))
+    chosen = ids.read().reshape(tokens, top_k)
+    for b in bufs + [y, ids]:
+        b.dispose()
+    logits = x.astype(np.float64) @ router.astype(np.float64).T
+    assert np.array_equal(chosen, np.argsort(-logits, axis=1, kind="stable")[:, :top_k])
+    for t in sorted({0, tokens // 2, tokens - 1}):
+        p = np.exp(logits[t, chosen[t]] - logits[t].max())
+        p /= p.sum()
+        want, size = np.zeros(model), np.zeros(model)
+        for k, e in enumerate(chosen[t]):
+            u = (w_in[e].astype(np.float32) @ x[t].astype(np.float64)) * in_scale[e]
+            h = activate64(u[:expert], og.ACTIVATION_SILU) * u[expert:]
+            part = p[k] * (w_out[e].astype(np.float32) @ h) * out_scale[e]
+            want += part
+            size += np.abs(part)
+        # below 2^-20 of the parts and of their root mean square, and one rounding of the result
+        tol = 2.0 ** -20 * (size + np.sqrt(np.mean(size ** 2))) + np.abs(want) * 2.0 ** (-11 if half else -24)
+        assert np.all(np.abs(first.reshape(tokens, model)[t].astype(np.float64) - want) <= tol + 1e-7), t
