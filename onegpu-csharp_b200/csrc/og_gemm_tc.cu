@@ -28,6 +28,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "og_gemm.h"
 #include "og_kernels.cuh"
@@ -40,9 +41,6 @@ constexpr int BN = 256;
 constexpr int BK = 128;                    // bytes of K per stage = one 128-byte swizzle row
 constexpr int NUM_ACC = 2;
 constexpr int TMEM_COLS = NUM_ACC * BN;    // 512: all of TMEM
-constexpr int EPI_WARPS = 8;               // two per TMEM lane quadrant, each taking half of the tile's columns
-constexpr int EPI_THREADS = 32 * EPI_WARPS;
-constexpr int THREADS = 64 + EPI_THREADS;  // producer, MMA, epilogue warps
 // Output tiles per raster group along M: 16 when there are at least 32 tile rows, 8 otherwise. A group walks its
 // rows of A against every column tile of B, so taller groups read B fewer times. Measured on B200, 8192^3 took
 // 319.4-320.4 us with 16 against 323.6 us with 8 (12, 20, 24 and 32 were 1-16 us slower than 16), while 4096^3
@@ -54,15 +52,25 @@ constexpr int GROUP_M_TALL = 16;
 // CG = 1: one CTA computes a 128 x 256 tile. CG = 2: a CTA pair computes a 256 x 256 tile with tcgen05.mma
 // cta_group::2; each CTA stages its own 128 rows of A and its own 128 columns of B, so every SM pulls 32 KB per
 // K block instead of 48 KB.
-template <int CG>
+//
+// Epilogue warps: two per TMEM lane quadrant, each taking half of the tile's columns, or four for the activated form (ACT),
+// each a quarter: its work per element (28 instructions, two of them exponentials or quotients at a quarter of the
+// rate) fits beside the MMAs of the next tile only with four warps to hide one another's latency on each scheduler. Their
+// boxes and the second set of column terms, filled while the accumulator is awaited, cost one stage of the operand ring.
+// 8192 x 8192 x 2048 into float32 with tanh GELU took 167 us with 8 warps and six stages, ACT_US with 16 and five.
+template <int CG, bool ACT = false>
 struct Cfg {
+    static constexpr int EPI_WARPS = ACT ? 16 : 8;
+    static constexpr int EPI_THREADS = 32 * EPI_WARPS;
+    static constexpr int THREADS = 64 + EPI_THREADS;      // producer, MMA, epilogue warps
+    static constexpr int EPI_CHUNKS = BN / 32 / (EPI_WARPS / 4);  // 32-column chunks of one epilogue warp
     static constexpr int BM = 128 * CG;
     static constexpr int A_BYTES = 128 * BK;          // 16 KB per CTA
     static constexpr int B_COLS = BN / CG;            // columns of B staged by one CTA
     static constexpr int B_BYTES = B_COLS * BK;       // 32 KB or 16 KB per CTA
     static constexpr int B_BOX = 128 * BK;            // one 128-column box of an MN-major B
-    static constexpr int STAGES = CG == 1 ? 4 : 6;
-    static constexpr int TERMS_BYTES = 5 * 4 * BN;     // per-column epilogue terms
+    static constexpr int STAGES = (CG == 1 ? 4 : 6) - (ACT ? 1 : 0);
+    static constexpr int TERMS_BYTES = (ACT ? 2 : 1) * 5 * 4 * BN;  // per-column epilogue terms
     static constexpr int BOX_BYTES = 32 * 64;          // one 32-row x 16-word store box (64-byte rows)
     static constexpr int BOXES = 1;                    // store boxes per epilogue warp
     static constexpr int STAGING_BYTES = EPI_WARPS * BOXES * BOX_BYTES;
@@ -242,6 +250,18 @@ __device__ __forceinline__ void sk_add(const int32_t* slot_smem, int c, int row,
     }
 }
 
+// The same for half h of the chunk: 16 of its columns.
+__device__ __forceinline__ void sk_add_16(const int32_t* slot_smem, int c, int h, int row, uint32_t (&r)[16]) {
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+        const int4 x = *reinterpret_cast<const int4*>(slot_smem + ((c * 8 + 4 * h + v) * 128 + row) * 4);
+        r[4 * v] += uint32_t(x.x);
+        r[4 * v + 1] += uint32_t(x.y);
+        r[4 * v + 2] += uint32_t(x.z);
+        r[4 * v + 3] += uint32_t(x.w);
+    }
+}
+
 template <int BM>
 __device__ __forceinline__ void tile_coords(const TcParams& p, int tile, int& b, int& tm, int& tn) {
     const int per_batch = p.tiles_m * p.tiles_n;
@@ -376,48 +396,59 @@ __device__ __forceinline__ void stage_half(const ColTerms& t, const Epilogue& e,
     }
 }
 
-// The activated form of N consecutive sums of one row (tile columns j0.., output element idx of the first; the first
-// `cols` of them inside the output).
-template <int OUT, int N>
-__device__ __forceinline__ void finish_activated(const ColTerms& t, const Epilogue& e, bool za_per_row, uint32_t za,
-                                                 uint32_t rt, float row_scale, int j0, int64_t idx, int cols,
-                                                 bool res_vec, const uint32_t* r, float (&f)[N]) {
+// ---- activated form -------------------------------------------------------------------------------------------------
+//
+// A warp finishes its 32 rows in boxes of 64-byte row segments (16 float32 or 32 float16 columns), one box of shared
+// memory in the layout of stage_half: residual in, results out. The residual arrives a box ahead in registers, read along
+// rows (four lanes per row, 64 consecutive bytes; a lane reading its own row would touch 32 lines per load), crosses the
+// box into the lanes' rows, and the results leave from the same box by TMA, or, where C's rows are not 16-byte
+// aligned, element by element along rows.
+template <int OUT>
+struct ActBox {
+    static constexpr int COLS = OUT == OUT_ACT_F16 ? 32 : 16;
+    static constexpr int SIZE = OUT == OUT_ACT_F16 ? 2 : 4;
+    static constexpr int UNIT = 16 / SIZE;  // columns of 16 bytes
+    using T = std::conditional_t<OUT == OUT_ACT_F16, unsigned short, unsigned int>;
+};
+
+// Bias-corrected, scaled, biased and activated values of N consecutive sums of one row (tile columns j0..). The column
+// terms are read four columns per 16-byte shared load.
+template <int N>
+__device__ __forceinline__ void activated_values(const ColTerms& t, const Epilogue& e, bool int_terms, bool za_per_row,
+                                                 uint32_t za, uint32_t rt, float row_scale, int j0, const uint32_t* r,
+                                                 float (&f)[N]) {
 #pragma unroll
-    for (int q = 0; q < N; q++)
-        f[q] = scaled_sum(tile_sum(t, za_per_row, za, rt, j0 + q, r[q]), row_scale, t.scale[j0 + q],
-                          e.float_bias != nullptr, t.fbias[j0 + q]);
-    activate_all(f, e.activation);
-    if (e.residual == nullptr) return;
-    if (res_vec && cols >= N) {
-        if constexpr (OUT == OUT_ACT_F16) {
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __half*>(e.residual) + idx);
-#pragma unroll
-            for (int q = 0; q < N; q += 8) {
-                const uint4 w = src[q / 8];
-                const uint32_t h[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[u]));
-                    f[q + 2 * u] = __fadd_rn(f[q + 2 * u], v.x);
-                    f[q + 2 * u + 1] = __fadd_rn(f[q + 2 * u + 1], v.y);
-                }
-            }
-        } else {
-            const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(e.residual) + idx);
-#pragma unroll
-            for (int q = 0; q < N; q += 4) {
-                const float4 v = src[q / 4];
-                f[q] = __fadd_rn(f[q], v.x);
-                f[q + 1] = __fadd_rn(f[q + 1], v.y);
-                f[q + 2] = __fadd_rn(f[q + 2], v.z);
-                f[q + 3] = __fadd_rn(f[q + 3], v.w);
+    for (int v = 0; v < N; v += 4) {
+        uint32_t s[4] = {r[v], r[v + 1], r[v + 2], r[v + 3]};
+        if (int_terms) {
+            const int4 zb = *reinterpret_cast<const int4*>(&t.zb[j0 + v]);
+            const int4 cc = *reinterpret_cast<const int4*>(&t.c[j0 + v]);
+            s[0] += uint32_t(zb.x) * rt + uint32_t(cc.x);
+            s[1] += uint32_t(zb.y) * rt + uint32_t(cc.y);
+            s[2] += uint32_t(zb.z) * rt + uint32_t(cc.z);
+            s[3] += uint32_t(zb.w) * rt + uint32_t(cc.w);
+            if (za_per_row) {
+                const int4 cs = *reinterpret_cast<const int4*>(&t.csb[j0 + v]);
+                s[0] -= za * uint32_t(cs.x);
+                s[1] -= za * uint32_t(cs.y);
+                s[2] -= za * uint32_t(cs.z);
+                s[3] -= za * uint32_t(cs.w);
             }
         }
-        return;
+        const float4 sc = *reinterpret_cast<const float4*>(&t.scale[j0 + v]);
+        f[v] = scaled_sum(s[0], row_scale, sc.x, false, 0.0f);
+        f[v + 1] = scaled_sum(s[1], row_scale, sc.y, false, 0.0f);
+        f[v + 2] = scaled_sum(s[2], row_scale, sc.z, false, 0.0f);
+        f[v + 3] = scaled_sum(s[3], row_scale, sc.w, false, 0.0f);
+        if (e.float_bias != nullptr) {
+            const float4 fb = *reinterpret_cast<const float4*>(&t.fbias[j0 + v]);
+            f[v] = __fadd_rn(f[v], fb.x);
+            f[v + 1] = __fadd_rn(f[v + 1], fb.y);
+            f[v + 2] = __fadd_rn(f[v + 2], fb.z);
+            f[v + 3] = __fadd_rn(f[v + 3], fb.w);
+        }
     }
-#pragma unroll
-    for (int q = 0; q < N; q++)
-        if (q < cols) f[q] = __fadd_rn(f[q], residual_at<OUT>(e, idx + q));
+    activate_all(f, e.activation);
 }
 
 // Two results as one word of float16.
@@ -426,37 +457,99 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One 64-byte row of a store box: 16 words in the 64-byte swizzle (see stage_half).
-__device__ __forceinline__ void stage_words(const uint32_t (&w)[16], uint8_t* box, int lane) {
-    const uint32_t row = smem_u32(box) + lane * 64;
-    const uint32_t sw = (lane >> 1) & 3;
+// The shared-memory address of 16-byte unit u of a box's row (64-byte swizzle, see stage_half).
+__device__ __forceinline__ uint32_t box_unit(uint32_t box, int row, int u) {
+    return box + row * 64 + ((u ^ ((row >> 1) & 3)) << 4);
+}
+
+__device__ __forceinline__ void st_shared_16(uint32_t addr, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// The residual of a box of rows row0.. and columns n0..: unit lane % 4 of rows lane / 4 + 8 i.
+template <int OUT>
+__device__ __forceinline__ void residual_box(const Epilogue& e, int64_t batch_at, int row0, int n0, int lane,
+                                             uint4 (&res)[4]) {
+    using B = ActBox<OUT>;
+    const int n = n0 + (lane & 3) * B::UNIT;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t addr = row + ((j ^ sw) << 4);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[4 * j]), "r"(w[4 * j + 1]),
-                     "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
-                     : "memory");
+    for (int i = 0; i < 4; i++) {
+        const int m = row0 + (lane >> 2) + 8 * i;
+        res[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (m < e.m && n < e.n)
+            res[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(e.residual) +
+                                                           (batch_at + static_cast<int64_t>(m) * e.ldc + n) * B::SIZE));
     }
 }
 
-// Stores 32 consecutive activated results of one row (output element idx, tile column j0, `cols` of them inside the
-// output) when the output's rows do not allow TMA stores.
+// Element `col` of a box's row.
 template <int OUT>
-__device__ __forceinline__ void store_chunk_activated(const ColTerms& t, const Epilogue& e, bool za_per_row, uint32_t za,
-                                                      uint32_t rt, float row_scale, int64_t idx, int j0, int cols,
-                                                      const uint32_t (&r)[32]) {
+__device__ __forceinline__ uint32_t box_element(uint32_t box, int row, int col) {
+    using B = ActBox<OUT>;
+    return box_unit(box, row, col / B::UNIT) + (col % B::UNIT) * B::SIZE;
+}
+
+// The same residual where 16-byte loads are not possible: straight into the box, along rows.
+template <int OUT>
+__device__ __forceinline__ void residual_elements(const Epilogue& e, int64_t batch_at, int row0, int n0, int lane,
+                                                  uint32_t box) {
+    using B = ActBox<OUT>;
+    using T = typename B::T;
+    constexpr int STEP = 32 / B::COLS;  // rows of one access; 16 accesses in flight
+    const int col = lane % B::COLS, n = n0 + col;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        float f[16];
-        finish_activated<OUT>(t, e, za_per_row, za, rt, row_scale, j0 + 16 * h, idx + 16 * h, cols - 16 * h, false,
-                              r + 16 * h, f);
+    for (int r0 = 0; r0 < 32; r0 += 16 * STEP) {
+        T v[16];
 #pragma unroll
-        for (int q = 0; q < 16; q++) {
-            if (16 * h + q >= cols) break;
+        for (int i = 0; i < 16; i++) {
+            const int m = row0 + r0 + i * STEP + lane / B::COLS;
+            v[i] = 0;
+            if (m < e.m && n < e.n)
+                v[i] = __ldcg(static_cast<const T*>(e.residual) + batch_at + static_cast<int64_t>(m) * e.ldc + n);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const uint32_t at = box_element<OUT>(box, r0 + i * STEP + lane / B::COLS, col);
             if constexpr (OUT == OUT_ACT_F16)
-                static_cast<__half*>(e.c)[idx + 16 * h + q] = __float2half_rn(f[q]);
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v[i]) : "memory");
             else
-                static_cast<float*>(e.c)[idx + 16 * h + q] = f[q];
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v[i]) : "memory");
+        }
+    }
+}
+
+// A box's results to C without TMA, along rows.
+template <int OUT>
+__device__ __forceinline__ void store_elements(const Epilogue& e, int64_t batch_at, int row0, int n0, int lane,
+                                               uint32_t box) {
+    using B = ActBox<OUT>;
+    using T = typename B::T;
+    constexpr int STEP = 32 / B::COLS;
+    const int col = lane % B::COLS, n = n0 + col;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 16 * STEP) {
+        T v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const uint32_t at = box_element<OUT>(box, r0 + i * STEP + lane / B::COLS, col);
+            if constexpr (OUT == OUT_ACT_F16)
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[i]) : "r"(at) : "memory");
+            else
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(at) : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int m = row0 + r0 + i * STEP + lane / B::COLS;
+            if (m < e.m && n < e.n) static_cast<T*>(e.c)[batch_at + static_cast<int64_t>(m) * e.ldc + n] = v[i];
         }
     }
 }
@@ -514,7 +607,7 @@ __device__ __forceinline__ void store_chunk(const ColTerms& t, const Epilogue& e
 template <int CG, bool B_MN, int OUT, bool SPLIT>
 __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CUtensorMap& tmap_b,
                                              const CUtensorMap& tmap_c, const TcParams& p, uint32_t idesc) {
-    using C = tc::Cfg<CG>;
+    using C = tc::Cfg<CG, out_activated(OUT)>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sA = smem;
@@ -548,7 +641,7 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
         }
         for (int a = 0; a < tc::NUM_ACC; a++) {
             mbar_init(&tfull[a], 1);
-            mbar_init(&tempty[a], tc::EPI_WARPS * CG);  // one arrival per epilogue warp of every CTA of the pair
+            mbar_init(&tempty[a], C::EPI_WARPS * CG);  // one arrival per epilogue warp of every CTA of the pair
         }
         mbar_init(sk_bar, 1);
         *abort_flag = 0;
@@ -677,13 +770,13 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
         }
     } else {
         // Epilogue: warp w reads TMEM lanes 32*(w%4) .. +31, i.e. rows 32*(w%4) + lane of this CTA's 128 rows; warps
-        // 2-5 take the tile's first 128 columns (chunks 0-3 of 32), warps 6-9 the other 128.
+        // 2-5 take the tile's first EPI_CHUNKS chunks of 32 columns, warps 6-9 the next, and so on.
         const int q = warp & 3;
         const int ew = warp - 2;
-        const int c_first = (ew >> 2) * (tc::BN / 64), c_end = c_first + tc::BN / 64;
+        const int c_first = (ew >> 2) * C::EPI_CHUNKS, c_end = c_first + C::EPI_CHUNKS;
         const uint32_t tempty_leader = CG == 2 ? mapa_shared(smem_u32(&tempty[0]), 0) : 0;
         const Epilogue& e = p.epi;
-        ColTerms& terms_smem = *reinterpret_cast<ColTerms*>(reinterpret_cast<uint8_t*>(bars) + 256);
+        ColTerms* terms_all = reinterpret_cast<ColTerms*>(reinterpret_cast<uint8_t*>(bars) + 256);
         // Column terms are needed unless the result is the raw int32 sum.
         const bool terms = OUT != OUT_I32 || e.za != nullptr || e.zb != nullptr || e.int_bias != nullptr;
         const bool za_per_row = e.za != nullptr && e.za_vector;
@@ -692,8 +785,8 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
             // turn) while the first MMAs run, then count the CTA in the launch's tally. C's rows start on 16-byte
             // boundaries and N is a multiple of 4 (the TMA-store condition), so whole 16-byte stores stay inside C.
             const int64_t rows_total = static_cast<int64_t>(p.total_tiles - p.dp_tiles) * C::BM;
-            for (int64_t r = static_cast<int64_t>(blockIdx.x) * tc::EPI_WARPS + ew; r < rows_total;
-                 r += static_cast<int64_t>(gridDim.x) * tc::EPI_WARPS) {
+            for (int64_t r = static_cast<int64_t>(blockIdx.x) * C::EPI_WARPS + ew; r < rows_total;
+                 r += static_cast<int64_t>(gridDim.x) * C::EPI_WARPS) {
                 int zb_, ztm, ztn;
                 tile_coords<C::BM>(p, p.dp_tiles + static_cast<int>(r / C::BM), zb_, ztm, ztn);
                 const int zm = ztm * C::BM + static_cast<int>(r % C::BM);
@@ -707,7 +800,7 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
             }
             __threadfence();
             fence_proxy_async_global();
-            asm volatile("bar.sync 1, %0;" ::"n"(tc::EPI_THREADS) : "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_THREADS) : "memory");
             if (threadIdx.x == 64) atomicAdd(p.tail_zeroed, 1u);
         }
         bool tail_ready = false;  // thread 64: the whole grid has cleared the tail
@@ -726,6 +819,20 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
             const bool sk_wait = stream_k && wi.kb0 == 0 && wi.kb1 < p.k_blocks;
             const bool tail_item = tail_split && wi.tile >= p.dp_tiles;
             const int sk_slot = (worker + 1) * CG + static_cast<int>(rank);
+            ColTerms& terms_smem = terms_all[ACT ? lt & 1 : 0];
+            if constexpr (ACT) {
+                // The terms this tile needs, before its accumulator is awaited: every warp has left the tile before last.
+                fill_col_terms(terms_smem, e, b, tn * tc::BN, threadIdx.x - 64, C::EPI_THREADS);
+                // This warp's part of the residual into L2 while the tile is multiplied, a row per lane.
+                const int rm = tm * C::BM + static_cast<int>(rank) * 128 + q * 32 + lane, rn = tn * tc::BN + c_first * 32;
+                const int cols = min(p.n - rn, 32 * (c_end - c_first));
+                if (e.residual != nullptr && p.residual_vec && rm < p.m && cols > 0)
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                                     static_cast<const uint8_t*>(e.residual) +
+                                     (b * e.batch_stride_c + static_cast<int64_t>(rm) * e.ldc + rn) * ActBox<OUT>::SIZE),
+                                 "r"(cols * ActBox<OUT>::SIZE)
+                                 : "memory");
+            }
             if (threadIdx.x == 64) {
                 bool ok = mbar_wait(&tfull[acc], aph, abort_flag);
                 if (ok && tail_item && !tail_ready) {
@@ -744,7 +851,7 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                 }
                 epi_go[lt & 1] = ok ? 1 : 0;
             }
-            asm volatile("bar.sync 1, %0;" ::"n"(tc::EPI_THREADS) : "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_THREADS) : "memory");
             if (!epi_go[lt & 1]) goto done;
             const bool reduce = tail_item;
             if (reduce && lane == 0) fence_proxy_async_global();  // the reductions follow the cleared tail
@@ -763,7 +870,7 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                     sk_put(slot, c, row_in_cta, r);
                 }
                 __threadfence();
-                asm volatile("bar.sync 1, %0;" ::"n"(tc::EPI_THREADS) : "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_THREADS) : "memory");
                 if (threadIdx.x == 64) {
                     unsigned int* flag = p.sk_flag + worker * CG + static_cast<int>(rank);
                     asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(*sk_gen) : "memory");
@@ -781,9 +888,9 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
             const int32_t* sk_in = sk_wait ? reinterpret_cast<const int32_t*>(sA) : nullptr;
             // The zero-point terms and the bias enter C once: with the K-block-0 piece of a tail tile.
             const bool with_terms = terms && (!reduce || wi.kb0 == 0);
-            if (with_terms) {  // every warp has left the previous tile (the barrier above), so its terms are free
-                fill_col_terms(terms_smem, e, b, tn * tc::BN, threadIdx.x - 64, tc::EPI_THREADS);
-                asm volatile("bar.sync 1, %0;" ::"n"(tc::EPI_THREADS) : "memory");
+            if (!ACT && with_terms) {  // every warp has left the previous tile (the barrier above), so its terms are free
+                fill_col_terms(terms_smem, e, b, tn * tc::BN, threadIdx.x - 64, C::EPI_THREADS);
+                asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_THREADS) : "memory");
             }
             const int m = tm * C::BM + static_cast<int>(rank) * 128 + q * 32 + lane;
             const bool row_ok = m < p.m;
@@ -793,13 +900,82 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                 const uint32_t rsa = e.row_sum_a ? row_sum_of(e, b, m) : 0u;
                 rt = static_cast<uint32_t>(p.k) * za - rsa;
             }
-            float row_scale = 0.0f;  // activated form: the scale of this row of A, and the row's place in the output
-            int64_t row_at = 0;
             if constexpr (ACT) {
-                if (row_ok) row_scale = row_scale_of(e, m);
-                row_at = b * e.batch_stride_c + static_cast<int64_t>(m) * e.ldc;
-            }
-            if (tma_store) {
+                using B = ActBox<OUT>;
+                const int box_row = tm * C::BM + static_cast<int>(rank) * 128 + q * 32;
+                const int64_t batch_at = b * e.batch_stride_c;
+                const bool int_terms = e.za != nullptr || e.zb != nullptr || e.int_bias != nullptr;
+                const bool res = e.residual != nullptr, res_ahead = res && p.residual_vec;
+                const float row_scale = row_ok ? row_scale_of(e, m) : 0.0f;  // the scale of this row of A
+                uint8_t* box = staging + ew * C::BOXES * C::BOX_BYTES;
+                const uint32_t box_s = smem_u32(box);
+                uint4 ahead[4];
+                if (res_ahead) residual_box<OUT>(e, batch_at, box_row, tn * tc::BN + c_first * 32, lane, ahead);
+#pragma unroll 1
+                for (int j0 = c_first * 32; j0 < c_end * 32; j0 += B::COLS) {  // a box at a time
+                    const int n0 = tn * tc::BN + j0;
+                    if (n0 >= p.n || box_row >= p.m) break;
+                    if (lane == 0) bulk_wait_group_read<0>();
+                    __syncwarp();  // the box is free
+                    if (res_ahead) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            st_shared_16(box_unit(box_s, (lane >> 2) + 8 * i, lane & 3), ahead[i]);
+                        if (j0 + B::COLS < c_end * 32) residual_box<OUT>(e, batch_at, box_row, n0 + B::COLS, lane, ahead);
+                    } else if (res) {
+                        residual_elements<OUT>(e, batch_at, box_row, n0, lane, box_s);
+                    }
+                    if (res) __syncwarp();
+                    // 16 columns at a time: two 16-byte units of float16, four of float32.
+#pragma unroll
+                    for (int g = 0; g < B::COLS; g += 16) {
+                        uint32_t r[16];
+                        tmem_ld_32x32b_x16(t_row + j0 + g, r);
+                        tmem_ld_wait();
+                        if (sk_in != nullptr) sk_add_16(sk_in, (j0 + g) / 32, ((j0 + g) / 16) & 1, row_in_cta, r);
+                        float f[16];
+                        activated_values(terms_smem, e, int_terms, za_per_row, za, rt, row_scale, j0 + g, r, f);
+#pragma unroll
+                        for (int u = 0; u < 16 / B::UNIT; u++) {
+                            const uint32_t at = box_unit(box_s, lane, g / B::UNIT + u);
+                            if (res) {
+                                const uint4 x = ld_shared_16(at);
+                                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    if constexpr (OUT == OUT_ACT_F16) {
+                                        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&y[i]));
+                                        f[8 * u + 2 * i] = __fadd_rn(f[8 * u + 2 * i], v.x);
+                                        f[8 * u + 2 * i + 1] = __fadd_rn(f[8 * u + 2 * i + 1], v.y);
+                                    } else {
+                                        f[4 * u + i] = __fadd_rn(f[4 * u + i], __uint_as_float(y[i]));
+                                    }
+                                }
+                            }
+                            uint4 w;
+                            if constexpr (OUT == OUT_ACT_F16)
+                                w = make_uint4(half_pair(f[8 * u], f[8 * u + 1]), half_pair(f[8 * u + 2], f[8 * u + 3]),
+                                               half_pair(f[8 * u + 4], f[8 * u + 5]), half_pair(f[8 * u + 6], f[8 * u + 7]));
+                            else
+                                w = make_uint4(__float_as_uint(f[4 * u]), __float_as_uint(f[4 * u + 1]),
+                                               __float_as_uint(f[4 * u + 2]), __float_as_uint(f[4 * u + 3]));
+                            st_shared_16(at, w);
+                        }
+                    }
+                    if (tma_store) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&tmap_c, box, n0, box_row, b);
+                            bulk_commit_group();
+                        }
+                    } else {
+                        __syncwarp();
+                        store_elements<OUT>(e, batch_at, box_row, n0, lane, box_s);
+                        __syncwarp();
+                    }
+                }
+            } else if (tma_store) {
                 // Each 32 x 32 chunk leaves as two TMA stores of 32 x 16 words (64-byte row segments) through this
                 // warp's boxes in turn (with two boxes, staging one half never waits for the store just issued);
                 // rows past M and columns past N are clipped by the tensor map.
@@ -812,29 +988,6 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                     tmem_ld_32x32b_x32(t_row + c * 32, r);
                     tmem_ld_wait();
                     if (sk_in != nullptr) sk_add(sk_in, c, row_in_cta, r);
-                    if constexpr (OUT == OUT_ACT_F16) {  // 32 float16 results fill one box
-                        uint8_t* box = staging + ew * C::BOXES * C::BOX_BYTES;
-                        uint32_t w[16];
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            float f[16];
-                            finish_activated<OUT>(terms_smem, e, za_per_row, za, rt, row_scale, c * 32 + 16 * h,
-                                                  row_at + n0 + 16 * h, row_ok ? p.n - n0 - 16 * h : 0, p.residual_vec,
-                                                  r + 16 * h, f);
-#pragma unroll
-                            for (int q = 0; q < 8; q++) w[8 * h + q] = half_pair(f[2 * q], f[2 * q + 1]);
-                        }
-                        if (lane == 0) bulk_wait_group_read<0>();
-                        __syncwarp();
-                        stage_words(w, box, lane);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store_3d(&tmap_c, box, n0, box_row, b);
-                            bulk_commit_group();
-                        }
-                        continue;
-                    }
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         if (n0 + 16 * h >= p.n) break;
@@ -842,19 +995,8 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                         uint8_t* box = staging + (ew * C::BOXES + h % C::BOXES) * C::BOX_BYTES;
                         if (lane == 0) bulk_wait_group_read<C::BOXES - 1>();
                         __syncwarp();
-                        if constexpr (OUT == OUT_ACT_F32) {
-                            float f[16];
-                            uint32_t w[16];
-                            finish_activated<OUT>(terms_smem, e, za_per_row, za, rt, row_scale, c * 32 + 16 * h,
-                                                  row_at + n0 + 16 * h, row_ok ? p.n - n0 - 16 * h : 0, p.residual_vec,
-                                                  r + 16 * h, f);
-#pragma unroll
-                            for (int q = 0; q < 16; q++) w[q] = __float_as_uint(f[q]);
-                            stage_words(w, box, lane);
-                        } else {
-                            stage_half<OUT>(terms_smem, e, with_terms, za_per_row, za, rt, c * 32 + 16 * h, r + 16 * h,
-                                            box, lane);
-                        }
+                        stage_half<OUT>(terms_smem, e, with_terms, za_per_row, za, rt, c * 32 + 16 * h, r + 16 * h,
+                                        box, lane);
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
@@ -875,13 +1017,7 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                     tmem_ld_32x32b_x32(t_row + c * 32, r);
                     tmem_ld_wait();
                     if (sk_in != nullptr) sk_add(sk_in, c, row_in_cta, r);
-                    if constexpr (ACT) {
-                        if (row_ok)
-                            store_chunk_activated<OUT>(terms_smem, e, za_per_row, za, rt, row_scale, row_at + n0, c * 32,
-                                                       min(32, p.n - n0), r);
-                    } else {
-                        if (row_ok) store_chunk<OUT>(terms_smem, e, terms, za_per_row, za, rt, b, m, n0, c * 32, r);
-                    }
+                    if (row_ok) store_chunk<OUT>(terms_smem, e, terms, za_per_row, za, rt, b, m, n0, c * 32, r);
                 }
             }
             tc_fence_before();
@@ -921,14 +1057,14 @@ done:
 }
 
 template <bool B_MN, int OUT, bool SPLIT>
-__global__ void __launch_bounds__(tc::THREADS, 1)
+__global__ void __launch_bounds__(tc::Cfg<1, out_activated(OUT)>::THREADS, 1)
     int8_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                         const __grid_constant__ CUtensorMap tmap_c, const TcParams p, uint32_t idesc) {
     gemm_tc_body<1, B_MN, OUT, SPLIT>(tmap_a, tmap_b, tmap_c, p, idesc);
 }
 
 template <bool B_MN, int OUT, bool SPLIT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(tc::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(tc::Cfg<2, out_activated(OUT)>::THREADS, 1)
     int8_gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_c, const TcParams p, uint32_t idesc) {
     gemm_tc_body<2, B_MN, OUT, SPLIT>(tmap_a, tmap_b, tmap_c, p, idesc);
@@ -1022,7 +1158,7 @@ static cudaError_t configure(K kern, int smem, std::atomic<uint64_t>& configured
 template <int CG, bool B_MN, int OUT, bool SPLIT>
 static LaunchFn bind_tc_t(const GemmLaunch& L, const TcParams& p, const CUtensorMap& ma, const CUtensorMap& mb,
                           const CUtensorMap& mc, int grid) {
-    using C = tc::Cfg<CG>;
+    using C = tc::Cfg<CG, out_activated(OUT)>;
     const uint32_t idesc = idesc_i8(L.a_signed, L.b_signed, false, B_MN, C::BM, tc::BN);
     return [=](cudaStream_t stream) -> cudaError_t {
         static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
@@ -1030,12 +1166,12 @@ static LaunchFn bind_tc_t(const GemmLaunch& L, const TcParams& p, const CUtensor
             auto kern = int8_gemm_tc2_kernel<B_MN, OUT, SPLIT>;
             cudaError_t e = configure(kern, C::SMEM_BYTES, configured);
             if (e != cudaSuccess) return e;
-            return launch_pdl(kern, dim3(grid), dim3(tc::THREADS), C::SMEM_BYTES, stream, ma, mb, mc, p, idesc);
+            return launch_pdl(kern, dim3(grid), dim3(C::THREADS), C::SMEM_BYTES, stream, ma, mb, mc, p, idesc);
         } else {
             auto kern = int8_gemm_tc_kernel<B_MN, OUT, SPLIT>;
             cudaError_t e = configure(kern, C::SMEM_BYTES, configured);
             if (e != cudaSuccess) return e;
-            return launch_pdl(kern, dim3(grid), dim3(tc::THREADS), C::SMEM_BYTES, stream, ma, mb, mc, p, idesc);
+            return launch_pdl(kern, dim3(grid), dim3(C::THREADS), C::SMEM_BYTES, stream, ma, mb, mc, p, idesc);
         }
     };
 }

@@ -103,14 +103,14 @@ __device__ __forceinline__ float scaled_sum(uint32_t s, float row_scale, float s
     return biased ? __fadd_rn(f, bias) : f;
 }
 
-// Element idx of the residual, as float32. A plain load: the residual may be the output itself, whose element idx is
-// written by the thread that has read it here.
+// Element idx of the residual, as float32, past L1: the residual may be the output itself, which the launch before may
+// have written.
 template <int OUT>
 __device__ __forceinline__ float residual_at(const Epilogue& e, int64_t idx) {
     if constexpr (OUT == OUT_ACT_F16)
-        return __half2float(static_cast<const __half*>(e.residual)[idx]);
+        return __half2float(__ldcg(static_cast<const __half*>(e.residual) + idx));
     else
-        return static_cast<const float*>(e.residual)[idx];
+        return __ldcg(static_cast<const float*>(e.residual) + idx);
 }
 
 // One result of the activated form at element idx of the output (row m, column n), stored.
