@@ -662,6 +662,16 @@ void record_gemm(og_int8_gemm* g, og_encoder* enc, og::GemmLaunch L, const og_op
         enc->dispatches += 1;
         return;
     }
+    const int slim = g->tile == 0 && g->stream_k != 2 ? og::slim_parts(L) : 0;
+    if (slim > 0) {
+        cudaError_t err;
+        og::LaunchFn fn = og::prepare_gemm_slim(L, slim, &err);  // tensor maps built now, at record time
+        check_cuda(err, "Int8Gemm tensor maps");
+        g->last = staged ? "tensor-core-slim-staged" : "tensor-core-slim";
+        enc->ops.push_back(std::move(fn));
+        enc->dispatches += 1;
+        return;
+    }
     if (g->tile == 0 && og::rows_eligible(L)) {
         const int workers = og::rows_workers(L);
         if (workers > 0) {

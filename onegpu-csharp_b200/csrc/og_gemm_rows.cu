@@ -98,8 +98,6 @@ __device__ __forceinline__ void store_one(const Epilogue& e, int b, int m, int n
         __stcs(static_cast<int32_t*>(e.c) + idx, static_cast<int32_t>(s));
     } else if constexpr (OUT == OUT_F32) {
         __stcs(static_cast<float*>(e.c) + idx, finish_float(e, n, s));
-    } else if constexpr (out_activated(OUT)) {
-        store_activated<OUT>(e, idx, m, n, s);
     } else {
         static_cast<uint8_t*>(e.c)[idx] = finish_byte(e, n, s, OUT == OUT_U8);
     }
@@ -700,7 +698,7 @@ done:
 // ---- host side ---------------------------------------------------------------------------------------------------
 
 bool rows_eligible(const GemmLaunch& L) {
-    return L.m >= 1 && L.m <= rows::MAXM && L.batch <= 65535 && tc_eligible(L);
+    return L.m >= 1 && L.m <= rows::MAXM && L.batch <= 65535 && tc_eligible(L) && !out_activated(L.epi.out_kind);
 }
 
 // Binds the kernel and its arguments; the returned function sets the shared-memory limit (first time per device)
@@ -806,10 +804,6 @@ LaunchFn prepare_gemm_rows(const GemmLaunch& L, cudaError_t* err) {
                                     : bind_rows_stream_t<false, OUT_I32>(p, ma, mb, grid, idesc);
             case OUT_F32: return km ? bind_rows_stream_t<true, OUT_F32>(p, ma, mb, grid, idesc)
                                     : bind_rows_stream_t<false, OUT_F32>(p, ma, mb, grid, idesc);
-            case OUT_ACT_F32: return km ? bind_rows_stream_t<true, OUT_ACT_F32>(p, ma, mb, grid, idesc)
-                                        : bind_rows_stream_t<false, OUT_ACT_F32>(p, ma, mb, grid, idesc);
-            case OUT_ACT_F16: return km ? bind_rows_stream_t<true, OUT_ACT_F16>(p, ma, mb, grid, idesc)
-                                        : bind_rows_stream_t<false, OUT_ACT_F16>(p, ma, mb, grid, idesc);
             case OUT_U8: return km ? bind_rows_stream_t<true, OUT_U8>(p, ma, mb, grid, idesc)
                                    : bind_rows_stream_t<false, OUT_U8>(p, ma, mb, grid, idesc);
             default: return km ? bind_rows_stream_t<true, OUT_S8>(p, ma, mb, grid, idesc)
@@ -822,10 +816,6 @@ LaunchFn prepare_gemm_rows(const GemmLaunch& L, cudaError_t* err) {
                                 : bind_rows_t<false, OUT_I32>(p, ma, mb, grid, idesc);
         case OUT_F32: return km ? bind_rows_t<true, OUT_F32>(p, ma, mb, grid, idesc)
                                 : bind_rows_t<false, OUT_F32>(p, ma, mb, grid, idesc);
-        case OUT_ACT_F32: return km ? bind_rows_t<true, OUT_ACT_F32>(p, ma, mb, grid, idesc)
-                                    : bind_rows_t<false, OUT_ACT_F32>(p, ma, mb, grid, idesc);
-        case OUT_ACT_F16: return km ? bind_rows_t<true, OUT_ACT_F16>(p, ma, mb, grid, idesc)
-                                    : bind_rows_t<false, OUT_ACT_F16>(p, ma, mb, grid, idesc);
         case OUT_U8: return km ? bind_rows_t<true, OUT_U8>(p, ma, mb, grid, idesc)
                                : bind_rows_t<false, OUT_U8>(p, ma, mb, grid, idesc);
         default: return km ? bind_rows_t<true, OUT_S8>(p, ma, mb, grid, idesc)

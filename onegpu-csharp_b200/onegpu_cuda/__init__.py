@@ -293,13 +293,18 @@ class GpuBuffer:
             _check(_lib.og_buffer_alloc(device.handle, max(self.nbytes, 16), ctypes.byref(p)))
             ptr = p.value
         self.ptr = ptr
+        self._ref = None
 
     @property
     def Length(self) -> int:  # noqa: N802 - the reference's property name
         return self.length
 
     def ref(self) -> og_buffer:
-        return og_buffer(self.ptr, self.length, self.type)
+        """The C view of the buffer, built once (building it anew for every argument of every call costs more than the
+        calls themselves) and again when the buffer has another address."""
+        if self._ref is None or self._ref[0] != self.ptr:
+            self._ref = (self.ptr, og_buffer(self.ptr, self.length, self.type))
+        return self._ref[1]
 
     def write(self, data: np.ndarray, offset: int = 0) -> None:
         a = np.ascontiguousarray(np.asarray(data).view(self.dtype).reshape(-1))
@@ -586,9 +591,12 @@ class Int8GemmProblem:
         return 2.0 * self.batch * self.m * self.n * self.k
 
     def c_struct(self) -> og_int8_gemm_problem:
-        return og_int8_gemm_problem(self.m, self.n, self.k, self.batch, int(bool(self.transpose_b)), self.lda,
-                                    self.ldb, self.offset_a, self.offset_b, self.offset_c, self.stride_a,
-                                    self.stride_b)
+        key = (self.m, self.n, self.k, self.batch, 1 if self.transpose_b else 0, self.lda, self.ldb, self.offset_a,
+               self.offset_b, self.offset_c, self.stride_a, self.stride_b)
+        known = self.__dict__.get("_known")
+        if known is None or known[0] != key:  # built once for the same values
+            known = self.__dict__["_known"] = (key, og_int8_gemm_problem(*key))
+        return known[1]
 
 
 @dataclass
@@ -599,8 +607,13 @@ class Int8Operand:
     is_vector: bool = False
 
     def c_struct(self) -> og_operand:
-        ref = self.buffer.ref() if self.buffer is not None else og_buffer(None, 0, 0)
-        return og_operand(ref, self.offset, int(bool(self.is_vector)))
+        buffer = self.buffer
+        key = (buffer, buffer.ptr if buffer is not None else None, self.offset, 1 if self.is_vector else 0)
+        known = self.__dict__.get("_known")
+        if known is None or known[0] != key:  # built once for the same values
+            ref = buffer.ref() if buffer is not None else og_buffer(None, 0, 0)
+            known = self.__dict__["_known"] = (key, og_operand(ref, key[2], key[3]))
+        return known[1]
 
 
 @dataclass
@@ -1067,7 +1080,14 @@ class MoeProblem:
     offset_weights: int = 0
 
     def c_struct(self) -> og_moe_problem:
-        return og_moe_problem(*[int(getattr(self, name)) for name, _ in og_moe_problem._fields_])
+        key = (self.tokens, self.model_size, self.expert_size, self.experts, self.top_k, self.activation,
+               1 if self.gated else 0, 1 if self.normalize else 0, self.offset_x, self.offset_router, self.offset_in,
+               self.offset_in_scale, self.offset_out, self.offset_out_scale, self.offset_y, self.offset_residual,
+               self.offset_ids, self.offset_weights)
+        known = self.__dict__.get("_known")
+        if known is None or known[0] != key:  # built once for the same values
+            known = self.__dict__["_known"] = (key, og_moe_problem(*key))
+        return known[1]
 
 
 def check_moe(problem: MoeProblem, x, router, w_in, w_in_scale, w_out, w_out_scale, y, residual=None, expert_ids=None,
