@@ -230,7 +230,8 @@ OG_API og_status og_int8_gemm_destroy(og_int8_gemm* gemm);
 /* Int8Gemm.Variant (Int8Gemm.cs:215). */
 OG_API og_status og_int8_gemm_variant(og_int8_gemm* gemm, char* buffer, uint64_t capacity);
 /* The kernel the last encode call recorded: "tensor-core-2sm" or "tensor-core-1sm" (with "-stream-k" when the
- * product's (tile, K block) work was split evenly across the SMs), "tensor-core-rows", "portable" or "none". */
+ * product's (tile, K block) work was split evenly across the SMs), "tensor-core-rows", "tensor-core-slim" (an
+ * activated product of few rows), "portable" or "none". */
 OG_API og_status og_int8_gemm_last_kernel(og_int8_gemm* gemm, char* buffer, uint64_t capacity);
 /* Int8Gemm.ScratchElements (Int8Gemm.cs:531). */
 OG_API int64_t og_int8_gemm_scratch_elements(const og_int8_gemm_problem* problem);
@@ -424,9 +425,9 @@ OG_API og_status og_dequantize_check_quantize(const og_buffer* x, int32_t offset
  *   h[j] = activation(u[j]) * u[expert_size + j] when `gated` is set (w_in holds the activated half's expert_size rows,
  *          then the other half's), activation(u[j]) otherwise
  *   y[t][d] = residual[t][d] + sum over the chosen experts of w w_out_scale[e][d] sum_j w_out[e][d][j] h[j]
- * The sums are exact or held in float32 and more. The fused kernel (og_int8_moe_last_kernel) multiplies x and the hidden
- * values in fixed point with a scale per token, 23 bits below the row's largest value for float16 and 31 for float32; a
- * token with an infinite or NaN value, or such a hidden value, gets NaN there. */
+ * The sums are exact or held in float32 and more: x and the hidden values are multiplied in fixed point with a scale per
+ * token, 23 bits below the row's largest value for float16 and 31 for float32; a token with an infinite or NaN value, or
+ * such a hidden value, gets NaN. */
 
 /* tokens 0 .. 128; model_size and expert_size 1 .. 65536; experts 1 .. 512; top_k 1 .. min(experts, 16); activation an
  * og_activation; gated and normalize 0 or 1; offsets in elements. */
@@ -442,8 +443,8 @@ typedef struct og_int8_moe og_int8_moe;
 OG_API og_status og_int8_moe_create(og_device* device, og_int8_moe** out);
 /* Waits for the device, releases the instance's workspace. */
 OG_API og_status og_int8_moe_destroy(og_int8_moe* moe);
-/* The kernel the last encode call recorded: "fused" (one cooperative kernel, for weights whose rows start on 16-byte
- * boundaries), "portable" or "none". */
+/* The kernel the last encode call recorded: "fused" (one cooperative kernel), "fused-unaligned" (the same with another
+ * load path, for weights whose rows do not all start on 16-byte boundaries) or "none". */
 OG_API og_status og_int8_moe_last_kernel(og_int8_moe* moe, char* buffer, uint64_t capacity);
 /* x, y and residual are float32 or float16 (one type), [tokens][model_size]; router float32 or float16,
  * [experts][model_size]; w_in int8 [experts][(gated ? 2 : 1) * expert_size][model_size] and w_out int8

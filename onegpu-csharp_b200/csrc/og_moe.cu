@@ -6,178 +6,15 @@
 //   y[t][d] = residual[t][d] + sum over the chosen e of w_e scale_out[e][d] sum_j w_out[e][d][j] h[j]
 //
 // Everything is accumulated in float32; the activations are not quantized. A NaN logit ranks below every number.
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 #include <string>
 #include <vector>
 
-#include "og_act.cuh"
 #include "og_gemm.h"
 #include "og_host.h"
 #include "og_moe.h"
-#include "og_ptx.cuh"
-
-namespace og {
-
-__device__ __forceinline__ float moe_value(const void* p, int half, int64_t i) {
-    return half ? __half2float(__ldg(static_cast<const __half*>(p) + i)) : __ldg(static_cast<const float*>(p) + i);
-}
-
-__device__ __forceinline__ float moe_warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
-}
-
-// The top_k experts of one token by a warp: logits in shared memory (NaN already replaced by -infinity for the
-// ranking; `sum` is the softmax's denominator over the true logits, `top` its maximum). Each round takes the largest
-// remaining logit, the lowest index among equals.
-__device__ __forceinline__ void moe_top_k(float* rank, const MoeLaunch& L, int t, float top, float sum) {
-    const int lane = threadIdx.x & 31;
-    float chosen_sum = 0.0f;
-    float weight = 0.0f;  // lane k: the k-th chosen weight
-    int id = 0;
-    for (int k = 0; k < L.top_k; k++) {
-        float best = -INFINITY;
-        int at = MOE_MAX_EXPERTS;
-        for (int e = lane; e < L.experts; e += 32)
-            if (rank[e] > best || (at == MOE_MAX_EXPERTS && rank[e] == best)) {
-                // strictly larger, or the first candidate of this lane (a taken expert is NaN and never compares)
-                best = rank[e];
-                at = e;
-            }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float b2 = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-            const int a2 = __shfl_xor_sync(0xFFFFFFFFu, at, o);
-            if (b2 > best || (b2 == best && a2 < at)) {
-                best = b2;
-                at = a2;
-            }
-        }
-        const float w = expf(best - top) / sum;
-        chosen_sum += w;
-        if (lane == k) {
-            weight = w;
-            id = at;
-        }
-        if (lane == 0) rank[at] = NAN;
-        __syncwarp();
-    }
-    if (lane < L.top_k) {
-        if (L.normalize) weight = weight / chosen_sum;
-        const int i = t * L.top_k + lane;
-        L.ids[i] = id;
-        L.weights[i] = weight;
-        if (L.ids_out != nullptr) L.ids_out[i] = id;
-        if (L.weights_out != nullptr) L.weights_out[i] = weight;
-    }
-}
-
-// Portable kernels: any sizes and alignment.
-
-// One block per token: its logits (a warp per expert), then the softmax and the top k.
-__global__ void __launch_bounds__(256) moe_router_kernel(const MoeLaunch L) {
-    __shared__ float logits[MOE_MAX_EXPERTS];
-    __shared__ float rank[MOE_MAX_EXPERTS];
-    pdl_trigger();
-    pdl_wait();
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int e = warp; e < L.experts; e += 8) {
-        double sum = 0.0;
-        for (int d = lane; d < L.model; d += 32)
-            sum += static_cast<double>(moe_value(L.x, L.x_half, static_cast<int64_t>(t) * L.model + d)) *
-                   moe_value(L.router, L.router_half, static_cast<int64_t>(e) * L.model + d);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (lane == 0) {
-            logits[e] = static_cast<float>(sum);
-            rank[e] = isnan(logits[e]) ? -INFINITY : logits[e];
-        }
-    }
-    __syncthreads();
-    if (warp != 0) return;
-    float top = -INFINITY;
-    bool nan = false;
-    for (int e = lane; e < L.experts; e += 32) {
-        nan |= isnan(logits[e]);
-        top = fmaxf(top, logits[e]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if (__any_sync(0xFFFFFFFFu, nan)) top = NAN;  // the softmax of a row with a NaN is NaN
-    float sum = 0.0f;
-    for (int e = lane; e < L.experts; e += 32) sum += expf(logits[e] - top);
-    moe_top_k(rank, L, t, top, moe_warp_sum(sum));
-}
-
-// One warp per (token, choice, hidden unit).
-__global__ void __launch_bounds__(256) moe_up_kernel(const MoeLaunch L) {
-    pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (unit >= static_cast<int64_t>(L.tokens) * L.top_k * L.expert) return;
-    const int pair = static_cast<int>(unit / L.expert), j = static_cast<int>(unit % L.expert);
-    const int t = pair / L.top_k, e = __ldcg(L.ids + pair);
-    const int64_t rows = static_cast<int64_t>(L.gated ? 2 : 1) * L.expert;
-    float u[2] = {0.0f, 0.0f};
-    for (int g = 0; g < (L.gated ? 2 : 1); g++) {
-        const int64_t row = e * rows + static_cast<int64_t>(g) * L.expert + j;
-        const int8_t* w = L.w_in + row * L.model;
-        float sum = 0.0f;
-        for (int d = lane; d < L.model; d += 32)
-            sum = fmaf(static_cast<float>(__ldg(w + d)), moe_value(L.x, L.x_half, static_cast<int64_t>(t) * L.model + d),
-                       sum);
-        u[g] = moe_warp_sum(sum) * __ldg(L.in_scale + row);
-    }
-    if (lane != 0) return;
-    float h[1] = {u[0]};
-    activate_all(h, L.activation);
-    L.hidden[unit] = L.gated ? h[0] * u[1] : h[0];
-}
-
-// One warp per (token, output).
-__global__ void __launch_bounds__(256) moe_down_kernel(const MoeLaunch L) {
-    pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (unit >= static_cast<int64_t>(L.tokens) * L.model) return;
-    const int t = static_cast<int>(unit / L.model), d = static_cast<int>(unit % L.model);
-    float out = 0.0f;
-    for (int k = 0; k < L.top_k; k++) {
-        const int pair = t * L.top_k + k;
-        const int64_t row = static_cast<int64_t>(__ldcg(L.ids + pair)) * L.model + d;
-        const int8_t* w = L.w_out + row * L.expert;
-        const float* h = L.hidden + static_cast<int64_t>(pair) * L.expert;
-        float sum = 0.0f;
-        for (int j = lane; j < L.expert; j += 32) sum = fmaf(static_cast<float>(__ldg(w + j)), __ldcg(h + j), sum);
-        out = fmaf(__ldcg(L.weights + pair), moe_warp_sum(sum) * __ldg(L.out_scale + row), out);
-    }
-    if (lane != 0) return;
-    if (L.x_half) {
-        if (L.residual != nullptr) out += __half2float(static_cast<const __half*>(L.residual)[unit]);
-        static_cast<__half*>(L.y)[unit] = __float2half_rn(out);
-    } else {
-        if (L.residual != nullptr) out += static_cast<const float*>(L.residual)[unit];
-        static_cast<float*>(L.y)[unit] = out;
-    }
-}
-
-cudaError_t launch_moe_portable(const MoeLaunch& L, cudaStream_t s) {
-    cudaError_t e = launch_pdl(moe_router_kernel, dim3(L.tokens), dim3(256), 0, s, L);
-    if (e != cudaSuccess) return e;
-    const int64_t up = static_cast<int64_t>(L.tokens) * L.top_k * L.expert, down = static_cast<int64_t>(L.tokens) * L.model;
-    e = launch_pdl(moe_up_kernel, dim3(static_cast<unsigned>((up + 7) / 8)), dim3(256), 0, s, L);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(moe_down_kernel, dim3(static_cast<unsigned>((down + 7) / 8)), dim3(256), 0, s, L);
-}
-
-}  // namespace og
 
 // ---- host layer ------------------------------------------------------------------------------------------------------
 
@@ -280,18 +117,17 @@ bool check_moe(const og_moe_problem* p, const og_buffer* x, const og_buffer* rou
 
 int64_t round256(int64_t v) { return (v + 255) & ~int64_t(255); }
 
-// Carves the layer's workspace out of the instance's, growing it geometrically. The portable kernels' part is always
-// there (the fused launch falls back to them).
-void bind_workspace(og_int8_moe* m, og::MoeLaunch& L, bool fused) {
+// Carves the layer's workspace out of the instance's, growing it geometrically.
+void bind_workspace(og_int8_moe* m, og::MoeLaunch& L) {
     const int64_t pairs = static_cast<int64_t>(L.tokens) * L.top_k;
-    const og::MoeFusedSizes s = fused ? og::moe_fused_sizes(L) : og::MoeFusedSizes{};
+    const og::MoeFusedSizes s = og::moe_fused_sizes(L);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
         at += round256(bytes);
         return here;
     };
-    const int64_t ids = take(pairs * 4), weights = take(pairs * 4), hidden = take(pairs * L.expert * 4);
+    const int64_t ids = take(pairs * 4), weights = take(pairs * 4), hidden = take(s.hidden);
     const int64_t logits = take(s.logits), x = take(s.x_digits), h = take(s.h_digits), outputs = take(s.outputs);
     const int64_t x_most = take(s.x_most), h_most = take(s.h_most), segments = take(s.segments);
     if (m->bytes < at) {
@@ -402,20 +238,13 @@ OG_API og_status og_int8_moe_encode(og_int8_moe* m, og_encoder* enc, const og_mo
         L.tickets = reinterpret_cast<unsigned int*>(m->arrivals + 1);
         L.error_flag = m->device->status;
         L.num_sms = m->device->sm_count;
-        const bool fused = og::moe_fused_eligible(L);
-        bind_workspace(m, L, fused);
-        if (fused) {
-            cudaError_t err;
-            auto fn = og::prepare_moe_fused(L, &err);  // tensor maps built now, at record time
-            check_cuda(err, "Int8Moe tensor maps");
-            m->last = "fused";
-            enc->ops.push_back(std::move(fn));
-            enc->dispatches += 1;
-            return;
-        }
-        m->last = "portable";
-        enc->ops.push_back([L](cudaStream_t s) { return og::launch_moe_portable(L, s); });
-        enc->dispatches += 3;
+        bind_workspace(m, L);
+        cudaError_t err;
+        auto fn = og::prepare_moe_fused(L, &err);  // tensor maps built now, at record time
+        check_cuda(err, "Int8Moe tensor maps");
+        m->last = og::moe_aligned(L) ? "fused" : "fused-unaligned";
+        enc->ops.push_back(std::move(fn));
+        enc->dispatches += 1;
     });
 }
 

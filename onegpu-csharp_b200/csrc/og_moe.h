@@ -31,16 +31,15 @@ struct MoeLaunch {
     int32_t* ids_out;      // [tokens][top_k], or null
     float* weights_out;    // [tokens][top_k], or null
     // Workspace of the instance.
-    int32_t* ids;    // [tokens][top_k]
-    float* weights;  // [tokens][top_k]
-    float* hidden;   // [tokens * top_k][expert]
-    // Fused kernel (og_moe_fused.cu).
+    int32_t* ids;                  // [tokens][top_k]
+    float* weights;                // [tokens][top_k]
+    float* hidden;                 // [tokens * top_k][expert], rows padded to 4
     float* logits;                 // [tokens][experts]
     uint8_t* x_digits;             // [tokens][chunks of model][digits][128] of x
     uint8_t* h_digits;             // [tokens * top_k][chunks of expert][digits][128] of the hidden values
     uint32_t* x_most;              // [tokens] the bits of a token's largest magnitude
     uint32_t* h_most;              // [tokens * top_k] and of a pair's hidden values
-    float* outputs;                // [tokens * top_k][model] weighted outputs of the chosen experts
+    float* outputs;                // [tokens * top_k][model], rows padded to 4: weighted outputs of the chosen experts
     long long* segments;           // partial sums of units cut between warps
     unsigned long long* arrivals;  // grid barrier: arrivals of all launches so far
     unsigned int* tickets;         // [MOE_MAX_TOKENS / 8] logits finished of each block of 8 tokens, 0 between launches
@@ -48,15 +47,14 @@ struct MoeLaunch {
     int num_sms;
 };
 
-// Whether the fused kernel can run the layer: weight rows on 16-byte boundaries (what TMA loads).
-bool moe_fused_eligible(const MoeLaunch& L);
 // The workspace sizes of the fused kernel, in bytes.
 struct MoeFusedSizes {
-    int64_t logits, x_digits, h_digits, x_most, h_most, outputs, segments;
+    int64_t logits, hidden, x_digits, h_digits, x_most, h_most, outputs, segments;
 };
 MoeFusedSizes moe_fused_sizes(const MoeLaunch& L);
-// Builds the tensor maps; the returned launch runs the portable kernels when the device refuses the cooperative launch.
+// Whether weight rows start on 16-byte boundaries, as TMA loads them.
+bool moe_aligned(const MoeLaunch& L);
+// Builds the tensor maps.
 std::function<cudaError_t(cudaStream_t)> prepare_moe_fused(const MoeLaunch& L, cudaError_t* err);
-cudaError_t launch_moe_portable(const MoeLaunch& L, cudaStream_t s);
 
 }  // namespace og

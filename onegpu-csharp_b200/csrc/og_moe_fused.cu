@@ -1,4 +1,4 @@
-// The mixture-of-experts layer as one cooperative kernel (a CTA of 16 warps per SM), for weights TMA can load.
+// The mixture-of-experts layer as one cooperative kernel, a CTA per SM.
 //
 // For a few tokens the layer is bound by reading the touched experts' weights once (3 x model x expert bytes each when
 // gated), so everything is arranged around keeping those reads in flight:
@@ -22,11 +22,11 @@
 // into D balanced base-256 digits that are int8 operands too: every digit's sum is an exact int32 (65536 x 128 x 128 stays
 // below 2^31) and the digits' sums together an exact int64, whatever the order. Held are 23 bits below the row's largest
 // value for float16 layers (D = 3) and 31 bits for float32 ones (D = 4), float32's own precision for values down to 2^-7
-// of the largest. Measured against converting
-// the weights to bfloat16 in registers and multiplying two or three bfloat16 pieces: 239 instructions per 2 KB of
-// weights became about 100, 8 tokens through 2 of 8 experts (4096 x 8192) went from 163 to 149 us (4.9 TB/s over the whole
-// launch, 6 TB/s while the weights stream), 64 tokens through 6 of 64 experts (2048 x 1408) from 199 to 164 us. The tensor cores' rate does not matter here (one token per expert uses an eighth of
-// a tile), and 128-row tcgen05 tiles would cut the work too coarsely for one token.
+// of the largest. Measured against converting the weights to bfloat16 in registers and multiplying two or three bfloat16
+// pieces: 239 instructions per 2 KB of weights became about 100, 8 tokens through 2 of 8 experts (4096 x 8192) went from
+// 163 to 149 us (4.9 TB/s over the whole launch, 6 TB/s while the weights stream), 64 tokens through 6 of 64 experts
+// (2048 x 1408) from 199 to 164 us. The tensor cores' rate does not matter here (one token per expert uses an eighth of a
+// tile), and 128-row tcgen05 tiles would cut the work too coarsely for one token.
 // A token with an infinite or NaN value, or such a hidden value, gets NaN.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -52,13 +52,18 @@ constexpr int MAX_PAIRS = MOE_MAX_TOKENS * MOE_MAX_TOP_K;
 // registers), the finest units, for one or two tokens, whose columns are all the same few rows. MT = 2: 8 warps, each
 // column digit read from L1 for 32 weight rows instead of 16: with 8 different rows a load touches 8 lines, and from
 // some 4 columns on these loads, not DRAM, set the time.
-template <int NT_, int MT_>
+//
+// ALIGNED: weight rows on 16-byte boundaries, loaded by TMA. Others arrive by 16-byte asynchronous copies of the aligned
+// units that hold a row's 128 bytes (nine of them), and the operands are put together from neighbouring words.
+template <int NT_, int MT_, bool ALIGNED_>
 struct Shape {
     static constexpr int NT = NT_, MT = MT_;
+    static constexpr bool ALIGNED = ALIGNED_;
+    static constexpr int PITCH = ALIGNED ? CHUNK : CHUNK + 16;  // bytes of a row in shared memory
     static constexpr int WARPS = MT == 1 ? 16 : 8;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr int ROWS = 16 * MT;
-    static constexpr int BOX = ROWS * CHUNK;              // 2 or 4 KB; 128 KB of boxes in flight per SM
+    static constexpr int BOX = ROWS * PITCH;              // 2 or 4 KB (and an eighth); 128 KB of boxes in flight per SM
     static constexpr int SUMS = ROWS * 8 * NT;            // of a unit
     static constexpr int WHOLE_FROM = WARPS * 3 / 4;      // warps with a whole unit each: 96 KB in flight are enough
     static constexpr int RING = WARPS * SLOTS * BOX;
@@ -71,6 +76,9 @@ struct MoeFusedParams {
     int blocks_in, blocks_out;  // units per group
     int router_split;           // warps that share one (expert, 8 tokens) of the router
     int vec;                    // rows of x and of the router allow loads of four elements
+    int hidden_pitch, out_pitch;  // elements between the rows of L.hidden and L.outputs, multiples of 4
+    const int8_t* end_in;       // past the last weight
+    const int8_t* end_out;
 };
 
 // A group: one expert and a run of the pairs sorted by expert.
@@ -99,6 +107,7 @@ struct MoeShared {
 
 template <class S>
 constexpr size_t moe_smem_bytes() {
+    static_assert(1024 + size_t(S::RING) + sizeof(MoeShared<S>) <= 232448, "shared memory of a CTA");
     return 1024 + size_t(S::RING) + sizeof(MoeShared<S>);
 }
 
@@ -169,6 +178,14 @@ __device__ __forceinline__ void moe_mma(int (&c)[4], const uint32_t (&a)[4], uin
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Four bytes from byte `shift` / 8 of the word at addr on.
+__device__ __forceinline__ uint32_t unaligned_word(uint32_t addr, uint32_t shift) {
+    uint32_t lo, hi;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(lo) : "r"(addr) : "memory");
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(hi) : "r"(addr + 4) : "memory");
+    return __funnelshift_r(lo, hi, shift);
+}
+
 // The 16 x 32 byte operand of one step: lane l gives the address of one of the four 8 x 16 byte parts' rows (rows 0-7 and
 // 8-15 of the first 16 bytes, then of the second), every lane gets its four words in the order the instruction takes them.
 __device__ __forceinline__ void load_rows(uint32_t (&a)[4], uint32_t addr) {
@@ -232,11 +249,14 @@ __device__ __forceinline__ float moe_load(const void* p, int half, int64_t i) {
     return half ? __half2float(__ldg(static_cast<const __half*>(p) + i)) : __ldg(static_cast<const float*>(p) + i);
 }
 
-// Four consecutive elements; VEC when they may be loaded as one.
+// Elements d .. d + 3 of a row of `size` that starts at element `row`, zeros past its end; VEC when they may be loaded as
+// one (then size is a multiple of 4).
 template <bool HALF, bool VEC>
-__device__ __forceinline__ float4 moe_load4(const void* p, int64_t i) {
+__device__ __forceinline__ float4 moe_load4(const void* p, int64_t row, int d, int size) {
+    const int64_t i = row + d;
     if constexpr (!VEC)
-        return make_float4(moe_load(p, HALF, i), moe_load(p, HALF, i + 1), moe_load(p, HALF, i + 2), moe_load(p, HALF, i + 3));
+        return make_float4(d < size ? moe_load(p, HALF, i) : 0.0f, d + 1 < size ? moe_load(p, HALF, i + 1) : 0.0f,
+                           d + 2 < size ? moe_load(p, HALF, i + 2) : 0.0f, d + 3 < size ? moe_load(p, HALF, i + 3) : 0.0f);
     if constexpr (!HALF) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
     const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(p) + i));
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
@@ -261,14 +281,14 @@ __device__ __forceinline__ void moe_digits_x(const MoeFusedParams& p) {
          u += gridDim.x * S::WARPS) {
         const int t = u / parts, part = u - t * parts;
         const int64_t x0 = static_cast<int64_t>(t) * L.model;
-        const int vectors = L.model / 4;  // model is a multiple of 16
+        const int vectors = (L.model + 3) / 4;
         uint32_t most = 0;
 #pragma unroll 1
         for (int v0 = lane; v0 < vectors; v0 += 256) {
             float4 x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++)  // all in flight; past the end, the last vector again
-                x[i] = moe_load4<HALF, VEC>(L.x, x0 + 4 * min(v0 + 32 * i, vectors - 1));
+                x[i] = moe_load4<HALF, VEC>(L.x, x0, 4 * min(v0 + 32 * i, vectors - 1), L.model);
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 most = max(max(most, max(__float_as_uint(x[i].x) & 0x7FFFFFFFu, __float_as_uint(x[i].y) & 0x7FFFFFFFu)),
@@ -280,7 +300,7 @@ __device__ __forceinline__ void moe_digits_x(const MoeFusedParams& p) {
 #pragma unroll 1
         for (int c = part * 4; c < min(part * 4 + 4, p.chunks_in); c++) {
             const int k = c * moe::CHUNK + lane * 4;
-            const float4 x = k < L.model ? moe_load4<HALF, VEC>(L.x, x0 + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4 x = k < L.model ? moe_load4<HALF, VEC>(L.x, x0, k, L.model) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             put_digits<D>(x, shift, L.x_digits + (static_cast<int64_t>(t) * p.chunks_in + c) * D * moe::CHUNK +
                                         digit_place(lane * 4));
         }
@@ -300,8 +320,10 @@ __device__ __forceinline__ void moe_digits_h(const MoeFusedParams& p) {
         const int pair = u / p.chunks_out, k = (u - pair * p.chunks_out) * moe::CHUNK + lane * 4;
         const uint32_t most = __ldcg(L.h_most + pair);
         float4 h = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (k < L.expert)  // expert is a multiple of 16
-            h = __ldcg(reinterpret_cast<const float4*>(L.hidden + static_cast<int64_t>(pair) * L.expert + k));
+        if (k < L.expert) h = __ldcg(reinterpret_cast<const float4*>(L.hidden + static_cast<int64_t>(pair) * p.hidden_pitch + k));
+        if (k + 1 >= L.expert) h.y = 0.0f;  // the pitch's last elements are not written
+        if (k + 2 >= L.expert) h.z = 0.0f;
+        if (k + 3 >= L.expert) h.w = 0.0f;
         put_digits<D>(h, finite_bits(most) ? row_shift<D>(most) : 0,
                       L.h_digits + static_cast<int64_t>(u) * D * moe::CHUNK + digit_place(lane * 4));
     }
@@ -316,7 +338,7 @@ __device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = p.router_split, per_cta = S::WARPS / split, part = warp % split;
     const int token_blocks = (L.tokens + 7) / 8, units = L.experts * token_blocks;
-    const int vectors = L.model / 4;  // of four elements (model is a multiple of 16); this warp's share of them
+    const int vectors = (L.model + 3) / 4;  // of four elements; this warp's share of them
     const int v0 = moe_split(vectors, part, split), v1 = moe_split(vectors, part + 1, split);
     int buffer = 0;
     for (int first = blockIdx.x * per_cta; first < units; first += gridDim.x * per_cta, buffer ^= 1) {
@@ -337,10 +359,10 @@ __device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int d = 4 * min(v + 32 * u, v1 - 1);
-                    r[u] = moe_load4<ROUTER_HALF, VEC>(L.router, r0 + d);
+                    r[u] = moe_load4<ROUTER_HALF, VEC>(L.router, r0, d, L.model);
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        x[u][i] = moe_load4<HALF, VEC>(L.x, x0 + static_cast<int64_t>(min(i, n - 1)) * L.model + d);
+                        x[u][i] = moe_load4<HALF, VEC>(L.x, x0 + static_cast<int64_t>(min(i, n - 1)) * L.model, d, L.model);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -681,13 +703,51 @@ struct MoeWarp {
         }
     }
 
+    // Row r of a box, as a row of the weights' matrix of its phase: rows past the expert's size are its last one again (their
+    // sums are not stored).
+    __device__ __forceinline__ int64_t weight_row(int phase, int e, int y, int r) const {
+        const bool halves = phase == 0 && p.L.gated;
+        const int size = phase == 0 ? p.L.expert : p.L.model;
+        const int half = halves && r >= 8 * MT ? 1 : 0;
+        return (static_cast<int64_t>(e) + half) * size + min(y + r - half * 8 * MT, size - 1);
+    }
+
+    // The aligned 16-byte units around the feed's 128 bytes of each row, nine a row, copied asynchronously; zeros for those
+    // that start past the weights.
+    __device__ __forceinline__ void copy_rows(uint8_t* box) const {
+        const int8_t* w = feed.phase == 0 ? p.L.w_in : p.L.w_out;
+        const int8_t* end = feed.phase == 0 ? p.end_in : p.end_out;
+        const int ld = feed.phase == 0 ? p.L.model : p.L.expert;
+        constexpr int UNITS = S::ROWS * 9;
+#pragma unroll 3
+        for (int u0 = 0; u0 < UNITS; u0 += 32) {
+            const int u = u0 + lane;
+            if (u >= UNITS) break;
+            const int r = u / 9, j = u - 9 * r;
+            const uintptr_t at = reinterpret_cast<uintptr_t>(w + weight_row(feed.phase, feed.e, feed.y, r) * ld + feed.x);
+            const int8_t* src = reinterpret_cast<const int8_t*>((at & ~uintptr_t(15)) + 16 * j);
+            const bool ok = src < end;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(box + r * S::PITCH + 16 * j)),
+                         "l"(ok ? src : w), "r"(ok ? 16 : 0)
+                         : "memory");
+        }
+    }
+
     // Issues the next box if any is left; the caller has freed a slot.
     __device__ __forceinline__ void issue() {
-        if (feed.left == 0 && !next_run()) return;
-        if (lane == 0) {
-            const int slot = feed.issued % moe::SLOTS;
-            mbar_arrive_expect_tx(&full[slot], S::BOX);
-            tma_load_3d(ring + slot * S::BOX, feed.phase == 0 ? map_in : map_out, &full[slot], feed.x, feed.y, feed.e);
+        if (feed.left == 0 && !next_run()) {
+            if constexpr (!S::ALIGNED) cp_async_commit();  // an empty group keeps their count
+            return;
+        }
+        const int slot = feed.issued % moe::SLOTS;
+        if constexpr (S::ALIGNED) {
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&full[slot], S::BOX);
+                tma_load_3d(ring + slot * S::BOX, feed.phase == 0 ? map_in : map_out, &full[slot], feed.x, feed.y, feed.e);
+            }
+        } else {
+            copy_rows(ring + slot * S::BOX);
+            cp_async_commit();
         }
         feed.issued++;
         feed.left--;
@@ -710,7 +770,7 @@ struct MoeWarp {
     // t in acc[i][t][digit]. The columns' digits start at values + row[t] (column g of the tile). `halves`: the box holds
     // the gate's rows, then the other half's, and a tile 8 of each.
     __device__ __forceinline__ bool products(const uint8_t* values, const uint32_t (&row)[NT], int tiles, bool halves,
-                                             int c0, int c1, int (&acc)[MT][NT][D][4]) {
+                                             const uint32_t (&skew)[MT][2], int c0, int c1, int (&acc)[MT][NT][D][4]) {
         // Where registers allow, the next chunk's digits are on their way while one is multiplied (64 tokens through 6 of
         // 64 experts 172 -> 165 us); elsewhere tile 0's are asked for before the wait for the box and the other tiles' when
         // their turn comes (with NT = 4 or at 16 warps the earlier loads only spill).
@@ -720,7 +780,7 @@ struct MoeWarp {
         // This lane's row of the parts of a step: part lane / 8 is rows 0-7 or 8-15 (odd) of the first or second (2, 3)
         // 16 bytes. A box's 16-byte units are swizzled by the row (its low three bits are lane % 8 in every part), so eight
         // lanes of a part touch eight different units of 128 bytes: no bank conflict.
-        const int tile_step = (halves ? 8 : 16) * moe::CHUNK, half_step = (halves ? 8 * MT : 8) * moe::CHUNK;
+        const int tile_step = (halves ? 8 : 16) * S::PITCH, half_step = (halves ? 8 * MT : 8) * S::PITCH;
         const uint32_t my_row = smem_u32(ring) + (lane & 7) * moe::CHUNK + ((lane >> 3) & 1) * half_step;
         const uint32_t my_unit = lane >> 4, my_swizzle = lane & 7;
 #pragma unroll
@@ -757,14 +817,34 @@ struct MoeWarp {
             } else {
                 load_digits(b[0], v + row[0]);
             }
-            const bool ok = mbar_wait(&full[slot], (taken / moe::SLOTS) & 1, &sh.abort);
-            if (!__all_sync(0xFFFFFFFFu, ok)) return false;
             uint32_t a[MT][4][4];
+            if constexpr (S::ALIGNED) {
+                const bool ok = mbar_wait(&full[slot], (taken / moe::SLOTS) & 1, &sh.abort);
+                if (!__all_sync(0xFFFFFFFFu, ok)) return false;
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+                for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    load_rows(a[m][i], my_row + slot * S::BOX + m * tile_step + (((2 * i + my_unit) ^ my_swizzle) << 4));
+                    for (int i = 0; i < 4; i++)
+                        load_rows(a[m][i], my_row + slot * S::BOX + m * tile_step + (((2 * i + my_unit) ^ my_swizzle) << 4));
+            } else {
+                cp_async_wait_group<moe::SLOTS - 1>();  // the oldest of the copies
+                __syncwarp();
+                // Bytes 32 i + 4 q (+ 16) of rows g and g + 8, which start `skew` bytes into their units: the rows lie
+                // 36 words apart, so equal skews meet no bank conflict.
+                const uint32_t box = smem_u32(ring) + slot * S::BOX + (lane >> 2) * S::PITCH + q * 4;
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t at = box + m * tile_step + h * half_step + (skew[m][h] & ~3u);
+                        const uint32_t shift = (skew[m][h] & 3u) * 8;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            a[m][i][h] = unaligned_word(at + 32 * i, shift);
+                            a[m][i][2 + h] = unaligned_word(at + 32 * i + 16, shift);
+                        }
+                    }
+            }
             taken++;
 #pragma unroll
             for (int t = 0; t < NT; t++) {
@@ -830,7 +910,7 @@ struct MoeWarp {
                 const int n = 8 * t + 2 * q + i;
                 const int pair = sh.order[grp.first + min(n, grp.count - 1)];
                 const int shift = sh.shift[pair];
-                float* hidden = L.hidden + static_cast<int64_t>(pair) * L.expert;
+                float* hidden = L.hidden + static_cast<int64_t>(pair) * p.hidden_pitch;
                 uint32_t most = 0;
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
@@ -874,7 +954,7 @@ struct MoeWarp {
                 const int pair = sh.order[grp.first + n];
                 const int shift = sh.shift[pair];
                 const float weight = sh.weight[pair];
-                float* to = L.outputs + static_cast<int64_t>(pair) * L.model;
+                float* to = L.outputs + static_cast<int64_t>(pair) * p.out_pitch;
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
                     const int d0 = (block * MT + m) * 16 + g;
@@ -935,7 +1015,21 @@ struct MoeWarp {
                     row[t] = static_cast<uint32_t>(phase == 0 ? pair / p.L.top_k : pair) * row_bytes;
                 }
                 int acc[MT][NT][D][4];
-                if (!products(values, row, tiles, phase == 0 && p.L.gated, c0, c1, acc)) {  // the abort flag is up
+                const bool halves = phase == 0 && p.L.gated;
+                uint32_t skew[MT][2] = {};
+                if constexpr (!S::ALIGNED) {
+                    const int8_t* w = phase == 0 ? p.L.w_in : p.L.w_out;
+                    const int ld = phase == 0 ? p.L.model : p.L.expert;
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int r = m * (halves ? 8 : 16) + h * (halves ? 8 * MT : 8) + g;
+                            const int64_t at = weight_row(phase, grp.expert * (halves ? 2 : 1), block * (halves ? 8 * MT : 16 * MT), r) * ld;
+                            skew[m][h] = static_cast<uint32_t>((reinterpret_cast<uintptr_t>(w) + at) & 15);
+                        }
+                }
+                if (!products(values, row, tiles, halves, skew, c0, c1, acc)) {  // the abort flag is up
                     round = r.rounds;
                     at = r.end;
                     continue;
@@ -1001,6 +1095,10 @@ struct MoeWarp {
 
     // Waits (bounded) for boxes still in flight: none may land after the CTA has gone.
     __device__ __forceinline__ void drain() {
+        if constexpr (!S::ALIGNED) {
+            cp_async_wait_all();
+            return;
+        }
         int give_up = 0;
         while (taken != feed.issued) {
             if (!mbar_wait(&full[taken % moe::SLOTS], (taken / moe::SLOTS) & 1, &give_up)) break;
@@ -1027,8 +1125,10 @@ __global__ void __launch_bounds__(S::THREADS, 1)
         sh.failed = 0;
         sh.complete = 0;
         fence_mbar_init();
-        prefetch_tmap(&map_in);
-        prefetch_tmap(&map_out);
+        if constexpr (S::ALIGNED) {
+            prefetch_tmap(&map_in);
+            prefetch_tmap(&map_out);
+        }
     }
     pdl_wait();
     for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS) sh.most[i] = 0;
@@ -1099,13 +1199,13 @@ __global__ void __launch_bounds__(S::THREADS, 1)
         return;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0 && L.tokens > S::WARPS) clear_tickets(L);
-    const int total = L.tokens * L.model / 4;  // model is a multiple of 16
+    const int vectors = (L.model + 3) / 4, total = L.tokens * vectors;
     for (int i = blockIdx.x * S::THREADS + threadIdx.x; i < total; i += gridDim.x * S::THREADS) {
-        const int t = i / (L.model / 4), d = (i - t * (L.model / 4)) * 4;
+        const int t = i / vectors, d = (i - t * vectors) * 4;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k = 0; k < L.top_k; k++) {
             const float4 v = __ldcg(reinterpret_cast<const float4*>(
-                L.outputs + (static_cast<int64_t>(t) * L.top_k + k) * L.model + d));
+                L.outputs + (static_cast<int64_t>(t) * L.top_k + k) * p.out_pitch + d));
             sum.x += v.x;
             sum.y += v.y;
             sum.z += v.z;
@@ -1115,6 +1215,7 @@ __global__ void __launch_bounds__(S::THREADS, 1)
         const int64_t at = static_cast<int64_t>(t) * L.model + d;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
+            if (d + u >= L.model) break;
             if constexpr (HALF) {
                 const float r = L.residual != nullptr ? __half2float(static_cast<const __half*>(L.residual)[at + u]) : 0.0f;
                 static_cast<__half*>(L.y)[at + u] = __float2half_rn(out[u] + r);
@@ -1136,17 +1237,19 @@ struct MoeChoice {
 // Groups of 8 columns hold all of an expert's tokens up to 8 tokens; groups of 16 most of them while the experts see 10
 // on average at most.
 static MoeChoice moe_choice(const MoeLaunch& L) {
-    if (L.tokens <= 2) return {1, 1, moe::Shape<1, 1>::WARPS};
+    if (L.tokens <= 2) return {1, 1, moe::Shape<1, 1, true>::WARPS};
     const int nt = L.tokens <= 8 ? 1 : L.tokens * L.top_k <= 10 * L.experts ? 2 : 4;
-    return {nt, 2, moe::Shape<1, 2>::WARPS};
+    return {nt, 2, moe::Shape<1, 2, true>::WARPS};
 }
 
 static int chunks_of(int size) { return (size + moe::CHUNK - 1) / moe::CHUNK; }
 
-bool moe_fused_eligible(const MoeLaunch& L) {
+bool moe_aligned(const MoeLaunch& L) {
     auto aligned = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
     return L.model % 16 == 0 && L.expert % 16 == 0 && aligned(L.w_in) && aligned(L.w_out);
 }
+
+static int round4(int v) { return (v + 3) & ~3; }
 
 MoeFusedSizes moe_fused_sizes(const MoeLaunch& L) {
     const int64_t pairs = int64_t(L.tokens) * L.top_k;
@@ -1157,7 +1260,8 @@ MoeFusedSizes moe_fused_sizes(const MoeLaunch& L) {
     s.h_digits = pairs * chunks_of(L.expert) * digits * moe::CHUNK;
     s.x_most = int64_t(L.tokens) * 4;
     s.h_most = pairs * 4;
-    s.outputs = pairs * L.model * 4;
+    s.outputs = pairs * round4(L.model) * 4;
+    s.hidden = pairs * round4(L.expert) * 4;
     const MoeChoice shape = moe_choice(L);
     s.segments = int64_t(L.num_sms) * shape.warps * 2 * (16 * shape.mt) * (8 * shape.nt) * int64_t(sizeof(long long));
     return s;
@@ -1189,11 +1293,20 @@ static std::function<cudaError_t(cudaStream_t)> bind_moe(const MoeFusedParams& p
         attr[0].val.cooperative = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, kern, in, out, p);
-        if (e != cudaErrorCooperativeLaunchTooLarge) return e;
-        cudaGetLastError();  // refused before anything ran
-        return launch_moe_portable(p.L, stream);
+        return cudaLaunchKernelEx(&cfg, kern, in, out, p);
     };
+}
+
+template <bool HALF, bool ALIGNED>
+static std::function<cudaError_t(cudaStream_t)> bind_moe_shape(int which, const MoeFusedParams& p, const CUtensorMap& in,
+                                                               const CUtensorMap& out) {
+    using moe::Shape;
+    switch (which) {
+        case 0: return bind_moe<HALF, Shape<1, 1, ALIGNED>>(p, in, out);
+        case 1: return bind_moe<HALF, Shape<1, 2, ALIGNED>>(p, in, out);
+        case 2: return bind_moe<HALF, Shape<2, 2, ALIGNED>>(p, in, out);
+        default: return bind_moe<HALF, Shape<4, 2, ALIGNED>>(p, in, out);
+    }
 }
 
 std::function<cudaError_t(cudaStream_t)> prepare_moe_fused(const MoeLaunch& L, cudaError_t* err) {
@@ -1210,21 +1323,23 @@ std::function<cudaError_t(cudaStream_t)> prepare_moe_fused(const MoeLaunch& L, c
     while (p.router_split < shape.warps && router_units * p.router_split * 2 <= int64_t(L.num_sms) * shape.warps)
         p.router_split *= 2;
     auto four = [](const void* q, int half) { return (reinterpret_cast<uintptr_t>(q) & (half ? 7 : 15)) == 0; };
-    p.vec = four(L.x, L.x_half) && four(L.router, L.router_half);  // model is a multiple of 16
+    p.vec = four(L.x, L.x_half) && four(L.router, L.router_half) && L.model % 4 == 0;
+    p.hidden_pitch = round4(L.expert);
+    p.out_pitch = round4(L.model);
+    p.end_in = L.w_in + int64_t(L.experts) * (L.gated ? 2 : 1) * L.expert * L.model;
+    p.end_out = L.w_out + int64_t(L.experts) * L.model * L.expert;
     const uint64_t d = L.model, f = L.expert, e = L.experts;
-    CUtensorMap in, out;
-    const bool ok = make_tensor_map_u8(&in, L.w_in, d, f, (L.gated ? 2 : 1) * e, d, d * f, moe::CHUNK, rows_in,
+    CUtensorMap in = {}, out = {};
+    const bool aligned = moe_aligned(L);
+    const bool ok = !aligned ||
+                    (make_tensor_map_u8(&in, L.w_in, d, f, (L.gated ? 2 : 1) * e, d, d * f, moe::CHUNK, rows_in,
                                        L.gated ? 2 : 1) &&
-                    make_tensor_map_u8(&out, L.w_out, f, d, e, f, d * f, moe::CHUNK, rows_out);
+                    make_tensor_map_u8(&out, L.w_out, f, d, e, f, d * f, moe::CHUNK, rows_out));
     *err = ok ? cudaSuccess : cudaErrorInvalidValue;
     if (!ok) return nullptr;
-    using moe::Shape;
-    if (shape.mt == 1) return L.x_half ? bind_moe<true, Shape<1, 1>>(p, in, out) : bind_moe<false, Shape<1, 1>>(p, in, out);
-    switch (shape.nt) {
-        case 1: return L.x_half ? bind_moe<true, Shape<1, 2>>(p, in, out) : bind_moe<false, Shape<1, 2>>(p, in, out);
-        case 2: return L.x_half ? bind_moe<true, Shape<2, 2>>(p, in, out) : bind_moe<false, Shape<2, 2>>(p, in, out);
-        default: return L.x_half ? bind_moe<true, Shape<4, 2>>(p, in, out) : bind_moe<false, Shape<4, 2>>(p, in, out);
-    }
+    const int which = shape.mt == 1 ? 0 : shape.nt;
+    if (aligned) return L.x_half ? bind_moe_shape<true, true>(which, p, in, out) : bind_moe_shape<false, true>(which, p, in, out);
+    return L.x_half ? bind_moe_shape<true, false>(which, p, in, out) : bind_moe_shape<false, false>(which, p, in, out);
 }
 
 }  // namespace og
