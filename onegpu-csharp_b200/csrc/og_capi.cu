@@ -582,63 +582,50 @@ uint8_t* own_stage(og_int8_gemm* g, int which, int64_t bytes) {
     return static_cast<uint8_t*>(p);
 }
 
-// Copies one operand (`rows` x `width` bytes per batch, `ld` apart, batches `stride` apart) into a pitched buffer of
-// the instance whose rows start on 16-byte boundaries, recording the copies; returns the new pitch.
-int64_t stage_operand(og_int8_gemm* g, og_encoder* enc, int which, const uint8_t*& base, int64_t ld, int64_t& stride,
-                      int batches, int64_t rows, int64_t width) {
-    const int64_t pitch = (width + 15) & ~int64_t(15);
-    uint8_t* dst = own_stage(g, which, batches * rows * pitch);
-    const uint8_t* src = base;
-    const int64_t sstride = stride;
-    if (batches == 1 || sstride == rows * ld) {
-        // One two-dimensional copy covers every batch (shared, or dense batches).
-        const int64_t height = (batches == 1 ? 1 : batches) * rows;
-        enc->ops.push_back([=](cudaStream_t s) {
-            return cudaMemcpy2DAsync(dst, static_cast<size_t>(pitch), src, static_cast<size_t>(ld),
-                                     static_cast<size_t>(width), static_cast<size_t>(height), cudaMemcpyDeviceToDevice,
-                                     s);
-        });
-    } else {
-        enc->ops.push_back([=](cudaStream_t s) {
-            for (int b = 0; b < batches; b++) {
-                const cudaError_t e = cudaMemcpy2DAsync(dst + b * rows * pitch, static_cast<size_t>(pitch),
-                                                        src + b * sstride, static_cast<size_t>(ld),
-                                                        static_cast<size_t>(width), static_cast<size_t>(rows),
-                                                        cudaMemcpyDeviceToDevice, s);
-                if (e != cudaSuccess) return e;
-            }
-            return cudaSuccess;
-        });
-    }
-    base = dst;
-    stride = batches > 1 ? rows * pitch : 0;
-    return pitch;
+// Points one operand (`rows` x `width` bytes per batch, `ld` apart, batches `stride` apart) at a pitched buffer of the
+// instance whose rows start on 16-byte boundaries; the copy that fills it.
+og::StageJob stage_operand(og_int8_gemm* g, int which, const uint8_t*& base, int64_t& ld, int64_t& stride, int batches,
+                           int64_t rows, int64_t width) {
+    og::StageJob job = {};
+    job.src = base;
+    job.ld = ld;
+    job.stride = stride;
+    job.pitch = (width + 15) & ~int64_t(15);
+    job.rows = rows;
+    job.width = width;
+    job.batches = batches;
+    job.dst = own_stage(g, which, batches * rows * job.pitch);
+    base = job.dst;
+    ld = job.pitch;
+    stride = batches > 1 ? rows * job.pitch : 0;
+    return job;
 }
 
 // Products large enough for the tensor cores whose A or B rows (or batches) do not start on 16-byte boundaries, so
 // that TMA cannot load them in place: the misaligned operand is copied into a pitched buffer (rows padded to 16 bytes;
 // the padding is never read) and the tensor-core product runs on the copy. The copy moves each operand byte once;
 // the portable kernel it replaces runs far below the tensor cores' rate at these sizes.
+// Activated products are always staged: the portable kernel walks K on a CTA per tile (2 x 333 x 6001: 1079 us, staged
+// 13.5; 1 x 1001 x 1001 184 and 12; for K of a few dozen the two are level: 64 x 65 x 33 21.5 and 19.5).
 constexpr int64_t kStageMinOps = int64_t(1) << 27;
 
 bool stage_for_tensor_cores(og_int8_gemm* g, og_encoder* enc, og::GemmLaunch& L) {
-    if (L.k < 1 || L.m < 1 || L.n < 1 || 2.0 * L.m * L.n * L.k * L.batch < double(kStageMinOps)) return false;
+    if (L.k < 1 || L.m < 1 || L.n < 1) return false;
+    if (!og::out_activated(L.epi.out_kind) && 2.0 * L.m * L.n * L.k * L.batch < double(kStageMinOps)) return false;
     auto misaligned = [](const uint8_t* p, int64_t ld, int64_t stride, int batches) {
         return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (ld & 15) != 0 || (batches > 1 && (stride & 15) != 0);
     };
     const int ba = (L.batch > 1 && L.stride_a != 0) ? L.batch : 1;
     const int bb = (L.batch > 1 && L.stride_b != 0) ? L.batch : 1;
-    bool staged = false;
-    if (misaligned(L.a, L.lda, L.stride_a, ba)) {
-        L.lda = stage_operand(g, enc, 0, L.a, L.lda, L.stride_a, ba, L.m, L.k);
-        staged = true;
-    }
+    og::StageJob a = {}, b = {};
+    if (misaligned(L.a, L.lda, L.stride_a, ba)) a = stage_operand(g, 0, L.a, L.lda, L.stride_a, ba, L.m, L.k);
     if (misaligned(L.b, L.ldb, L.stride_b, bb)) {
         const int64_t rows = L.trans_b ? L.n : L.k, width = L.trans_b ? L.k : L.n;
-        L.ldb = stage_operand(g, enc, 1, L.b, L.ldb, L.stride_b, bb, rows, width);
-        staged = true;
+        b = stage_operand(g, 1, L.b, L.ldb, L.stride_b, bb, rows, width);
     }
-    return staged;
+    if (a.src == nullptr && b.src == nullptr) return false;
+    enc->ops.push_back([a, b](cudaStream_t s) { return og::launch_stage(a, b, s); });
+    return true;
 }
 
 void record_gemm(og_int8_gemm* g, og_encoder* enc, og::GemmLaunch L, const og_operand* caller_scratch) {
@@ -655,7 +642,9 @@ void record_gemm(og_int8_gemm* g, og_encoder* enc, og::GemmLaunch L, const og_op
                     "boundaries",
                     "TensorCoreInt8", "16-byte aligned operands", "unaligned operand or K = 0");
     }
-    if (tc && g->kernel == OG_KERNEL_AUTO && static_cast<int64_t>(L.m) * L.n * L.k < (int64_t(1) << 16)) tc = false;
+    if (tc && g->kernel == OG_KERNEL_AUTO && !og::out_activated(L.epi.out_kind) &&
+        static_cast<int64_t>(L.m) * L.n * L.k < (int64_t(1) << 16))
+        tc = false;
     if (!tc) {
         g->last = "portable";
         enc->ops.push_back([L](cudaStream_t s) { return og::launch_gemm_simt(L, s); });

@@ -105,6 +105,19 @@ LaunchFn prepare_gemm_slim(const GemmLaunch& L, int parts, cudaError_t* err);
 bool make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t x, uint64_t y, uint64_t z, uint64_t stride_y,
                         uint64_t stride_z, uint32_t box_x, uint32_t box_y, uint32_t box_z = 1);
 
+// Copies `batches` x `rows` rows of `width` bytes, ld (batches stride) apart, to rows `pitch` apart (og_stage.cu): pitch is
+// width rounded up to 16, dst 16-byte aligned; what the padding holds is not defined. One launch for two jobs, the second
+// (or first) with a null src for none.
+struct StageJob {
+    const uint8_t* src;
+    uint8_t* dst;
+    int64_t ld, stride, pitch, rows, width;
+    int batches;
+    int lanes_log2;  // set by the launch, as is `blocks`
+    int64_t blocks;
+};
+cudaError_t launch_stage(StageJob a, StageJob b, cudaStream_t stream);
+
 // Portable SIMT product (og_gemm_simt.cu): any alignment, subtracts the zero points while staging, so it needs no
 // byte sums; its epilogue ignores row_sum_a / col_sum_b.
 cudaError_t launch_gemm_simt(const GemmLaunch& L, cudaStream_t stream);
