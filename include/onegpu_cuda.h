@@ -231,7 +231,8 @@ OG_API og_status og_int8_gemm_destroy(og_int8_gemm* gemm);
 OG_API og_status og_int8_gemm_variant(og_int8_gemm* gemm, char* buffer, uint64_t capacity);
 /* The kernel the last encode call recorded: "tensor-core-2sm" or "tensor-core-1sm" (with "-stream-k" when the
  * product's (tile, K block) work was split evenly across the SMs), "tensor-core-rows", "tensor-core-slim" (an
- * activated product of few rows), "portable" or "none". */
+ * activated product of few rows or few tiles), each with "-staged" when an operand is copied to 16-byte boundaries first,
+ * "portable" or "none". */
 OG_API og_status og_int8_gemm_last_kernel(og_int8_gemm* gemm, char* buffer, uint64_t capacity);
 /* Int8Gemm.ScratchElements (Int8Gemm.cs:531). */
 OG_API int64_t og_int8_gemm_scratch_elements(const og_int8_gemm_problem* problem);

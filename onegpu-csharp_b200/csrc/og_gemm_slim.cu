@@ -8,8 +8,8 @@
 // finishes every P-th row from all of them. Against whole tiles (128 x 256 per CTA: 32 CTAs for 8192 columns) and against
 // the even split with records in global memory and a ticket per tile: see the rule in slim_parts.
 //
-// Warp 0 loads (TMA, no multicast), warp 1 issues the MMAs, warps 2-5 sum the rows of A over the CTA's share of K while B
-// streams (the zero point of B needs them), then drain TMEM (lane = column) and finish: stores and residual reads run
+// Warp 0 loads (TMA, no multicast), warp 1 issues the MMAs, warps 2-5 sum the rows of A in the boxes (the zero
+// point of B needs them), then drain TMEM (lane = column) and finish: stores and residual reads run
 // along N. Every wait on an mbarrier is bounded; the cluster's own barriers are always reached, by CTAs that gave up too.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -52,8 +52,6 @@ struct SlimParams {
     int k_blocks;
     int tiles, row_chunks;  // column tiles and chunks of MR rows of one batch
     int a_batched, b_batched;
-    int64_t lda, stride_a;  // for the row sums of A, read from global memory
-    const uint8_t* a;
     Epilogue epi;
     int* error_flag;
 };
@@ -114,7 +112,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], p.epi.zb != nullptr ? 5 : 1);  // the MMAs, and the four warps that sum the rows of A
         }
         mbar_init(tfull, 1);
         *abort_flag = 0;
@@ -193,42 +191,25 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
             row_zero[r] = zp_value(e.za, e.za_vector, e.za_signed, row0 + r);
         }
         if (e.zb != nullptr) {
-            // Row sums of A over this CTA's share of K: a warp per row, four rows' loads of 2 KB in flight.
-            const int k0 = kb0 * slim::BK, k1 = min(p.k, kb1 * slim::BK);
-            const int k_vec = k1 & ~15;
-            for (int r0 = w; r0 < MR && row0 + r0 < p.m; r0 += 16) {
-                int32_t sum[4] = {0, 0, 0, 0};
-                const uint8_t* row[4];
+            // Row sums of A over this CTA's share of K, from the boxes in shared memory (zeros past K and M): LANES threads
+            // a row. The order of a row's 16-byte units does not matter, so the swizzle is not undone but used: lanes of
+            // different rows read different units.
+            constexpr int LANES = slim::FINISH_THREADS / MR, UNITS = 8 / LANES;
+            const int r = t / LANES, u0 = (t % LANES) * UNITS;
+            int32_t sum = 0;
+            for (int kb = kb0; kb < kb1; kb++) {
+                const int it = kb - kb0, s = it % C::STAGES;
+                if (!mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag)) break;
+                const uint4* box = reinterpret_cast<const uint4*>(sX + s * C::A_BYTES + r * slim::BK);
 #pragma unroll
-                for (int i = 0; i < 4; i++)  // past the rows, the last one again (its sum is not used)
-                    row[i] = p.a + ba * p.stride_a + min(row0 + r0 + 4 * i, p.m - 1) * p.lda;
-#pragma unroll 1
-                for (int k = k0 + lane * 16; k < k_vec; k += 2048) {
-                    uint4 v[4][4];
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            v[u][i] = k + 512 * u < k_vec ? __ldg(reinterpret_cast<const uint4*>(row[i] + k + 512 * u))
-                                                          : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) sum[i] = byte_sum(v[u][i], e.za_signed, sum[i]);
-                }
-                if (k_vec + lane < k1) {  // the last K % 16 bytes
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint8_t x = __ldg(row[i] + k_vec + lane);
-                        sum[i] += e.za_signed ? static_cast<int32_t>(static_cast<int8_t>(x)) : x;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int32_t all = __reduce_add_sync(0xFFFFFFFFu, sum[i]);
-                    if (lane == 0 && r0 + 4 * i < MR) row_sum[r0 + 4 * i] = all;
-                }
+                for (int i = 0; i < UNITS; i++) sum = byte_sum(box[(u0 + i) ^ (r & 7)], e.za_signed, sum);
+                asm volatile("" ::"r"(sum) : "memory");  // the reads are done before the box is given back
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[s]);
             }
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            if (t % LANES == 0) row_sum[r] = sum;
         }
         if (t == 0) *ready = mbar_wait(tfull, 0, abort_flag) ? 1 : 0;
         asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -339,7 +320,65 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
 
 static int slim_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
 
-// The parts of K that a cluster shares, or 0 when the kernel for whole tiles serves better.
+// Sets the kernel's shared memory once per device.
+template <int MR, class Kernel>
+static cudaError_t configure_slim(Kernel kern, std::atomic<uint64_t>& configured) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (configured.load() & bit) return cudaSuccess;
+    const cudaError_t set = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, slim::Cfg<MR>::SMEM_BYTES);
+    if (set == cudaSuccess) configured.fetch_or(bit);
+    return set;
+}
+
+// Clusters of `parts` CTAs that the current device holds at once (a cluster stays within a group of SMs, so this is less
+// than its CTA slots over `parts`). One of the kernels of MR stands for all: they hold as much shared memory.
+template <int MR>
+static int slim_clusters_at_once(int parts) {
+    static std::atomic<int> known[64][slim::MAX_PARTS + 1] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::atomic<int>& slot = known[dev & 63][parts];
+    if (slot.load() != 0) return slot.load();
+    static std::atomic<uint64_t> configured{0};
+    auto kern = int8_gemm_slim_kernel<MR, true, OUT_ACT_F32>;
+    if (configure_slim<MR>(kern, configured) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, static_cast<unsigned>(parts));
+    cfg.blockDim = dim3(slim::THREADS);
+    cfg.dynamicSmemBytes = slim::Cfg<MR>::SMEM_BYTES;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = static_cast<unsigned>(parts);
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess) return 0;
+    slot.store(clusters);
+    return clusters;
+}
+
+static int slim_clusters_at_once(int mr, int parts) {
+    switch (mr) {
+        case 16: return slim_clusters_at_once<16>(parts);
+        case 32: return slim_clusters_at_once<32>(parts);
+        case 64: return slim_clusters_at_once<64>(parts);
+        default: return slim_clusters_at_once<128>(parts);
+    }
+}
+
+// The parts of K that a cluster shares, or 0 when the kernel for whole tiles serves better. Up to 64 rows always. From 65
+// rows on K needs some length to outweigh the finish, less where whole tiles would need a pass for the byte sums:
+// 512 x 2048 x 512 with zero points 23.3 us in whole tiles and 19.4 here, 4096 x 512 x 512 without 17.3 and 19.5. Each 128
+// rows read B again (from L2), which pays while whole tiles would leave SMs idle: 256 x 8192 x 8192 55 and 45, 300 x 512 x
+// 4096 28.7 and 17.4, 2048 x 256 x 1024 19.3 and 17.3, 2048 x 1024 x 2048 (the edge of the rule) 22.7 and 23.5, with zero
+// points 27.6 and 25.6.
+// As many parts as still run at once: a cluster left over would wait for a whole pass (5 x 5120 x 5120 with one part more
+// 23.4, without 17.4).
 int slim_parts(const GemmLaunch& L) {
     if (!out_activated(L.epi.out_kind) || !tc_eligible(L) || L.batch > 65535) return 0;
     const int mr = slim_rows(L.m);
@@ -348,8 +387,14 @@ int slim_parts(const GemmLaunch& L) {
     const int64_t slots = 2 * static_cast<int64_t>(L.num_sms);  // two CTAs on each SM
     const int64_t k_blocks = (L.k + slim::BK - 1) / slim::BK;
     if (tiles > 0x7FFFFFFF) return 0;
-    if (chunks > 2 || (chunks == 2 && 2 * tiles > slots) || (L.m > 64 && k_blocks < 8)) return 0;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({slots / tiles, k_blocks / 2, slim::MAX_PARTS})));
+    if (L.m > 64 && k_blocks < (L.epi.za != nullptr || L.epi.zb != nullptr ? 4 : 8)) return 0;
+    if (chunks > 1 && 2 * tiles > slots) return 0;
+    int64_t parts = std::max<int64_t>(1, std::min<int64_t>({slots / tiles, k_blocks / 2, slim::MAX_PARTS}));
+    auto at_once = [&](int64_t size) {  // the query counts one CTA on an SM
+        return slots / std::max(1, slim_clusters_at_once(mr, 1)) * slim_clusters_at_once(mr, static_cast<int>(size));
+    };
+    while (parts > 1 && at_once(parts) < tiles) parts--;
+    return static_cast<int>(parts);
 }
 
 template <int MR, bool B_KMAJOR, int OUT>
@@ -359,15 +404,8 @@ static LaunchFn bind_slim_t(const SlimParams& p, const CUtensorMap& ma, const CU
         using C = slim::Cfg<MR>;
         auto kern = int8_gemm_slim_kernel<MR, B_KMAJOR, OUT>;
         static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
+        const cudaError_t e = configure_slim<MR>(kern, configured);
         if (e != cudaSuccess) return e;
-        const uint64_t bit = uint64_t(1) << (dev & 63);
-        if (!(configured.load() & bit)) {
-            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
-            if (e != cudaSuccess) return e;
-            configured.fetch_or(bit);
-        }
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = grid;
         cfg.blockDim = dim3(slim::THREADS);
@@ -423,9 +461,6 @@ LaunchFn prepare_gemm_slim(const GemmLaunch& L, int parts, cudaError_t* err) {
     p.row_chunks = (L.m + mr - 1) / mr;
     p.a_batched = ba > 1;
     p.b_batched = bb > 1;
-    p.lda = L.lda;
-    p.stride_a = L.stride_a;
-    p.a = L.a;
     p.epi = L.epi;
     p.error_flag = L.error_flag;
     const dim3 grid(static_cast<unsigned>(p.tiles * p.row_chunks * L.batch), static_cast<unsigned>(parts));
