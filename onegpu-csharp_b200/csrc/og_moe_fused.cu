@@ -11,7 +11,7 @@
 //     barrier.
 //  2. Output products: units of one group and 16 rows of w_out; weighted results per pair. Grid barrier.
 //  3. The sum over each token's pairs, in the order of their rank: the result does not depend on the schedule.
-// A CTA owns a contiguous range of units and its warps equal contiguous ranges of the units' chunks; a unit cut between
+// A CTA owns a contiguous range of units of equal cost (unit_cost) and its warps equal contiguous ranges of the units' chunks; a unit cut between
 // warps meets through partial sums (`segments`), added by the warp that holds its start. Each warp feeds itself: a ring of
 // SLOTS 2 KB boxes loaded by TMA (128-byte swizzle, no multicast), the next box issued as soon as one is in registers. The
 // ring runs on into phase 2's weights, which do not depend on the barriers: DRAM stays busy while the hidden values
@@ -83,8 +83,19 @@ struct MoeFusedParams {
 
 // A group: one expert and a run of the pairs sorted by expert.
 struct MoeGroup {
-    uint16_t expert, first, count, pad;
+    uint16_t expert, first, count;
+    uint16_t before;  // the cost of a unit of every group before it
 };
+
+// What a unit of a group costs next to others: its columns' digits come from L1 or L2 and cost more the more of them
+// differ, and each further tile has its own loads and products. Shares of equal bytes took, in us a phase: 64 tokens through
+// 6 of 64 experts (2048 x 1408) 66 with up to 6 pairs, 71 with 7 or 8, 89 with 9 to 12 (a second tile); 8 tokens through 2
+// of 8 experts (4096 x 8192) 80 (phase 1) and 39 (2) with one pair, 88 and 48 with 2 to 4; NT = 4, two, three and four
+// tiles 50, 68 and 86.
+template <int NT>
+__device__ __forceinline__ int unit_cost(int pairs) {
+    return (pairs == 1 ? 16 : pairs <= 6 ? 18 : 20) + (pairs - 1) / 8 * (NT == 4 ? 12 : 5);
+}
 
 template <class S>
 struct MoeShared {
@@ -101,6 +112,7 @@ struct MoeShared {
     int warp_total[2][S::WARPS];
     unsigned complete;                 // token blocks whose logits this CTA completed
     int groups;
+    int cost;                          // of a unit of every group
     int abort;
     int failed;
 };
@@ -527,13 +539,14 @@ __device__ __forceinline__ void moe_group(const MoeLaunch& L, MoeShared<S>& sh) 
         rank[i] = atomicAdd(&sh.count[sh.id[pair]], 1);
     }
     __syncthreads();
-    int count[EXPERTS], first = 0, group = 0;
+    int count[EXPERTS], first = 0, group = 0;  // pairs; groups and, from bit 10 on, their units' cost (at most 768 and 40000)
     bool many = false;
 #pragma unroll
     for (int i = 0; i < EXPERTS; i++) {
         count[i] = sh.count[thread * EXPERTS + i];
         first += count[i];
-        group += (count[i] + FULL - 1) / FULL;
+        group += (count[i] + FULL - 1) / FULL + (count[i] / FULL * unit_cost<S::NT>(FULL) << 10);
+        if (count[i] % FULL != 0) group += unit_cost<S::NT>(count[i] % FULL) << 10;
         many |= count[i] > FULL;
     }
     if (__syncthreads_or(many)) {
@@ -577,16 +590,24 @@ __device__ __forceinline__ void moe_group(const MoeLaunch& L, MoeShared<S>& sh) 
             first += sh.warp_total[0][w];
             group += sh.warp_total[1][w];
         }
-    if (thread == S::THREADS - 1) sh.groups = group;
+    if (thread == S::THREADS - 1) {
+        sh.groups = group & 1023;
+        sh.cost = group >> 10;
+    }
     first -= own;
     group -= own_groups;
+    int cost = group >> 10;
+    group &= 1023;
 #pragma unroll
     for (int i = 0; i < EXPERTS; i++) {
         const int e = thread * EXPERTS + i;
         sh.count[e] = first;
-        for (int done = 0; done < count[i]; done += FULL)
+        for (int done = 0; done < count[i]; done += FULL) {
+            const int n = min(FULL, count[i] - done);
             sh.group[group++] = MoeGroup{static_cast<uint16_t>(e), static_cast<uint16_t>(first + done),
-                                         static_cast<uint16_t>(min(FULL, count[i] - done)), 0};
+                                         static_cast<uint16_t>(n), static_cast<uint16_t>(cost)};
+            cost += unit_cost<S::NT>(n);
+        }
         first += count[i];
     }
     __syncthreads();
@@ -613,11 +634,36 @@ struct MoeRange {
     int at, end;  // the warp's run of the cut units' chunks
 };
 
+// Where the share of CTA `block` starts: a group, and how far into its units (a fraction of 2^16). Shares cost the same.
+struct MoePlace {
+    int group;
+    uint32_t into;
+    __device__ __forceinline__ int unit(int blocks) const {
+        return group * blocks + static_cast<int>((static_cast<uint64_t>(into) * blocks) >> 16);
+    }
+};
+
 template <class S>
-__device__ __forceinline__ MoeRange moe_range(int units, int chunks, int warp) {
+__device__ __forceinline__ MoePlace moe_place(const MoeShared<S>& sh, unsigned block) {
+    const unsigned scaled = static_cast<unsigned>(sh.cost) * block, whole = scaled / gridDim.x;  // below 2^16 * 2^10
+    const unsigned part = ((scaled - whole * gridDim.x) << 16) / gridDim.x;
+    int low = 0, high = sh.groups;  // the last group that does not start past it
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (sh.group[mid].before <= whole)
+            low = mid;
+        else
+            high = mid;
+    }
+    const MoeGroup& g = sh.group[low];
+    return {low, ((whole - g.before) << 16 | part) / static_cast<unsigned>(unit_cost<S::NT>(g.count))};
+}
+
+template <class S>
+__device__ __forceinline__ MoeRange moe_range(int first, int past, int chunks, int warp) {
     MoeRange r;
-    r.u0 = moe_split(units, blockIdx.x, gridDim.x);
-    r.units = moe_split(units, blockIdx.x + 1, gridDim.x) - r.u0;
+    r.u0 = first;
+    r.units = past - first;
     r.rounds = r.units / S::WARPS;
     r.tail = r.rounds * S::WARPS;
     int left = r.units - r.tail;
@@ -645,6 +691,7 @@ struct MoeFeed {
     int left;          // boxes left of this run of boxes (a unit, or the run over the cut units)
     int x, x_end;      // byte of K of the next box, and past the last one
     int y, e;          // row and expert (gate half) of the next box
+    bool whole;        // a whole unit, walked around from its first box
     uint32_t issued;   // boxes so far
 };
 
@@ -662,6 +709,12 @@ struct MoeWarp {
     MoeFeed feed;
     uint32_t taken;  // boxes read so far
     float2 scale[MT];  // of the unit at hand
+
+    // Whole units are walked around from a chunk that differs from CTA to CTA: in step, all CTAs would read the same few
+    // columns of rows a power of two apart (8 tokens through 2 of 2 experts, 4096 x 8192: phase 1 33.3 us in step, 26.9 so).
+    __device__ __forceinline__ static int first_chunk(int chunks) {
+        return MT == 1 ? 0 : static_cast<int>(static_cast<unsigned>(chunks) * blockIdx.x / gridDim.x);
+    }
 
     __device__ __forceinline__ int chunks(int phase) const { return phase == 0 ? p.chunks_in : p.chunks_out; }
     __device__ __forceinline__ int blocks(int phase) const { return phase == 0 ? p.blocks_in : p.blocks_out; }
@@ -682,8 +735,9 @@ struct MoeWarp {
             const int c = chunks(feed.phase);
             if (feed.rounds < r.rounds) {
                 aim(r.u0 + feed.rounds * S::WARPS + warp);
-                feed.x = 0;
+                feed.x = first_chunk(c) * moe::CHUNK;
                 feed.x_end = c * moe::CHUNK;
+                feed.whole = true;
                 feed.left = c;
                 feed.rounds++;
                 return true;
@@ -695,6 +749,7 @@ struct MoeWarp {
                 feed.x = (r.at - local * c) * moe::CHUNK;
                 feed.x_end = c * moe::CHUNK;
                 feed.left = r.end - r.at;
+                feed.whole = false;
                 return true;
             }
             if (feed.phase == 1) return false;
@@ -754,7 +809,7 @@ struct MoeWarp {
         feed.x += moe::CHUNK;
         if (feed.x == feed.x_end && feed.left > 0) {
             feed.x = 0;
-            aim(feed.unit + 1);
+            if (!feed.whole) aim(feed.unit + 1);
         }
     }
 
@@ -770,7 +825,8 @@ struct MoeWarp {
     // t in acc[i][t][digit]. The columns' digits start at values + row[t] (column g of the tile). `halves`: the box holds
     // the gate's rows, then the other half's, and a tile 8 of each.
     __device__ __forceinline__ bool products(const uint8_t* values, const uint32_t (&row)[NT], int tiles, bool halves,
-                                             const uint32_t (&skew)[MT][2], int c0, int c1, int (&acc)[MT][NT][D][4]) {
+                                             const uint32_t (&skew)[MT][2], int c0, int count, int wrap,
+                                             int (&acc)[MT][NT][D][4]) {
         // Where registers allow, the next chunk's digits are on their way while one is multiplied (64 tokens through 6 of
         // 64 experts 172 -> 165 us); elsewhere tile 0's are asked for before the wait for the box and the other tiles' when
         // their turn comes (with NT = 4 or at 16 warps the earlier loads only spill).
@@ -799,7 +855,14 @@ struct MoeWarp {
                 if (t < tiles) load_digits(next[t], v + row[t]);
         }
 #pragma unroll 1
-        for (int c = c0; c < c1; c++, v += D * moe::CHUNK) {
+        for (int c = c0; count > 0; count--) {
+            const uint8_t* here = v;
+            if (++c == wrap) {
+                c = 0;
+                v = values + q * 16;
+            } else {
+                v += D * moe::CHUNK;
+            }
             const int slot = taken % moe::SLOTS;
             uint4 b[EARLY][D][2];
             if constexpr (AHEAD) {
@@ -809,13 +872,13 @@ struct MoeWarp {
                     for (int d = 0; d < D; d++)
 #pragma unroll
                         for (int j = 0; j < 2; j++) b[t][d][j] = next[t][d][j];
-                if (c + 1 < c1) {
+                if (count > 1) {
 #pragma unroll
                     for (int t = 0; t < EARLY; t++)
-                        if (t < tiles) load_digits(next[t], v + D * moe::CHUNK + row[t]);
+                        if (t < tiles) load_digits(next[t], v + row[t]);
                 }
             } else {
-                load_digits(b[0], v + row[0]);
+                load_digits(b[0], here + row[0]);
             }
             uint32_t a[MT][4][4];
             if constexpr (S::ALIGNED) {
@@ -850,7 +913,7 @@ struct MoeWarp {
             for (int t = 0; t < NT; t++) {
                 if (t >= tiles) break;
                 uint4 (&bt)[D][2] = b[t % EARLY];
-                if (t >= EARLY) load_digits(bt, v + row[t]);
+                if (t >= EARLY) load_digits(bt, here + row[t]);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
 #pragma unroll
@@ -1029,7 +1092,7 @@ struct MoeWarp {
                             skew[m][h] = static_cast<uint32_t>((reinterpret_cast<uintptr_t>(w) + at) & 15);
                         }
                 }
-                if (!products(values, row, tiles, halves, skew, c0, c1, acc)) {  // the abort flag is up
+                if (!products(values, row, tiles, halves, skew, in_round ? first_chunk(c) : c0, c1 - c0, c, acc)) {  // the abort flag is up
                     round = r.rounds;
                     at = r.end;
                     continue;
@@ -1165,8 +1228,21 @@ __global__ void __launch_bounds__(S::THREADS, 1)
     moe_group(L, sh);
 
     MoeWarp<S, D> me{p, sh, &map_in, &map_out, smem + warp * moe::SLOTS * S::BOX, sh.full[warp], warp, lane, {}, {}, {}, 0, {}};
-    me.range_in = moe_range<S>(sh.groups * p.blocks_in, p.chunks_in, warp);
-    me.range_out = moe_range<S>(sh.groups * p.blocks_out, p.chunks_out, warp);
+    if constexpr (S::MT == 1) {  // one or two tokens: every unit costs the same
+        const int units_in = sh.groups * p.blocks_in, units_out = sh.groups * p.blocks_out;
+        me.range_in = moe_range<S>(moe_split(units_in, blockIdx.x, gridDim.x), moe_split(units_in, blockIdx.x + 1, gridDim.x),
+                                   p.chunks_in, warp);
+        me.range_out = moe_range<S>(moe_split(units_out, blockIdx.x, gridDim.x),
+                                    moe_split(units_out, blockIdx.x + 1, gridDim.x), p.chunks_out, warp);
+    } else {
+        const MoePlace mine = moe_place(sh, blockIdx.x + (lane & 1));  // even lanes: the share's start, odd ones: its end
+        auto of = [&](int l) {
+            return MoePlace{__shfl_sync(0xFFFFFFFFu, mine.group, l), __shfl_sync(0xFFFFFFFFu, mine.into, l)};
+        };
+        const MoePlace from = of(0), to = of(1);
+        me.range_in = moe_range<S>(from.unit(p.blocks_in), to.unit(p.blocks_in), p.chunks_in, warp);
+        me.range_out = moe_range<S>(from.unit(p.blocks_out), to.unit(p.blocks_out), p.chunks_out, warp);
+    }
     for (int s = 0; s < moe::SLOTS; s++) me.issue();
 
 #pragma unroll 1
