@@ -441,43 +441,72 @@ struct DqRow {
             }
         }
     }
+    // float16 pairs are folded as they are; NaN is skipped like fminf and fmaxf do.
     __device__ __forceinline__ static void fold(const uint4& w, float& mn, float& mx) {
-        float v[E];
-        unpack(w, v);
+        if constexpr (HALF) {
+            const __half2* h = reinterpret_cast<const __half2*>(&w);
+            const float2 lo = __half22float2(__hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3])));
+            const float2 hi = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+            mn = fminf(mn, fminf(lo.x, lo.y));
+            mx = fmaxf(mx, fmaxf(hi.x, hi.y));
+        } else {
+            const float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            mn = fminf(mn, v[i]);
-            mx = fmaxf(mx, v[i]);
+            for (int i = 0; i < 4; i++) {
+                mn = fminf(mn, v[i]);
+                mx = fmaxf(mx, v[i]);
+            }
         }
     }
     __device__ __forceinline__ static void store(const uint4& w, uint8_t* y, bool aligned, const DqQuant& q) {
         float v[E];
         unpack(w, v);
+        // DqQuant::one for all of them, with one branch. The products are off from the float32 quotients by at most
+        // 256 (2^-23 + 2^-24) < 2^-14 (x lies in the row's range, so |x / s| <= 256): only that near a tie the quotient
+        // itself decides, in one of 8192 elements.
+        uint32_t code[E];
+        bool ok = q.r_ok;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const float m = __fmul_rn(v[i], q.r);
+            const float t = __fadd_rn(m, q.cz);
+            const float d = __fsub_rn(m, __fsub_rn(t, q.cz));
+            ok = ok && fabsf(d) < 0.5f - 0x1p-14f;
+            code[i] = min(max(__float_as_uint(t), 0x4B400000u), 0x4B4000FFu);
+        }
+        if (!ok) {
+#pragma unroll
+            for (int i = 0; i < E; i++) code[i] = q.one(v[i]);
+        }
         if (aligned) {
+            uint32_t word[E / 4];
+#pragma unroll
+            for (int i = 0; i < E / 4; i++)
+                word[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040),
+                                      __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410);
             if constexpr (HALF)
-                *reinterpret_cast<uint2*>(y) = make_uint2(q.four(make_float4(v[0], v[1], v[2], v[3])),
-                                                          q.four(make_float4(v[4], v[5], v[6], v[7])));
+                *reinterpret_cast<uint2*>(y) = make_uint2(word[0], word[1]);
             else
-                *reinterpret_cast<uint32_t*>(y) = q.four(make_float4(v[0], v[1], v[2], v[3]));
+                *reinterpret_cast<uint32_t*>(y) = word[0];
         } else {
 #pragma unroll
-            for (int i = 0; i < E; i++) y[i] = static_cast<uint8_t>(q.one(v[i]));
+            for (int i = 0; i < E; i++) y[i] = static_cast<uint8_t>(code[i]);
         }
     }
 };
 
-// TPR threads per row: a warp, or the whole block.
+// TPR threads per row: a warp (8 rows a block), or the whole block.
 template <bool HALF, int TPR>
-__global__ void __launch_bounds__(DQR_THREADS)
+__global__ void __launch_bounds__(TPR == 32 ? DQR_THREADS : TPR)
     dq_rows_kernel(const void* __restrict__ x, int64_t rows, int columns, int64_t row_stride, uint8_t* __restrict__ y,
                    float* __restrict__ scale_out, uint8_t* __restrict__ zp_out) {
     using Row = DqRow<HALF>;
-    constexpr int E = Row::E;
+    constexpr int E = Row::E, KEEP = TPR == 32 ? DQR_KEEP : 2 * DQR_KEEP;
     __shared__ float smin[32], smax[32];
     __shared__ float range[2];
     pdl_trigger();
     pdl_wait();
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (DQR_THREADS / TPR) + threadIdx.x / TPR;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (TPR == 32 ? DQR_THREADS / TPR : 1) + threadIdx.x / TPR;
     if (row >= rows) return;  // whole warps (a block's one row always exists)
     const int t = threadIdx.x % TPR;
     const int64_t size = HALF ? 2 : 4;
@@ -491,17 +520,17 @@ __global__ void __launch_bounds__(DQR_THREADS)
     const uint4 none = HALF ? make_uint4(0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u)   // NaN, skipped
                             : make_uint4(0x7FC00000u, 0x7FC00000u, 0x7FC00000u, 0x7FC00000u);  // by fminf / fmaxf
     float mn = INFINITY, mx = -INFINITY;
-    uint4 keep[DQR_KEEP];
+    uint4 keep[KEEP];
 #pragma unroll
-    for (int j = 0; j < DQR_KEEP; j++) keep[j] = t + j * TPR < nvec ? __ldg(xv + t + j * TPR) : none;
+    for (int j = 0; j < KEEP; j++) keep[j] = t + j * TPR < nvec ? __ldg(xv + t + j * TPR) : none;
     for (int i = t; i < head + (columns - tail0); i += TPR) {
         const float v = Row::at(xr, i < head ? i : tail0 + i - head);
         mn = fminf(mn, v);
         mx = fmaxf(mx, v);
     }
-    for (int i = t + DQR_KEEP * TPR; i < nvec; i += TPR) Row::fold(__ldg(xv + i), mn, mx);
+    for (int i = t + KEEP * TPR; i < nvec; i += TPR) Row::fold(__ldg(xv + i), mn, mx);
 #pragma unroll
-    for (int j = 0; j < DQR_KEEP; j++) Row::fold(keep[j], mn, mx);
+    for (int j = 0; j < KEEP; j++) Row::fold(keep[j], mn, mx);
     if constexpr (TPR == 32) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -532,9 +561,9 @@ __global__ void __launch_bounds__(DQR_THREADS)
     uint8_t* yv = yr + head;
     const bool aligned = (reinterpret_cast<uintptr_t>(yv) & (E - 1)) == 0;
 #pragma unroll
-    for (int j = 0; j < DQR_KEEP; j++)
+    for (int j = 0; j < KEEP; j++)
         if (t + j * TPR < nvec) Row::store(keep[j], yv + static_cast<int64_t>(t + j * TPR) * E, aligned, q);
-    for (int i = t + DQR_KEEP * TPR; i < nvec; i += TPR)
+    for (int i = t + KEEP * TPR; i < nvec; i += TPR)
         Row::store(__ldg(xv + i), yv + static_cast<int64_t>(i) * E, aligned, q);
     for (int i = t; i < head + (columns - tail0); i += TPR) {
         const int c = i < head ? i : tail0 + i - head;
@@ -551,8 +580,12 @@ static cudaError_t launch_rows_t(const void* x, int64_t rows, int columns, int64
         return launch_pdl(dq_rows_kernel<HALF, 32>, dim3(blocks), dim3(DQR_THREADS), 0, stream, x, rows, columns,
                           row_stride, y, scale, zp);
     }
-    return launch_pdl(dq_rows_kernel<HALF, DQR_THREADS>, dim3(static_cast<unsigned>(rows)), dim3(DQR_THREADS), 0, stream,
-                      x, rows, columns, row_stride, y, scale, zp);
+    // Finding the row's range and scale costs a warp some 250 instructions whatever it holds: half the warps where 128
+    // threads hold the row.
+    const bool few = columns <= 2 * DQR_KEEP * 128 * DqRow<HALF>::E;
+    auto kern = few ? dq_rows_kernel<HALF, 128> : dq_rows_kernel<HALF, DQR_THREADS>;
+    return launch_pdl(kern, dim3(static_cast<unsigned>(rows)), dim3(few ? 128 : DQR_THREADS), 0, stream, x, rows, columns,
+                      row_stride, y, scale, zp);
 }
 
 cudaError_t launch_dynamic_quantize_rows(const void* x, bool half, int64_t rows, int columns, int64_t row_stride,
