@@ -5,7 +5,8 @@
 // one batch per CTA) in a grouped order so that concurrently running CTAs share A rows and B columns in L2. Warp 0
 // issues the TMA loads of a STAGES-deep ring of K blocks (BK = 128 bytes); warp 1 owns the TMEM allocation and
 // issues the MMAs (four K = 32 instructions per K block) into one of two accumulators; warps 2-9 drain the other
-// accumulator (tcgen05.ld; two warps per TMEM lane quadrant, each half of the columns), apply the zero-point
+// accumulator (tcgen05.ld; two warps per TMEM lane quadrant, each half of the columns; four, warps 2-17, each a quarter,
+// for the activated product), apply the zero-point
 // correction and the epilogue and store C (through one shared-memory box per warp and TMA stores) while the next
 // tile is being multiplied.
 //
@@ -57,7 +58,7 @@ constexpr int GROUP_M_TALL = 16;
 // each a quarter: its work per element (28 instructions, two of them exponentials or quotients at a quarter of the
 // rate) fits beside the MMAs of the next tile only with four warps to hide one another's latency on each scheduler. Their
 // boxes and the second set of column terms, filled while the accumulator is awaited, cost one stage of the operand ring.
-// 8192 x 8192 x 2048 into float32 with tanh GELU took 167 us with 8 warps and six stages, ACT_US with 16 and five.
+// 8192 x 8192 x 2048 into float32 with tanh GELU took 167 us with 8 warps and six stages, 134 us with 16 and five.
 template <int CG, bool ACT = false>
 struct Cfg {
     static constexpr int EPI_WARPS = ACT ? 16 : 8;
