@@ -821,7 +821,21 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
             const bool tail_item = tail_split && wi.tile >= p.dp_tiles;
             const int sk_slot = (worker + 1) * CG + static_cast<int>(rank);
             ColTerms& terms_smem = terms_all[ACT ? lt & 1 : 0];
+            const int m = tm * C::BM + static_cast<int>(rank) * 128 + q * 32 + lane;
+            const bool row_ok = m < p.m;
+            uint32_t za = 0, rt = 0;  // zero point of A for this row, and K * za - rowsumA
+            float row_scale = 0.0f;   // the scale of this row of A
+            auto row_terms = [&] {
+                if (row_ok && terms) {
+                    za = static_cast<uint32_t>(zp_value(e.za, e.za_vector, e.za_signed, m));
+                    const uint32_t rsa = e.row_sum_a ? row_sum_of(e, b, m) : 0u;
+                    rt = static_cast<uint32_t>(p.k) * za - rsa;
+                }
+            };
             if constexpr (ACT) {
+                // The row's terms and the columns' are on their way together.
+                row_terms();
+                if (row_ok) row_scale = row_scale_of(e, m);
                 // The terms this tile needs, before its accumulator is awaited: every warp has left the tile before last.
                 fill_col_terms(terms_smem, e, b, tn * tc::BN, threadIdx.x - 64, C::EPI_THREADS);
                 // This warp's part of the residual into L2 while the tile is multiplied, a row per lane.
@@ -893,21 +907,13 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                 fill_col_terms(terms_smem, e, b, tn * tc::BN, threadIdx.x - 64, C::EPI_THREADS);
                 asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_THREADS) : "memory");
             }
-            const int m = tm * C::BM + static_cast<int>(rank) * 128 + q * 32 + lane;
-            const bool row_ok = m < p.m;
-            uint32_t za = 0, rt = 0;  // zero point of A for this row, and K * za - rowsumA
-            if (row_ok && terms) {
-                za = static_cast<uint32_t>(zp_value(e.za, e.za_vector, e.za_signed, m));
-                const uint32_t rsa = e.row_sum_a ? row_sum_of(e, b, m) : 0u;
-                rt = static_cast<uint32_t>(p.k) * za - rsa;
-            }
+            if constexpr (!ACT) row_terms();
             if constexpr (ACT) {
                 using B = ActBox<OUT>;
                 const int box_row = tm * C::BM + static_cast<int>(rank) * 128 + q * 32;
                 const int64_t batch_at = b * e.batch_stride_c;
                 const bool int_terms = e.za != nullptr || e.zb != nullptr || e.int_bias != nullptr;
                 const bool res = e.residual != nullptr, res_ahead = res && p.residual_vec;
-                const float row_scale = row_ok ? row_scale_of(e, m) : 0.0f;  // the scale of this row of A
                 uint8_t* box = staging + ew * C::BOXES * C::BOX_BYTES;
                 const uint32_t box_s = smem_u32(box);
                 uint4 ahead[4];
@@ -916,8 +922,13 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                 for (int j0 = c_first * 32; j0 < c_end * 32; j0 += B::COLS) {  // a box at a time
                     const int n0 = tn * tc::BN + j0;
                     if (n0 >= p.n || box_row >= p.m) break;
-                    if (lane == 0) bulk_wait_group_read<0>();
-                    __syncwarp();  // the box is free
+                    // The box is free once the last store has read it: awaited when the first results are ready, or for the
+                    // residual.
+                    auto box_free = [&] {
+                        if (lane == 0) bulk_wait_group_read<0>();
+                        __syncwarp();
+                    };
+                    if (res) box_free();
                     if (res_ahead) {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
@@ -936,6 +947,7 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                         if (sk_in != nullptr) sk_add_16(sk_in, (j0 + g) / 32, ((j0 + g) / 16) & 1, row_in_cta, r);
                         float f[16];
                         activated_values(terms_smem, e, int_terms, za_per_row, za, rt, row_scale, j0 + g, r, f);
+                        if (g == 0 && !res) box_free();
 #pragma unroll
                         for (int u = 0; u < 16 / B::UNIT; u++) {
                             const uint32_t at = box_unit(box_s, lane, g / B::UNIT + u);
