@@ -62,18 +62,24 @@ __device__ __forceinline__ int32_t zp_value(const uint8_t* z, int vector, int is
 }
 
 // The byte sum of row m of A (batch b) and of column n of B: the partial sums of the K splits added up (wrapping).
-__device__ __forceinline__ uint32_t row_sum_of(const Epilogue& e, int b, int m) {
+// Four at a time: their loads are in flight together.
+__device__ __forceinline__ uint32_t split_sum(const int32_t* p, int splits, int64_t stride) {
     uint32_t s = 0;
-    for (int i = 0; i < e.sum_splits; i++)
-        s += static_cast<uint32_t>(__ldg(e.row_sum_a + i * e.row_sum_split_stride + b * e.row_sum_a_stride + m));
+    for (int i = 0; i < splits; i += 4) {
+        int32_t v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) v[u] = i + u < splits ? __ldg(p + (i + u) * stride) : 0;
+        s += static_cast<uint32_t>(v[0]) + static_cast<uint32_t>(v[1]) + static_cast<uint32_t>(v[2]) + static_cast<uint32_t>(v[3]);
+    }
     return s;
 }
 
+__device__ __forceinline__ uint32_t row_sum_of(const Epilogue& e, int b, int m) {
+    return split_sum(e.row_sum_a + b * e.row_sum_a_stride + m, e.sum_splits, e.row_sum_split_stride);
+}
+
 __device__ __forceinline__ uint32_t col_sum_of(const Epilogue& e, int b, int n) {
-    uint32_t s = 0;
-    for (int i = 0; i < e.sum_splits; i++)
-        s += static_cast<uint32_t>(__ldg(e.col_sum_b + i * e.col_sum_split_stride + b * e.col_sum_b_stride + n));
-    return s;
+    return split_sum(e.col_sum_b + b * e.col_sum_b_stride + n, e.sum_splits, e.col_sum_split_stride);
 }
 
 // The scale of column n: scale[n] (or the single scale), times the scale of A when one is given - one float32
