@@ -451,7 +451,8 @@ OG_API og_status og_int8_moe_last_kernel(og_int8_moe* moe, char* buffer, uint64_
  * [experts][model_size]; w_in int8 [experts][(gated ? 2 : 1) * expert_size][model_size] and w_out int8
  * [experts][model_size][expert_size], a float32 scale per row of each; expert_ids int32 and expert_weights float32,
  * [tokens][top_k] by falling p, receive the routing. residual, expert_ids and expert_weights may be NULL; y may be x,
- * and residual may be y or x (the same elements). */
+ * and residual may be y or x (the same elements). What one instance records shares its workspace and its barrier: it runs
+ * in one stream at a time (captured graphs of it too), like the other classes' recorded work. */
 OG_API og_status og_int8_moe_encode(og_int8_moe* moe, og_encoder* encoder, const og_moe_problem* problem,
                                     const og_buffer* x, const og_buffer* router, const og_buffer* w_in,
                                     const og_buffer* w_in_scale, const og_buffer* w_out, const og_buffer* w_out_scale,

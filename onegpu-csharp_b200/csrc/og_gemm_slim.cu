@@ -146,7 +146,8 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
     if (warp == 0) {
         for (int kb = kb0; kb < kb1; kb++) {
             const int it = kb - kb0, s = it % C::STAGES;
-            if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag)) break;
+            const bool ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;  // a warp gives up as one
             if (lane == 0) {
                 mbar_arrive_expect_tx(&full[s], C::B_BYTES + C::A_BYTES);
                 if constexpr (B_KMAJOR)
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
         bool ok = true;
         for (int kb = kb0; kb < kb1; kb++) {
             const int it = kb - kb0, s = it % C::STAGES;
-            ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
@@ -199,7 +200,8 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
             int32_t sum = 0;
             for (int kb = kb0; kb < kb1; kb++) {
                 const int it = kb - kb0, s = it % C::STAGES;
-                if (!mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag)) break;
+                const bool ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag);
+                if (!__all_sync(0xFFFFFFFFu, ok)) break;
                 const uint4* box = reinterpret_cast<const uint4*>(sX + s * C::A_BYTES + r * slim::BK);
 #pragma unroll
                 for (int i = 0; i < UNITS; i++) sum = byte_sum(box[(u0 + i) ^ (r & 7)], e.za_signed, sum);

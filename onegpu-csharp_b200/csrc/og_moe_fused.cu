@@ -781,9 +781,10 @@ struct MoeWarp {
             const int r = u / 9, j = u - 9 * r;
             const uintptr_t at = reinterpret_cast<uintptr_t>(w + weight_row(feed.phase, feed.e, feed.y, r) * ld + feed.x);
             const int8_t* src = reinterpret_cast<const int8_t*>((at & ~uintptr_t(15)) + 16 * j);
-            const bool ok = src < end;
+            const bool ok = src < end;  // else nothing is read; the address is one that is read elsewhere
+            const int8_t* from = ok ? src : reinterpret_cast<const int8_t*>(reinterpret_cast<uintptr_t>(w) & ~uintptr_t(15));
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(box + r * S::PITCH + 16 * j)),
-                         "l"(ok ? src : w), "r"(ok ? 16 : 0)
+                         "l"(from), "r"(ok ? 16 : 0)
                          : "memory");
         }
     }

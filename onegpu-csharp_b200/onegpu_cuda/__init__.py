@@ -301,9 +301,10 @@ class GpuBuffer:
 
     def ref(self) -> og_buffer:
         """The C view of the buffer, built once (building it anew for every argument of every call costs more than the
-        calls themselves) and again when the buffer has another address."""
-        if self._ref is None or self._ref[0] != self.ptr:
-            self._ref = (self.ptr, og_buffer(self.ptr, self.length, self.type))
+        calls themselves) and again when the buffer has another address, length or type."""
+        key = (self.ptr, self.length, self.type)
+        if self._ref is None or self._ref[0] != key:
+            self._ref = (key, og_buffer(*key))
         return self._ref[1]
 
     def write(self, data: np.ndarray, offset: int = 0) -> None:
@@ -607,12 +608,12 @@ class Int8Operand:
     is_vector: bool = False
 
     def c_struct(self) -> og_operand:
-        buffer = self.buffer
-        key = (buffer, buffer.ptr if buffer is not None else None, self.offset, 1 if self.is_vector else 0)
+        if self.buffer is None:
+            return og_operand(og_buffer(None, 0, 0), self.offset, 1 if self.is_vector else 0)
+        key = (self.buffer.ref(), self.offset, 1 if self.is_vector else 0)  # the same view: the same buffer as before
         known = self.__dict__.get("_known")
         if known is None or known[0] != key:  # built once for the same values
-            ref = buffer.ref() if buffer is not None else og_buffer(None, 0, 0)
-            known = self.__dict__["_known"] = (key, og_operand(ref, key[2], key[3]))
+            known = self.__dict__["_known"] = (key, og_operand(*key))
         return known[1]
 
 
