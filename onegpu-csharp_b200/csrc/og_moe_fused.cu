@@ -24,8 +24,8 @@
 // value for float16 layers (D = 3) and 31 bits for float32 ones (D = 4), float32's own precision for values down to 2^-7
 // of the largest. Measured against converting the weights to bfloat16 in registers and multiplying two or three bfloat16
 // pieces: 239 instructions per 2 KB of weights became about 100, 8 tokens through 2 of 8 experts (4096 x 8192) went from
-// 163 to 149 us (4.9 TB/s over the whole launch, 6 TB/s while the weights stream), 64 tokens through 6 of 64 experts
-// (2048 x 1408) from 199 to 164 us. The tensor cores' rate does not matter here (one token per expert uses an eighth of a
+// 163 to 149 us (6.1 TB/s while the weights stream), 64 tokens through 6 of 64 experts (2048 x 1408) from 199 to 164 us
+// (149 with shares of equal cost). The tensor cores' rate does not matter here (one token per expert uses an eighth of a
 // tile), and 128-row tcgen05 tiles would cut the work too coarsely for one token.
 // A token with an infinite or NaN value, or such a hidden value, gets NaN.
 #include <cuda.h>
