@@ -11,6 +11,9 @@ public struct MoeProblem
     public int OffsetX, OffsetRouter, OffsetIn, OffsetInScale, OffsetOut, OffsetOutScale, OffsetY;
     public int OffsetResidual, OffsetIds, OffsetWeights;
 
+    // Without it `new MoeProblem { .. }` would skip the initializers above.
+    public MoeProblem() { }
+
     public MoeProblem(int tokens, int modelSize, int expertSize, int experts, int topK)
     {
         Tokens = tokens;
