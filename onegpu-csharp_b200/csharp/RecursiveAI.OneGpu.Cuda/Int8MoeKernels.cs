@@ -1,4 +1,6 @@
 // The mixture-of-experts layer on int8 weights of the CUDA backend (og_int8_moe_*). No counterpart in the reference.
+using RecursiveAI.OneGpu.Kernels;
+
 namespace RecursiveAI.OneGpu.Cuda;
 
 /// <summary>A layer for up to 128 tokens, offsets in elements. Gated: hidden values are activation(first half) * second

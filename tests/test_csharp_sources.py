@@ -39,3 +39,20 @@ def test_structs_with_defaults_have_a_parameterless_constructor(path):
         assigned = [f for f in re.findall(r"\bpublic\s+[^;()=]*=(?!>)[^;]*;", block)]
         if assigned or constructors:
             assert any(not c.strip() for c in constructors), (m.group(1), assigned)
+
+
+def namespace_of(path):
+    return re.search(r"^namespace\s+([\w.]+);", code(path), re.M).group(1)
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=os.path.basename)
+def test_types_of_the_other_namespace_are_imported(path):
+    """A file names another namespace's types only with a using of it."""
+    own, text = namespace_of(path), code(path)
+    using = set(re.findall(r"^using\s+([\w.]+);", text, re.M))
+    for other in SOURCES:
+        space = namespace_of(other)
+        if space == own or own.startswith(space + "."):
+            continue
+        for name in re.findall(r"\b(?:struct|class|enum)\s+(\w+)", code(other)):
+            assert space in using or not re.search(r"(?<![\w.])%s\b" % name, text), (name, space)
