@@ -458,6 +458,11 @@ OG_API og_status og_int8_moe_encode(og_int8_moe* moe, og_encoder* encoder, const
                                     const og_buffer* w_in_scale, const og_buffer* w_out, const og_buffer* w_out_scale,
                                     const og_buffer* y, const og_buffer* residual, const og_buffer* expert_ids,
                                     const og_buffer* expert_weights);
+/* Watchdog self-test: the next layer this instance records runs with its waits at the grid barriers limited to limit_us
+ * (1 .. 500000), and one CTA comes to `barrier` (1 .. 4: after the router, the input products, the hidden values' exchange,
+ * the output products) three times that late. The launch ends by itself; the next og_device_wait_idle or readback reports
+ * OG_ERROR_COMMAND_FAILED (reason Watchdog), y and the routing are not defined, and the instance stays usable. */
+OG_API og_status og_int8_moe_watchdog_selftest(og_int8_moe* moe, int32_t barrier, uint32_t limit_us);
 /* Its argument checks alone (no device needed). */
 OG_API og_status og_int8_moe_check(const og_moe_problem* problem, const og_buffer* x, const og_buffer* router,
                                    const og_buffer* w_in, const og_buffer* w_in_scale, const og_buffer* w_out,

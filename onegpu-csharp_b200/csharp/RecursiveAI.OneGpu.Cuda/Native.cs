@@ -169,6 +169,7 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int og_int8_moe_create(nint device, nint* moe);
     [LibraryImport(Lib)] internal static partial int og_int8_moe_destroy(nint moe);
     [LibraryImport(Lib)] internal static partial int og_int8_moe_last_kernel(nint moe, byte* buffer, ulong capacity);
+    [LibraryImport(Lib)] internal static partial int og_int8_moe_watchdog_selftest(nint moe, int barrier, uint limitUs);
     [LibraryImport(Lib)] internal static partial int og_int8_moe_encode(nint moe, nint encoder, OgMoeProblem* p,
         OgBuffer* x, OgBuffer* router, OgBuffer* wIn, OgBuffer* wInScale, OgBuffer* wOut, OgBuffer* wOutScale, OgBuffer* y,
         OgBuffer* residual, OgBuffer* expertIds, OgBuffer* expertWeights);

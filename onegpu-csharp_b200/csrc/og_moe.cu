@@ -15,6 +15,7 @@
 #include "og_gemm.h"
 #include "og_host.h"
 #include "og_moe.h"
+#include "og_ptx.cuh"
 
 // ---- host layer ------------------------------------------------------------------------------------------------------
 
@@ -25,14 +26,16 @@ struct og_int8_moe {
     std::string last = "none";
     std::vector<void*> buffers;  // workspaces, the latest last; older ones live until destroy (recorded work names them)
     int64_t bytes = 0;
-    unsigned long long* arrivals = nullptr;  // the fused kernel's grid barrier
+    og::MoeCounts* counts = nullptr;  // of the fused kernel, followed by its tickets
+    int late_barrier = 0;             // watchdog self-test of the next layer recorded, 0 for none
+    uint64_t limit_ns = 0;
 };
 
 namespace {
 
 const char* kMoe = "Int8Moe";
-// The fused kernel's barrier count, then its tickets.
-constexpr size_t kBarrierBytes = sizeof(unsigned long long) + og::MOE_MAX_TOKENS / 8 * sizeof(unsigned int);
+// The fused kernel's counts, then its tickets.
+constexpr size_t kCountBytes = sizeof(og::MoeCounts) + og::MOE_MAX_TOKENS / 8 * sizeof(unsigned int);
 
 void require_float(const og_buffer* b, const char* arg) {
     if (b->type != OG_F32 && b->type != OG_F16)
@@ -160,13 +163,13 @@ OG_API og_status og_int8_moe_create(og_device* d, og_int8_moe** out) {
         if (out == nullptr) null_arg(kMoe, "out");
         use(d);
         void* p = nullptr;
-        check_cuda(cudaMalloc(&p, kBarrierBytes), "Int8Moe barrier");
-        const cudaError_t e = cudaMemset(p, 0, kBarrierBytes);
+        check_cuda(cudaMalloc(&p, kCountBytes), "Int8Moe counts");
+        const cudaError_t e = cudaMemset(p, 0, kCountBytes);
         if (e != cudaSuccess) cudaFree(p);
-        check_cuda(e, "Int8Moe barrier");
+        check_cuda(e, "Int8Moe counts");
         auto* m = new og_int8_moe();
         m->device = d;
-        m->arrivals = static_cast<unsigned long long*>(p);
+        m->counts = static_cast<og::MoeCounts*>(p);
         *out = m;
     });
 }
@@ -177,7 +180,7 @@ OG_API og_status og_int8_moe_destroy(og_int8_moe* m) {
         use(m->device);
         cudaStreamSynchronize(m->device->stream);
         for (void* p : m->buffers) cudaFree(p);
-        cudaFree(m->arrivals);
+        cudaFree(m->counts);
         delete m;
     });
 }
@@ -189,6 +192,19 @@ OG_API og_status og_int8_moe_last_kernel(og_int8_moe* m, char* buffer, uint64_t 
         const size_t n = std::min(static_cast<size_t>(capacity) - 1, m->last.size());
         m->last.copy(buffer, n);
         buffer[n] = 0;
+    });
+}
+
+OG_API og_status og_int8_moe_watchdog_selftest(og_int8_moe* m, int32_t barrier, uint32_t limit_us) {
+    return guard([&] {
+        if (m == nullptr) throw OgError{OG_ERROR_INVALID_HANDLE, kMoe, "moe", "null handle", "", "", ""};
+        if (barrier < 1 || barrier > 4)
+            throw OgError{OG_ERROR_ARGUMENT_RANGE, kMoe, "barrier", "the layer's barriers are 1 .. 4", "", "", ""};
+        if (limit_us < 1 || limit_us > 500000)
+            throw OgError{OG_ERROR_ARGUMENT_RANGE, kMoe, "limitMicroseconds",
+                          "the self-test wait limit is 1 .. 500000 microseconds", "", "", ""};
+        m->late_barrier = barrier;
+        m->limit_ns = uint64_t(limit_us) * 1000;
     });
 }
 
@@ -234,16 +250,20 @@ OG_API og_status og_int8_moe_encode(og_int8_moe* m, og_encoder* enc, const og_mo
         L.residual = residual != nullptr ? at<void>(residual, p->offset_residual) : nullptr;
         L.ids_out = ids != nullptr ? at<int32_t>(ids, p->offset_ids) : nullptr;
         L.weights_out = weights != nullptr ? at<float>(weights, p->offset_weights) : nullptr;
-        L.arrivals = m->arrivals;
-        L.tickets = reinterpret_cast<unsigned int*>(m->arrivals + 1);
+        L.counts = m->counts;
+        L.tickets = reinterpret_cast<unsigned int*>(m->counts + 1);
         L.error_flag = m->device->status;
         L.num_sms = m->device->sm_count;
+        L.wait_limit_ns = m->late_barrier != 0 ? m->limit_ns : og::OG_WAIT_LIMIT_NS;
+        L.late_barrier = m->late_barrier;
+        L.late_ns = 3 * L.wait_limit_ns;
         bind_workspace(m, L);
         cudaError_t err;
         auto fn = og::prepare_moe_fused(L, &err);  // tensor maps built now, at record time
         check_cuda(err, "Int8Moe tensor maps");
         m->last = og::moe_aligned(L) ? "fused" : "fused-unaligned";
         enc->ops.push_back(std::move(fn));
+        m->late_barrier = 0;
         enc->dispatches += 1;
     });
 }

@@ -13,6 +13,12 @@ constexpr int MOE_MAX_EXPERTS = 512;
 constexpr int MOE_MAX_TOP_K = 16;
 constexpr int MOE_MAX_SIZE = 65536;
 
+// What the CTAs of a launch count; all zero between launches.
+struct MoeCounts {
+    unsigned int arrivals;  // at the grid barriers
+    unsigned int exits;     // CTAs that are through with the counts
+};
+
 // One validated layer, pointers resolved (offsets applied). Rows of the weights are contiguous over the summed axis:
 // w_in [experts][up * expert_size][model_size] (up = 2 when gated: the gate's rows, then the other half's; else 1),
 // w_out [experts][model_size][expert_size], each row with its scale.
@@ -41,10 +47,13 @@ struct MoeLaunch {
     uint32_t* h_most;              // [tokens * top_k] and of a pair's hidden values
     float* outputs;                // [tokens * top_k][model], rows padded to 4: weighted outputs of the chosen experts
     long long* segments;           // partial sums of units cut between warps
-    unsigned long long* arrivals;  // grid barrier: arrivals of all launches so far
+    MoeCounts* counts;
     unsigned int* tickets;         // [MOE_MAX_TOKENS / 8] logits finished of each block of 8 tokens, 0 between launches
     int* error_flag;
     int num_sms;
+    uint64_t wait_limit_ns;  // of the waits at the grid barriers
+    int late_barrier;        // watchdog self-test: the barrier (1 .. 4) that one CTA comes late_ns late to, 0 for none
+    uint64_t late_ns;
 };
 
 // The workspace sizes of the fused kernel, in bytes.

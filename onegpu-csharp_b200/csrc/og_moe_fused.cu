@@ -209,37 +209,48 @@ __device__ __forceinline__ void load_rows(uint32_t (&a)[4], uint32_t addr) {
 
 // ---- grid barrier ---------------------------------------------------------------------------------------------------
 
-// Every CTA of the launch arrives; `wait` false only arrives (a CTA that has failed keeps the count whole for the
-// others and for later launches). Bounded; false when it gave up.
-__device__ __forceinline__ bool grid_arrive(unsigned long long* arrivals, bool wait) {
+// The counts start every launch at zero. A CTA that gives up leaves without arriving any further, so a barrier that is
+// passed has been reached by every CTA with its work done; the others' bounded waits at the next one run out too.
+
+// Arrives and waits, bounded, for `target` arrivals; false when it gave up.
+__device__ __forceinline__ bool grid_arrive(unsigned int* arrivals, unsigned int target, uint64_t limit_ns) {
     __threadfence();
-    const unsigned G = gridDim.x;
-    const unsigned long long before = atomicAdd(arrivals, 1ull);
-    if (!wait) return true;
-    const unsigned long long target = (before / G + 1ull) * G;
-    if (before + 1ull != target) {
+    if (atomicAdd(arrivals, 1u) + 1u != target) {
         const uint64_t t0 = global_timer_ns();
         while (true) {
-            unsigned long long now;
-            asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(arrivals) : "memory");
+            unsigned int now;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(arrivals) : "memory");
             if (now >= target) break;
-            if (global_timer_ns() - t0 > OG_WAIT_LIMIT_NS) return false;
+            if (global_timer_ns() - t0 > limit_ns) return false;
         }
     }
     __threadfence();
     return true;
 }
 
-// The whole CTA meets the grid; false (for every thread) when this CTA has failed or gives up here. Out of line: the
-// kernel runs each of its parts once or twice, so instructions that are fetched a second time are what it waits for.
-static __device__ __noinline__ bool grid_barrier(unsigned long long* arrivals, const int* abort, int* failed) {
+// The whole CTA meets the grid for the time `which` (1 .. 4); false (for every thread) when this CTA has failed or gives up
+// here. Out of line: the kernel runs each of its parts once or twice, so instructions that are fetched a second time are
+// what it waits for.
+static __device__ __noinline__ bool grid_barrier(unsigned int* arrivals, unsigned int which, uint64_t limit_ns,
+                                                 const int* abort, int* failed) {
     __syncthreads();
-    if (threadIdx.x == 0) {
-        const bool ok = *abort == 0;
-        if (!grid_arrive(arrivals, ok) || !ok) *failed = 1;
-    }
+    if (threadIdx.x == 0 && (*abort != 0 || !grid_arrive(arrivals, which * gridDim.x, limit_ns))) *failed = 1;
     __syncthreads();
     return *failed == 0;
+}
+
+// One thread of a CTA that is through with the counts. The last one of the launch clears them for the next launch, whatever
+// happened in this one.
+__device__ __forceinline__ unsigned int count_out(const MoeLaunch& L) {
+    __threadfence();
+    return atomicAdd(&L.counts->exits, 1u);
+}
+
+__device__ __forceinline__ void clear_counts(const MoeLaunch& L, unsigned int out_before) {
+    if (out_before != gridDim.x - 1) return;
+    __threadfence();
+    L.counts->arrivals = 0;
+    L.counts->exits = 0;
 }
 
 // The counts of finished logits, for the next launch; by CTA 0, once every CTA is past the first barrier.
@@ -247,12 +258,23 @@ __device__ __forceinline__ void clear_tickets(const MoeLaunch& L) {
     for (int i = 0; i < MOE_MAX_TOKENS / 8; i++) atomicExch(L.tickets + i, 0u);
 }
 
-// A CTA that gives up: the launch's failure is raised and the barriers it will not wait at still count it.
-__device__ __forceinline__ void leave_early(const MoeLaunch& L, int barriers_left) {
+// A CTA that gives up raises the launch's failure.
+__device__ __forceinline__ void leave_early(const MoeLaunch& L) {
     if (threadIdx.x != 0) return;
     if (blockIdx.x == 0) clear_tickets(L);
-    for (int i = 0; i < barriers_left; i++) grid_arrive(L.arrivals, false);
     atomicExch(L.error_flag, 1);
+    clear_counts(L, count_out(L));
+}
+
+// The watchdog self-test: the second CTA comes late to the barrier `which`, later than the others wait.
+static __device__ __noinline__ void come_late(uint64_t ns) {
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < ns) {
+    }
+}
+
+__device__ __forceinline__ void self_test(const MoeLaunch& L, int which) {
+    if (L.late_barrier == which && blockIdx.x == 1) come_late(L.late_ns);
 }
 
 // ---- phase 0 --------------------------------------------------------------------------------------------------------
@@ -1195,6 +1217,7 @@ __global__ void __launch_bounds__(S::THREADS, 1)
         }
     }
     pdl_wait();
+    self_test(L, 1);
     for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS) sh.most[i] = 0;
     if (p.vec)
         moe_digits_x<S, HALF, true>(p);
@@ -1212,9 +1235,11 @@ __global__ void __launch_bounds__(S::THREADS, 1)
             moe_choose_tokens<S, D>(L, sh, t0, min(8, L.tokens - t0), true);
         }
     }
-    // Four grid barriers; a CTA that leaves early still arrives at the ones it skips.
-    if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
-        leave_early(L, 3);
+    auto meet = [&](unsigned int which) {
+        return grid_barrier(&L.counts->arrivals, which, L.wait_limit_ns, &sh.abort, &sh.failed);
+    };
+    if (!meet(1)) {
+        leave_early(L);
         return;
     }
     if (L.tokens <= S::WARPS) {
@@ -1255,15 +1280,17 @@ __global__ void __launch_bounds__(S::THREADS, 1)
             for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS)
                 if (sh.most[i] != 0) atomicMax(L.h_most + i, sh.most[i]);
         }
-        if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
+        self_test(L, 2);
+        if (!meet(2)) {
             me.drain();
-            leave_early(L, 2);
+            leave_early(L);
             return;
         }
         moe_digits_h<S, D>(p);
-        if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
+        self_test(L, 3);
+        if (!meet(3)) {
             me.drain();
-            leave_early(L, 1);
+            leave_early(L);
             return;
         }
         for (int i = threadIdx.x; i < L.tokens * L.top_k; i += S::THREADS)
@@ -1271,10 +1298,12 @@ __global__ void __launch_bounds__(S::THREADS, 1)
         __syncthreads();
     }
     me.drain();
-    if (!grid_barrier(L.arrivals, &sh.abort, &sh.failed)) {
-        leave_early(L, 0);
+    self_test(L, 4);
+    if (!meet(4)) {
+        leave_early(L);
         return;
     }
+    const unsigned int out_before = threadIdx.x == 0 ? count_out(L) : 0;  // its answer comes while the sums are formed
     if (blockIdx.x == 0 && threadIdx.x == 0 && L.tokens > S::WARPS) clear_tickets(L);
     const int vectors = (L.model + 3) / 4, total = L.tokens * vectors;
     for (int i = blockIdx.x * S::THREADS + threadIdx.x; i < total; i += gridDim.x * S::THREADS) {
@@ -1302,6 +1331,7 @@ __global__ void __launch_bounds__(S::THREADS, 1)
             }
         }
     }
+    if (threadIdx.x == 0) clear_counts(L, out_before);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------

@@ -166,6 +166,7 @@ EXPORTS = {
     "og_int8_moe_create": [_P, _PP],
     "og_int8_moe_destroy": [_P],
     "og_int8_moe_last_kernel": [_P, ctypes.c_char_p, ctypes.c_uint64],
+    "og_int8_moe_watchdog_selftest": [_P, ctypes.c_int32, ctypes.c_uint32],
     "og_int8_moe_encode": [_P, _P, _P] + [_BUF] * 10,
     "og_int8_moe_check": [_P] + [_BUF] * 10,
     "og_conv_integer_create": [_P, _P, _PP],
@@ -1123,6 +1124,12 @@ class Int8MoeKernels:
         _check(_lib.og_int8_moe_encode(self.handle, encoder.handle if encoder else None, ctypes.byref(p), _buf(x),
                                        _buf(router), _buf(w_in), _buf(w_in_scale), _buf(w_out), _buf(w_out_scale),
                                        _buf(y), _buf(residual), _buf(expert_ids), _buf(expert_weights)))
+
+    def watchdog_selftest(self, barrier: int, limit_us: int) -> None:
+        """The next layer recorded runs with its grid barriers' waits limited to ``limit_us`` and one CTA late to
+        ``barrier`` (1 .. 4): the next wait_idle raises GpuCommandFailedException with reason "Watchdog" and the instance
+        stays usable."""
+        _check(_lib.og_int8_moe_watchdog_selftest(self.handle, barrier, limit_us))
 
     Encode = encode
 
