@@ -26,7 +26,7 @@ struct og_int8_moe {
     std::string last = "none";
     std::vector<void*> buffers;  // workspaces, the latest last; older ones live until destroy (recorded work names them)
     int64_t bytes = 0;
-    og::MoeCounts* counts = nullptr;  // of the fused kernel, followed by its tickets
+    og::MoeCounts* counts = nullptr;  // of the fused kernel
     int late_barrier = 0;             // watchdog self-test of the next layer recorded, 0 for none
     uint64_t limit_ns = 0;
 };
@@ -34,8 +34,6 @@ struct og_int8_moe {
 namespace {
 
 const char* kMoe = "Int8Moe";
-// The fused kernel's counts, then its tickets.
-constexpr size_t kCountBytes = sizeof(og::MoeCounts) + og::MOE_MAX_TOKENS / 8 * sizeof(unsigned int);
 
 void require_float(const og_buffer* b, const char* arg) {
     if (b->type != OG_F32 && b->type != OG_F16)
@@ -163,8 +161,8 @@ OG_API og_status og_int8_moe_create(og_device* d, og_int8_moe** out) {
         if (out == nullptr) null_arg(kMoe, "out");
         use(d);
         void* p = nullptr;
-        check_cuda(cudaMalloc(&p, kCountBytes), "Int8Moe counts");
-        const cudaError_t e = cudaMemset(p, 0, kCountBytes);
+        check_cuda(cudaMalloc(&p, sizeof(og::MoeCounts)), "Int8Moe counts");
+        const cudaError_t e = cudaMemset(p, 0, sizeof(og::MoeCounts));
         if (e != cudaSuccess) cudaFree(p);
         check_cuda(e, "Int8Moe counts");
         auto* m = new og_int8_moe();
@@ -251,7 +249,6 @@ OG_API og_status og_int8_moe_encode(og_int8_moe* m, og_encoder* enc, const og_mo
         L.ids_out = ids != nullptr ? at<int32_t>(ids, p->offset_ids) : nullptr;
         L.weights_out = weights != nullptr ? at<float>(weights, p->offset_weights) : nullptr;
         L.counts = m->counts;
-        L.tickets = reinterpret_cast<unsigned int*>(m->counts + 1);
         L.error_flag = m->device->status;
         L.num_sms = m->device->sm_count;
         L.wait_limit_ns = m->late_barrier != 0 ? m->limit_ns : og::OG_WAIT_LIMIT_NS;

@@ -17,6 +17,7 @@ constexpr int MOE_MAX_SIZE = 65536;
 struct MoeCounts {
     unsigned int arrivals;  // at the grid barriers
     unsigned int exits;     // CTAs that are through with the counts
+    unsigned int tickets[MOE_MAX_TOKENS / 8];  // logits finished of each block of 8 tokens
 };
 
 // One validated layer, pointers resolved (offsets applied). Rows of the weights are contiguous over the summed axis:
@@ -48,7 +49,6 @@ struct MoeLaunch {
     float* outputs;                // [tokens * top_k][model], rows padded to 4: weighted outputs of the chosen experts
     long long* segments;           // partial sums of units cut between warps
     MoeCounts* counts;
-    unsigned int* tickets;         // [MOE_MAX_TOKENS / 8] logits finished of each block of 8 tokens, 0 between launches
     int* error_flag;
     int num_sms;
     uint64_t wait_limit_ns;  // of the waits at the grid barriers

@@ -239,30 +239,21 @@ static __device__ __noinline__ bool grid_barrier(unsigned int* arrivals, unsigne
     return *failed == 0;
 }
 
-// One thread of a CTA that is through with the counts. The last one of the launch clears them for the next launch, whatever
-// happened in this one.
-__device__ __forceinline__ unsigned int count_out(const MoeLaunch& L) {
-    __threadfence();
-    return atomicAdd(&L.counts->exits, 1u);
-}
+// One thread of a CTA that is through with the counts (its last use of them, an acquiring load or fenced, comes before).
+// The last one of the launch clears them for the next launch, whatever happened in this one.
+__device__ __forceinline__ unsigned int count_out(const MoeLaunch& L) { return atomicAdd(&L.counts->exits, 1u); }
 
 __device__ __forceinline__ void clear_counts(const MoeLaunch& L, unsigned int out_before) {
     if (out_before != gridDim.x - 1) return;
     __threadfence();
-    L.counts->arrivals = 0;
-    L.counts->exits = 0;
-}
-
-// The counts of finished logits, for the next launch; by CTA 0, once every CTA is past the first barrier.
-__device__ __forceinline__ void clear_tickets(const MoeLaunch& L) {
-    for (int i = 0; i < MOE_MAX_TOKENS / 8; i++) atomicExch(L.tickets + i, 0u);
+    *L.counts = MoeCounts{};
 }
 
 // A CTA that gives up raises the launch's failure.
 __device__ __forceinline__ void leave_early(const MoeLaunch& L) {
     if (threadIdx.x != 0) return;
-    if (blockIdx.x == 0) clear_tickets(L);
     atomicExch(L.error_flag, 1);
+    __threadfence();
     clear_counts(L, count_out(L));
 }
 
@@ -439,7 +430,7 @@ __device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>
             __syncwarp();
             if (lane == 0) {
                 __threadfence();
-                if (atomicAdd(L.tickets + t0 / 8, 1u) == static_cast<unsigned>(L.experts) - 1) atomicOr(&sh.complete, 1u << (t0 / 8));
+                if (atomicAdd(&L.counts->tickets[t0 / 8], 1u) == static_cast<unsigned>(L.experts) - 1) atomicOr(&sh.complete, 1u << (t0 / 8));
             }
         }
     }
@@ -1304,7 +1295,6 @@ __global__ void __launch_bounds__(S::THREADS, 1)
         return;
     }
     const unsigned int out_before = threadIdx.x == 0 ? count_out(L) : 0;  // its answer comes while the sums are formed
-    if (blockIdx.x == 0 && threadIdx.x == 0 && L.tokens > S::WARPS) clear_tickets(L);
     const int vectors = (L.model + 3) / 4, total = L.tokens * vectors;
     for (int i = blockIdx.x * S::THREADS + threadIdx.x; i < total; i += gridDim.x * S::THREADS) {
         const int t = i / vectors, d = (i - t * vectors) * 4;

@@ -42,6 +42,16 @@ def test_a_late_cta_fails_the_launch_and_the_instance_stays_usable(device, barri
             late_then_right(device, moe, size, barrier, half=half)
 
 
+@pytest.mark.parametrize("barrier", [1, 2, 3, 4])
+def test_blocks_of_tokens_ranked_by_one_cta_start_anew(device, barrier):
+    """More than 8 tokens: the CTA that completes a block's logits ranks it, so what a late CTA still counts after others
+    have left must not be found by the next launch."""
+    with og.Int8MoeKernels(device) as moe:
+        for size, half in [((16, 256, 128, 64, 8), True), ((30, 160, 96, 8, 2), False), ((100, 96, 272, 4, 3), True),
+                           ((128, 160, 48, 512, 16), True)]:
+            late_then_right(device, moe, size, barrier, half=half)
+
+
 def test_self_test_arguments(device):
     with og.Int8MoeKernels(device) as moe:
         for barrier, limit in [(0, 1000), (5, 1000), (1, 0), (1, 500001)]:
