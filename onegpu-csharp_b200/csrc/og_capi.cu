@@ -90,6 +90,16 @@ void put_string(char* buf, uint64_t cap, const std::string& s) {
     copy_field(buf, static_cast<size_t>(cap), s);
 }
 
+void* device_zeros(size_t bytes, const char* what) {
+    void* p = nullptr;
+    check_cuda(cudaMalloc(&p, bytes), what);
+    cudaError_t e = cudaMemset(p, 0, bytes);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+    if (e != cudaSuccess) cudaFree(p);
+    check_cuda(e, what);
+    return p;
+}
+
 void use(og_device* d) { check_cuda(cudaSetDevice(d->ordinal), "cudaSetDevice"); }
 
 const char* type_name(int32_t t) {
@@ -669,12 +679,10 @@ void record_gemm(og_int8_gemm* g, og_encoder* enc, og::GemmLaunch L, const og_op
             const int64_t part = og::rows_part_ints(L, workers), tickets = og::rows_tickets(L);
             if (g->rows_part_ints < part || g->rows_ticket_count < tickets) {
                 void* pp = nullptr;
-                void* tp = nullptr;
                 check_cuda(cudaMalloc(&pp, static_cast<size_t>(part) * sizeof(int32_t)), "Int8Gemm split partials");
                 g->rows_bufs.push_back(pp);
-                check_cuda(cudaMalloc(&tp, static_cast<size_t>(tickets) * sizeof(unsigned int)), "Int8Gemm tickets");
+                void* tp = device_zeros(static_cast<size_t>(tickets) * sizeof(unsigned int), "Int8Gemm tickets");
                 g->rows_bufs.push_back(tp);
-                check_cuda(cudaMemset(tp, 0, static_cast<size_t>(tickets) * sizeof(unsigned int)), "Int8Gemm tickets");
                 g->rows_part = static_cast<int32_t*>(pp);
                 g->rows_ticket = static_cast<unsigned int*>(tp);
                 g->rows_part_ints = part;
@@ -732,8 +740,7 @@ void record_gemm(og_int8_gemm* g, og_encoder* enc, og::GemmLaunch L, const og_op
         // they share it.
         if (g->sk_buf == nullptr) {
             const int64_t bytes = og::sk_bytes_needed(L.num_sms);
-            check_cuda(cudaMalloc(&g->sk_buf, static_cast<size_t>(bytes)), "Int8Gemm stream-K buffer");
-            check_cuda(cudaMemset(g->sk_buf, 0, static_cast<size_t>(bytes)), "Int8Gemm stream-K buffer");
+            g->sk_buf = device_zeros(static_cast<size_t>(bytes), "Int8Gemm stream-K buffer");
             g->sk_bytes = bytes;
         }
         og::sk_bind(L, g->sk_buf, g->sk_bytes);
@@ -798,8 +805,7 @@ OG_API og_status og_device_create(int32_t ordinal, og_device** out) {
             check_cuda(cudaStreamCreateWithFlags(&d->stream, cudaStreamNonBlocking), "cudaStreamCreate");
             check_cuda(cudaStreamCreateWithFlags(&d->upload, cudaStreamNonBlocking), "cudaStreamCreate");
             check_cuda(cudaStreamCreateWithFlags(&d->readback, cudaStreamNonBlocking), "cudaStreamCreate");
-            check_cuda(cudaMalloc(&d->status, sizeof(int)), "cudaMalloc");
-            check_cuda(cudaMemset(d->status, 0, sizeof(int)), "cudaMemset");
+            d->status = static_cast<int*>(device_zeros(sizeof(int), "status word"));
             check_cuda(cudaMallocHost(&d->status_host, sizeof(int)), "cudaMallocHost");
             check_cuda(cudaMallocHost(&d->readback_words, kReadbackWords * sizeof(int)), "cudaMallocHost");
             d->readback_free.reserve(kReadbackWords);
@@ -1419,15 +1425,9 @@ OG_API og_status og_dynamic_quantize_create(og_device* d, og_dynamic_quantize** 
         if (d == nullptr) null_arg(kDq, "device");
         if (out == nullptr) null_arg(kDq, "out");
         use(d);
+        void* p = device_zeros(og::dq_scratch_bytes(), "dynamic quantize ranges");
         auto* q = new og_dynamic_quantize();
         q->device = d;
-        void* p = nullptr;
-        cudaError_t e = cudaMalloc(&p, og::dq_scratch_bytes());
-        if (e != cudaSuccess) {
-            delete q;
-            check_cuda(e, "dynamic quantize ranges");
-        }
-        check_cuda(cudaMemset(p, 0, og::dq_scratch_bytes()), "dynamic quantize ranges");
         q->scratch = static_cast<og::DqScratch*>(p);
         *out = q;
     });

@@ -61,6 +61,9 @@ void set_last(const OgError& e);
 // cudaErrorMemoryAllocation -> OG_ERROR_OUT_OF_MEMORY, sticky errors -> OG_ERROR_DEVICE_LOST, others OG_ERROR_CUDA.
 void check_cuda(cudaError_t e, const char* what);
 void use(og_device* d);
+// Device memory of zeros, there for every stream when this returns: cudaMemset works in the legacy stream, which the
+// devices' own streams do not wait for.
+void* device_zeros(size_t bytes, const char* what);
 const char* type_name(int32_t t);
 int elem_size(int32_t t);
 

@@ -160,11 +160,7 @@ OG_API og_status og_int8_moe_create(og_device* d, og_int8_moe** out) {
         if (d == nullptr) null_arg(kMoe, "device");
         if (out == nullptr) null_arg(kMoe, "out");
         use(d);
-        void* p = nullptr;
-        check_cuda(cudaMalloc(&p, sizeof(og::MoeCounts)), "Int8Moe counts");
-        const cudaError_t e = cudaMemset(p, 0, sizeof(og::MoeCounts));
-        if (e != cudaSuccess) cudaFree(p);
-        check_cuda(e, "Int8Moe counts");
+        void* p = device_zeros(sizeof(og::MoeCounts), "Int8Moe counts");
         auto* m = new og_int8_moe();
         m->device = d;
         m->counts = static_cast<og::MoeCounts*>(p);
