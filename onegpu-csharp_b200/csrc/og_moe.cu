@@ -142,7 +142,7 @@ void bind_workspace(og_int8_moe* m, og::MoeLaunch& L) {
     L.ids = reinterpret_cast<int32_t*>(base + ids);
     L.weights = reinterpret_cast<float*>(base + weights);
     L.hidden = reinterpret_cast<float*>(base + hidden);
-    L.logits = reinterpret_cast<float*>(base + logits);
+    L.logits = reinterpret_cast<double*>(base + logits);
     L.x_digits = base + x;
     L.h_digits = base + h;
     L.x_most = reinterpret_cast<uint32_t*>(base + x_most);

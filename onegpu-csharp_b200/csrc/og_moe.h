@@ -41,7 +41,7 @@ struct MoeLaunch {
     int32_t* ids;                  // [tokens][top_k]
     float* weights;                // [tokens][top_k]
     float* hidden;                 // [tokens * top_k][expert], rows padded to 4
-    float* logits;                 // [tokens][experts]
+    double* logits;                // [tokens][experts]
     uint8_t* x_digits;             // [tokens][chunks of model][digits][128] of x
     uint8_t* h_digits;             // [tokens * top_k][chunks of expert][digits][128] of the hidden values
     uint32_t* x_most;              // [tokens] the bits of a token's largest magnitude

@@ -355,11 +355,12 @@ __device__ __forceinline__ void moe_digits_h(const MoeFusedParams& p) {
 }
 
 // Logits: units of one expert and 8 tokens, each shared by router_split warps of a CTA (so that a few units still occupy
-// the SMs). Eight products at a time in float32, the rest in float64, so that near-equal logits rank as their exact
-// values do.
+// the SMs). Held in float64 from the products (exact there) to the ranking and the softmax: an error of float32's size in a
+// large logit would be one of that size, not of its last bit, in a weight.
 template <class S, bool HALF, bool VEC, bool ROUTER_HALF>
 __device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>& sh) {
     const MoeLaunch& L = p.L;
+    constexpr int TOKENS = S::MT == 1 ? 2 : 8;  // a unit has no more
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = p.router_split, per_cta = S::WARPS / split, part = warp % split;
     const int token_blocks = (L.tokens + 7) / 8, units = L.experts * token_blocks;
@@ -379,29 +380,27 @@ __device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>
             // Past the tokens or the share, the last one again (its sums are dropped): every load of a step is in flight
             // at once.
             for (int v = v0 + lane; v < v1; v += 64) {
-                float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                float4 r[2], x[2][8];
+                float4 r[2], x[2][TOKENS];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int d = 4 * min(v + 32 * u, v1 - 1);
                     r[u] = moe_load4<ROUTER_HALF, VEC>(L.router, r0, d, L.model);
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
+                    for (int i = 0; i < TOKENS; i++)
                         x[u][i] = moe_load4<HALF, VEC>(L.x, x0 + static_cast<int64_t>(min(i, n - 1)) * L.model, d, L.model);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     if (u == 1 && v + 32 >= v1) break;
+                    const double rx = r[u].x, ry = r[u].y, rz = r[u].z, rw = r[u].w;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        f[i] = fmaf(x[u][i].x, r[u].x, f[i]);
-                        f[i] = fmaf(x[u][i].y, r[u].y, f[i]);
-                        f[i] = fmaf(x[u][i].z, r[u].z, f[i]);
-                        f[i] = fmaf(x[u][i].w, r[u].w, f[i]);
+                    for (int i = 0; i < TOKENS; i++) {
+                        sum[i] = fma(static_cast<double>(x[u][i].x), rx, sum[i]);
+                        sum[i] = fma(static_cast<double>(x[u][i].y), ry, sum[i]);
+                        sum[i] = fma(static_cast<double>(x[u][i].z), rz, sum[i]);
+                        sum[i] = fma(static_cast<double>(x[u][i].w), rw, sum[i]);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 8; i++) sum[i] += f[i];
             }
         }
         // Lane bits 4, 3 and 2 choose the token: 4 + 2 + 1 exchanges, then two more within each token's four lanes.
@@ -424,7 +423,7 @@ __device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>
         if (part == 0 && lane < n) {
             double total = 0.0;
             for (int w = 0; w < split; w++) total += sh.logit_part[buffer][warp + w][lane];
-            L.logits[static_cast<int64_t>(t0 + lane) * L.experts + e] = static_cast<float>(total);
+            L.logits[static_cast<int64_t>(t0 + lane) * L.experts + e] = total;
         }
         if (L.tokens > S::WARPS && part == 0 && n > 0) {
             __syncwarp();
@@ -438,63 +437,78 @@ __device__ __forceinline__ void moe_logits(const MoeFusedParams& p, MoeShared<S>
 
 // ---- routing --------------------------------------------------------------------------------------------------------
 
-// A key that orders floats as unsigned numbers; NaN below every number, with -infinity (what it ranks as).
-__device__ __forceinline__ uint32_t rank_key(float v) {
-    const uint32_t u = __float_as_uint(isnan(v) ? -INFINITY : (v == 0.0f ? 0.0f : v));
-    return u & 0x80000000u ? ~u : u | 0x80000000u;  // -infinity is 0x007FFFFF: 0 marks a taken expert
+// A key that orders numbers as unsigned ones; NaN below every number, with -infinity (what it ranks as).
+__device__ __forceinline__ uint64_t rank_key(double v) {
+    const uint64_t u = __double_as_longlong(isnan(v) ? -INFINITY : (v == 0.0 ? 0.0 : v));
+    return u >> 63 ? ~u : u | uint64_t(1) << 63;  // -infinity is 0x000FFFFFFFFFFFFF: 0 marks a taken expert
+}
+
+__device__ __forceinline__ double rank_value(uint64_t key) {
+    return __longlong_as_double(key >> 63 ? key & ~(uint64_t(1) << 63) : ~key);
+}
+
+// The largest key of a warp.
+__device__ __forceinline__ uint64_t warp_max(uint64_t key) {
+    const uint32_t high = __reduce_max_sync(0xFFFFFFFFu, static_cast<uint32_t>(key >> 32));
+    const uint32_t low = __reduce_max_sync(0xFFFFFFFFu, static_cast<uint32_t>(key >> 32) == high ? static_cast<uint32_t>(key) : 0u);
+    return static_cast<uint64_t>(high) << 32 | low;
+}
+
+// exp(d) for d <= 0 (or NaN) in float32, with what d's rounding to float32 drops.
+__device__ __forceinline__ float exp_of(double d) {
+    const float high = static_cast<float>(d);
+    if (high < -150.0f) return 0.0f;  // below half the smallest float32
+    const float e = expf(high);
+    return fmaf(e, static_cast<float>(d - high), e);
 }
 
 // A token's experts by one warp: the largest key, the lowest expert among equals, top_k times. PER_LANE logits per lane.
 template <class S, int D, int PER_LANE>
-__device__ __forceinline__ void moe_choose(const MoeLaunch& L, MoeShared<S>& sh, int t, float (&v)[PER_LANE], uint32_t x_most,
-                                           bool publish) {
+__device__ __forceinline__ void moe_choose(const MoeLaunch& L, MoeShared<S>& sh, int t, const double (&v)[PER_LANE],
+                                           uint32_t x_most, bool publish) {
     const int lane = threadIdx.x & 31;
-    uint32_t key[PER_LANE];
-    float top = -INFINITY;
+    uint64_t key[PER_LANE], best = 0;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < PER_LANE; i++) {
-        key[i] = lane + 32 * i < L.experts ? rank_key(v[i]) : 0u;
-        nan |= isnan(v[i]);
-        top = fmaxf(top, v[i]);
+        key[i] = lane + 32 * i < L.experts ? rank_key(v[i]) : 0;
+        nan |= lane + 32 * i < L.experts && isnan(v[i]);
+        best = max(best, key[i]);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    double top = rank_value(warp_max(best));
     if (__any_sync(0xFFFFFFFFu, nan)) top = NAN;  // the softmax of a row with a NaN is NaN
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER_LANE; i++) {
-        v[i] = lane + 32 * i < L.experts ? expf(v[i] - top) : 0.0f;
-        sum += v[i];
-    }
+    for (int i = 0; i < PER_LANE; i++)
+        if (lane + 32 * i < L.experts) sum += exp_of(rank_value(key[i]) - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    float weight = 0.0f, chosen = 0.0f;
+    uint64_t picked = 0;  // lane k: the k-th expert's key and index
     int id = 0;
 #pragma unroll 1
     for (int k = 0; k < L.top_k; k++) {
-        uint32_t best = 0;
-        float share = 0.0f;
+        uint64_t own = 0;
         int at = MOE_MAX_EXPERTS;
 #pragma unroll
         for (int i = 0; i < PER_LANE; i++)
-            if (key[i] > best) {
-                best = key[i];
+            if (key[i] > own) {
+                own = key[i];
                 at = lane + 32 * i;
-                share = v[i];
             }
-        const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, best);
-        const int chosen_at = __reduce_min_sync(0xFFFFFFFFu, best == most ? at : MOE_MAX_EXPERTS);
-        share = __shfl_sync(0xFFFFFFFFu, share, chosen_at & 31);
-        chosen += share;
+        const uint64_t most = warp_max(own);
+        const int chosen_at = __reduce_min_sync(0xFFFFFFFFu, own == most ? at : MOE_MAX_EXPERTS);
         if (lane == k) {
-            weight = share;
+            picked = most;
             id = chosen_at;
         }
 #pragma unroll
         for (int i = 0; i < PER_LANE; i++)
             if (chosen_at == lane + 32 * i) key[i] = 0;
     }
+    float weight = lane < L.top_k ? exp_of(rank_value(picked) - top) : 0.0f;
+    float chosen = weight;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) chosen += __shfl_xor_sync(0xFFFFFFFFu, chosen, o);
     if (lane < L.top_k) {
         weight = weight / (L.normalize ? chosen : sum);
         const int i = t * L.top_k + lane;
@@ -516,11 +530,10 @@ __device__ __forceinline__ void moe_choose_some(const MoeLaunch& L, MoeShared<S>
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int t = first + warp; t < first + count; t += S::WARPS) {
-        float v[PER_LANE];
+        double v[PER_LANE];
 #pragma unroll
         for (int i = 0; i < PER_LANE; i++)
-            v[i] = lane + 32 * i < L.experts ? __ldcg(L.logits + static_cast<int64_t>(t) * L.experts + lane + 32 * i)
-                                             : -INFINITY;
+            v[i] = lane + 32 * i < L.experts ? __ldcg(L.logits + static_cast<int64_t>(t) * L.experts + lane + 32 * i) : 0.0;
         moe_choose<S, D, PER_LANE>(L, sh, t, v, L.tokens > S::WARPS ? 0u : __ldcg(L.x_most + t), publish);
     }
 }
@@ -1351,7 +1364,7 @@ static int round4(int v) { return (v + 3) & ~3; }
 MoeFusedSizes moe_fused_sizes(const MoeLaunch& L) {
     const int64_t pairs = int64_t(L.tokens) * L.top_k;
     MoeFusedSizes s;
-    s.logits = int64_t(L.tokens) * L.experts * 4;
+    s.logits = int64_t(L.tokens) * L.experts * 8;
     const int digits = L.x_half ? 3 : 4;
     s.x_digits = int64_t(L.tokens) * chunks_of(L.model) * digits * moe::CHUNK;
     s.h_digits = pairs * chunks_of(L.expert) * digits * moe::CHUNK;
