@@ -418,7 +418,7 @@ OG_API og_status og_dequantize_check_quantize(const og_buffer* x, int32_t offset
                                               int32_t offset_output);
 
 /* ---- Int8MoeKernels: a mixture-of-experts layer on int8 weights (no counterpart in the reference) ------------------
- * For a few tokens (a decode step), float activations that are not quantized:
+ * For a few tokens (a decode step), float32 or float16 activations:
  *   logits[t][e] = sum_d x[t][d] router[e][d];  p = softmax of a token's logits over the experts
  *   a token's top_k experts by p (equal ones: the lowest index first; a NaN logit ranks below every number);
  *   w = p, or p / (the sum of the chosen p) when `normalize` is set
@@ -426,9 +426,9 @@ OG_API og_status og_dequantize_check_quantize(const og_buffer* x, int32_t offset
  *   h[j] = activation(u[j]) * u[expert_size + j] when `gated` is set (w_in holds the activated half's expert_size rows,
  *          then the other half's), activation(u[j]) otherwise
  *   y[t][d] = residual[t][d] + sum over the chosen experts of w w_out_scale[e][d] sum_j w_out[e][d][j] h[j]
- * The sums are exact or held in float32 and more: x and the hidden values are multiplied in fixed point with a scale per
- * token, 23 bits below the row's largest value for float16 and 31 for float32; a token with an infinite or NaN value, or
- * such a hidden value, gets NaN. */
+ * The logits are held in float64. x and the hidden values are rounded to fixed point, 31 bits below the largest value of
+ * their row (token) for float16 layers and 39 for float32 ones, and their products with the weights summed as integers; the
+ * rest is float32. A token with an infinite or NaN value, or such a hidden value, gets NaN. */
 
 /* tokens 0 .. 128; model_size and expert_size 1 .. 65536; experts 1 .. 512; top_k 1 .. min(experts, 16); activation an
  * og_activation; gated and normalize 0 or 1; offsets in elements. */

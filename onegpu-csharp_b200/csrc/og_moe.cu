@@ -5,7 +5,7 @@
 //   u = scale_in[e][j] sum_d w_in[e][j][d] x[t][d];   h[j] = activation(u[j]) u[F + j]  (gated), activation(u[j])
 //   y[t][d] = residual[t][d] + sum over the chosen e of w_e scale_out[e][d] sum_j w_out[e][d][j] h[j]
 //
-// Everything is accumulated in float32; the activations are not quantized. A NaN logit ranks below every number.
+// How the sums are held: og_moe_fused.cu. A NaN logit ranks below every number.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -20,13 +20,18 @@
 // Arithmetic: the int8 weights multiply as they are (mma.sync m16n8k32 s8, weights as the 16-row operand, 8 pairs as its
 // columns). The other operand is a row of x or of hidden values in fixed point, q = rint(v 2^s) with the row's own s, cut
 // into D balanced base-256 digits that are int8 operands too: every digit's sum is an exact int32 (65536 x 128 x 128 stays
-// below 2^31) and the digits' sums together an exact int64, whatever the order. Held are 23 bits below the row's largest
-// value for float16 layers (D = 3) and 31 bits for float32 ones (D = 4), float32's own precision for values down to 2^-7
-// of the largest. Measured against converting the weights to bfloat16 in registers and multiplying two or three bfloat16
-// pieces: 239 instructions per 2 KB of weights became about 100, 8 tokens through 2 of 8 experts (4096 x 8192) went from
-// 163 to 149 us (6.1 TB/s while the weights stream), 64 tokens through 6 of 64 experts (2048 x 1408) from 199 to 164 us
-// (149 with shares of equal cost). The tensor cores' rate does not matter here (one token per expert uses an eighth of a
-// tile), and 128-row tcgen05 tiles would cut the work too coarsely for one token.
+// below 2^31). The lowest digit's sum over a chunk is rounded to the next digit's unit and added there, so that it needs no
+// accumulators of its own: an error of a fraction of what rounding the values themselves costs, and the same one in
+// whatever order the chunks come. The other digits' sums together are an exact int64. Held are 31 bits below the row's
+// largest value for float16 layers (D = 4) and 39 bits for float32 ones (D = 5): the step has to be small next to the quiet
+// channels of a row, not to its largest value, since an output's weights may leave the loud ones out. With a digit less (23
+// and 31 bits) such outputs were off by up to 15 roundings of float16 for channels 3000 to 60000 times the others; 64 tokens
+// through 6 of 64 experts (2048 x 1408) took 152 us then and 156 now, one token (2048 x 1024) 35.5 and 36.5.
+// Measured against converting the weights to bfloat16 in registers and multiplying two or three bfloat16 pieces, with three
+// digits: 239 instructions per 2 KB of weights became about 100, 8 tokens through 2 of 8 experts (4096 x 8192) went from
+// 163 to 149 us (6.1 TB/s while the weights stream), 64 tokens through 6 of 64 experts from 199 to 164 us. The tensor
+// cores' rate does not matter here (one token per expert uses an eighth of a tile), and 128-row tcgen05 tiles would cut the
+// work too coarsely for one token.
 // A token with an infinite or NaN value, or such a hidden value, gets NaN.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -35,6 +40,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "og_act.cuh"
 #include "og_gemm.h"
@@ -88,13 +94,15 @@ struct MoeGroup {
 };
 
 // What a unit of a group costs next to others: its columns' digits come from L1 or L2 and cost more the more of them
-// differ, and each further tile has its own loads and products. Shares of equal bytes took, in us a phase: 64 tokens through
-// 6 of 64 experts (2048 x 1408) 66 with up to 6 pairs, 71 with 7 or 8, 89 with 9 to 12 (a second tile); 8 tokens through 2
-// of 8 experts (4096 x 8192) 80 (phase 1) and 39 (2) with one pair, 88 and 48 with 2 to 4; NT = 4, two, three and four
-// tiles 50, 68 and 86.
+// differ, and each further tile has its own loads and products. Shares of equal bytes took, in us a phase and with three
+// digits: 64 tokens through 6 of 64 experts (2048 x 1408) 66 with up to 6 pairs, 71 with 7 or 8, 89 with 9 to 12 (a second
+// tile); 8 tokens through 2 of 8 experts (4096 x 8192) 80 (phase 1) and 39 (2) with one pair, 88 and 48 with 2 to 4; NT = 4,
+// two, three and four tiles 50, 68 and 86. With four digits the second tile of NT = 2 weighs more: the 64 tokens took 178,
+// 168, 162 and 156 us with 5, 8, 11 and 14 for it, float32 ones 177, 173, 172 and 174. Read off float16 and float32 layers
+// with aligned weights; the unaligned load path shares by the same numbers.
 template <int NT>
 __device__ __forceinline__ int unit_cost(int pairs) {
-    return (pairs == 1 ? 16 : pairs <= 6 ? 18 : 20) + (pairs - 1) / 8 * (NT == 4 ? 12 : 5);
+    return (pairs == 1 ? 16 : pairs <= 6 ? 18 : 20) + (pairs - 1) / 8 * (NT == 4 ? 12 : 14);
 }
 
 template <class S>
@@ -125,6 +133,9 @@ constexpr size_t moe_smem_bytes() {
 
 // ---- digits ---------------------------------------------------------------------------------------------------------
 
+// Digits of a value of a float16 or float32 layer.
+__host__ __device__ constexpr int moe_digits(bool half) { return half ? 4 : 5; }
+
 // v * 2^n, by two factors so that every n that occurs (below 2 * 126 in size) can be formed.
 __device__ __forceinline__ float times_pow2(float v, int n) {
     const int a = n / 2;
@@ -138,15 +149,16 @@ __device__ __forceinline__ int row_shift(uint32_t most) {
     if (most == 0) return 0;
     const int exponent = most >= 0x00800000u ? static_cast<int>(most >> 23) - 127 : -118 - __clz(most);
     const int s = 8 * D - 2 - exponent;  // the largest in [2^(8 D - 2), 2^(8 D - 1))
-    const float limit = D == 3 ? 8355711.0f : 2139062016.0f;  // 127 (256^D - 1) / 255, rounded down to a float32
+    const float limit = D == 4 ? 2139062016.0f : 547599876096.0f;  // 127 (256^D - 1) / 255, rounded down to a float32
     return times_pow2(__uint_as_float(most), s) > limit ? s - 1 : s;
 }
 
 constexpr int NOT_FINITE = 0x7FFF;  // in place of the shift of a row that holds an infinity or NaN
 
+// What the sums over a row are to be shifted back by: they count units of the second lowest digit.
 template <int D>
 __device__ __forceinline__ int16_t shift_or_not(uint32_t most) {
-    return static_cast<int16_t>(most < 0x7F800000u ? row_shift<D>(most) : NOT_FINITE);
+    return static_cast<int16_t>(most < 0x7F800000u ? row_shift<D>(most) - 8 : NOT_FINITE);
 }
 
 // A digits' sum as the value it stands for.
@@ -163,7 +175,11 @@ __device__ __forceinline__ void put_digits(const float4& v, int shift, uint8_t* 
     uint32_t word[D] = {};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        int q = __float2int_rn(times_pow2(f[i], shift));
+        std::conditional_t<D == 5, long long, int> q;
+        if constexpr (D == 5)
+            q = __float2ll_rn(times_pow2(f[i], shift));
+        else
+            q = __float2int_rn(times_pow2(f[i], shift));
 #pragma unroll
         for (int d = 0; d < D; d++) {
             const int digit = static_cast<int8_t>(q);
@@ -297,7 +313,7 @@ __device__ __forceinline__ int moe_split(int total, int part, int parts) {
 // x as digits, row chunk by row chunk [D][128]. A warp finds its token's largest value and converts a part of four chunks.
 template <class S, bool HALF, bool VEC>
 __device__ __forceinline__ void moe_digits_x(const MoeFusedParams& p) {
-    constexpr int D = HALF ? 3 : 4;
+    constexpr int D = moe_digits(HALF);
     const MoeLaunch& L = p.L;
     const int lane = threadIdx.x & 31;
     const int parts = (p.chunks_in + 3) / 4;
@@ -849,16 +865,15 @@ struct MoeWarp {
     }
 
     // The digits' sums of one unit's chunks [c0, c1): rows g and g + 8 of matrix tile i, columns 2 q and 2 q + 1 of n-tile
-    // t in acc[i][t][digit]. The columns' digits start at values + row[t] (column g of the tile). `halves`: the box holds
+    // t in acc[i][t][digit - 1]. The columns' digits start at values + row[t] (column g of the tile). `halves`: the box holds
     // the gate's rows, then the other half's, and a tile 8 of each.
     __device__ __forceinline__ bool products(const uint8_t* values, const uint32_t (&row)[NT], int tiles, bool halves,
                                              const uint32_t (&skew)[MT][2], int c0, int count, int wrap,
-                                             int (&acc)[MT][NT][D][4]) {
-        // Where registers allow, the next chunk's digits are on their way while one is multiplied (64 tokens through 6 of
-        // 64 experts 172 -> 165 us); elsewhere tile 0's are asked for before the wait for the box and the other tiles' when
-        // their turn comes (with NT = 4 or at 16 warps the earlier loads only spill).
-        constexpr bool AHEAD = MT == 2 && NT * D <= 6;
-        constexpr int EARLY = AHEAD ? NT : 1;
+                                             int (&acc)[MT][NT][D - 1][4]) {
+        // Where registers allow, the next chunk's digits of tile 0 are on their way while one is multiplied (64 tokens through
+        // 6 of 64 experts 172 -> 165 us); elsewhere they are asked for before the wait for the box. The other tiles' are when
+        // their turn comes.
+        constexpr bool AHEAD = MT == 2 && NT * (D - 1) <= 12;
         const int q = lane & 3;
         // This lane's row of the parts of a step: part lane / 8 is rows 0-7 or 8-15 (odd) of the first or second (2, 3)
         // 16 bytes. A box's 16-byte units are swizzled by the row (its low three bits are lane % 8 in every part), so eight
@@ -871,16 +886,12 @@ struct MoeWarp {
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int d = 0; d < D; d++)
+                for (int d = 0; d < D - 1; d++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[m][t][d][i] = 0;
         const uint8_t* v = values + c0 * D * moe::CHUNK + q * 16;
-        uint4 next[EARLY][D][2];
-        if constexpr (AHEAD) {
-#pragma unroll
-            for (int t = 0; t < EARLY; t++)
-                if (t < tiles) load_digits(next[t], v + row[t]);
-        }
+        uint4 next[D][2];
+        if constexpr (AHEAD) load_digits(next, v + row[0]);
 #pragma unroll 1
         for (int c = c0; count > 0; count--) {
             const uint8_t* here = v;
@@ -891,21 +902,15 @@ struct MoeWarp {
                 v += D * moe::CHUNK;
             }
             const int slot = taken % moe::SLOTS;
-            uint4 b[EARLY][D][2];
+            uint4 b[D][2];
             if constexpr (AHEAD) {
 #pragma unroll
-                for (int t = 0; t < EARLY; t++)
+                for (int d = 0; d < D; d++)
 #pragma unroll
-                    for (int d = 0; d < D; d++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++) b[t][d][j] = next[t][d][j];
-                if (count > 1) {
-#pragma unroll
-                    for (int t = 0; t < EARLY; t++)
-                        if (t < tiles) load_digits(next[t], v + row[t]);
-                }
+                    for (int j = 0; j < 2; j++) b[d][j] = next[d][j];
+                if (count > 1) load_digits(next, v + row[0]);
             } else {
-                load_digits(b[0], here + row[0]);
+                load_digits(b, here + row[0]);
             }
             uint32_t a[MT][4][4];
             if constexpr (S::ALIGNED) {
@@ -939,19 +944,27 @@ struct MoeWarp {
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 if (t >= tiles) break;
-                uint4 (&bt)[D][2] = b[t % EARLY];
-                if (t >= EARLY) load_digits(bt, here + row[t]);
+                if (t > 0) load_digits(b, here + row[t]);
+                int low[MT][4] = {};
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
-#pragma unroll
-                        for (int d = 0; d < D; d++) moe_mma(acc[m][t][d], a[m][2 * j], bt[d][j].x, bt[d][j].y);
+                    for (int m = 0; m < MT; m++) moe_mma(low[m], a[m][2 * j], b[0][j].x, b[0][j].y);
 #pragma unroll
                     for (int m = 0; m < MT; m++)
 #pragma unroll
-                        for (int d = 0; d < D; d++) moe_mma(acc[m][t][d], a[m][2 * j + 1], bt[d][j].z, bt[d][j].w);
+                        for (int d = 1; d < D; d++) moe_mma(acc[m][t][d - 1], a[m][2 * j], b[d][j].x, b[d][j].y);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) moe_mma(low[m], a[m][2 * j + 1], b[0][j].z, b[0][j].w);
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int d = 1; d < D; d++) moe_mma(acc[m][t][d - 1], a[m][2 * j + 1], b[d][j].z, b[d][j].w);
                 }
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[m][t][0][i] += (low[m][i] + 128) >> 8;  // at most 2^21 in size before
                 // Every row part has been an operand, so the slot's reads are done: a box loaded over it any earlier could
                 // overtake reads that still wait in line behind the digits' loads.
                 if (t == 0) {
@@ -963,11 +976,11 @@ struct MoeWarp {
         return true;
     }
 
-    // The digits' sums as one exact sum.
-    __device__ __forceinline__ static long long whole(const int (&acc)[D][4], int i) {
-        long long sum = acc[D - 1][i];
+    // The digits' sums as one, exact in units of the second lowest digit.
+    __device__ __forceinline__ static long long whole(const int (&acc)[D - 1][4], int i) {
+        long long sum = acc[D - 2][i];
 #pragma unroll
-        for (int d = D - 2; d >= 0; d--) sum = sum * 256 + acc[d][i];
+        for (int d = D - 3; d >= 0; d--) sum = sum * 256 + acc[d][i];
         return sum;
     }
 
@@ -1104,7 +1117,7 @@ struct MoeWarp {
                     const int pair = sh.order[grp.first + min(8 * t + g, grp.count - 1)];
                     row[t] = static_cast<uint32_t>(phase == 0 ? pair / p.L.top_k : pair) * row_bytes;
                 }
-                int acc[MT][NT][D][4];
+                int acc[MT][NT][D - 1][4];
                 const bool halves = phase == 0 && p.L.gated;
                 uint32_t skew[MT][2] = {};
                 if constexpr (!S::ALIGNED) {
@@ -1201,7 +1214,7 @@ template <bool HALF, class S>
 __global__ void __launch_bounds__(S::THREADS, 1)
     moe_fused_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_out,
                      const __grid_constant__ MoeFusedParams p) {
-    constexpr int D = HALF ? 3 : 4;
+    constexpr int D = moe_digits(HALF);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     MoeShared<S>& sh = *reinterpret_cast<MoeShared<S>*>(smem + S::RING);
@@ -1365,7 +1378,7 @@ MoeFusedSizes moe_fused_sizes(const MoeLaunch& L) {
     const int64_t pairs = int64_t(L.tokens) * L.top_k;
     MoeFusedSizes s;
     s.logits = int64_t(L.tokens) * L.experts * 8;
-    const int digits = L.x_half ? 3 : 4;
+    const int digits = moe_digits(L.x_half);
     s.x_digits = int64_t(L.tokens) * chunks_of(L.model) * digits * moe::CHUNK;
     s.h_digits = pairs * chunks_of(L.expert) * digits * moe::CHUNK;
     s.x_most = int64_t(L.tokens) * 4;
