@@ -286,6 +286,10 @@ OG_API og_status og_int8_gemm_encode_activated(og_int8_gemm* gemm, og_encoder* e
                                                const og_operand* zero_point_b, const og_operand* float_bias,
                                                const og_operand* int_bias, int32_t activation,
                                                const og_operand* residual);
+/* Watchdog self-test: the next activated product that this instance records on the kernel for few rows ("tensor-core-slim")
+ * leaves a load out and waits limit_us (1 .. 500000) for it. The launch ends by itself; the next og_device_wait_idle or
+ * readback reports OG_ERROR_COMMAND_FAILED (reason Watchdog), c is not defined, and the instance stays usable. */
+OG_API og_status og_int8_gemm_activated_watchdog_selftest(og_int8_gemm* gemm, uint32_t limit_us);
 /* Its argument checks alone (no device needed): EncodeFloat's order and names, then "activation" and "residual". */
 OG_API og_status og_int8_gemm_check_activated(const og_int8_gemm_problem* problem, const og_buffer* a,
                                               const og_buffer* b, const og_buffer* c, const og_operand* a_scale,

@@ -130,6 +130,7 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int og_int8_gemm_check_dequantize(OgProblem* p, OgBuffer* a,
         OgBuffer* b, OgBuffer* c, OgOperand* aScale, OgOperand* bScale, OgOperand* zpA, OgOperand* zpB,
         OgOperand* floatBias, OgOperand* intBias);
+    [LibraryImport(Lib)] internal static partial int og_int8_gemm_activated_watchdog_selftest(nint gemm, uint limitUs);
     [LibraryImport(Lib)] internal static partial int og_int8_gemm_check_activated(OgProblem* p, OgBuffer* a,
         OgBuffer* b, OgBuffer* c, OgOperand* aScale, OgOperand* bScale, OgOperand* zpA, OgOperand* zpB,
         OgOperand* floatBias, OgOperand* intBias, int activation, OgOperand* residual);

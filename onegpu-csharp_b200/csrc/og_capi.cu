@@ -200,6 +200,7 @@ struct og_int8_gemm {
     int stream_k = 0;  // 0: whole tiles + the split tail of int32 products; 1: whole tiles only; 2: stream-K
     std::string variant;
     std::string last = "none";
+    uint64_t self_test_ns = 0;  // watchdog self-test of the next activated product of few rows, 0 for none
     // Device buffers freed with the instance: byte sums and staged operands, older ones too (recorded work may name them)
     std::vector<void*> scratch;
     int32_t* sums = nullptr;  // the latest byte-sum buffer, scratch_elements int32
@@ -664,8 +665,9 @@ void record_gemm(og_int8_gemm* g, og_encoder* enc, og::GemmLaunch L, const og_op
     const int slim = g->tile == 0 && g->stream_k != 2 ? og::slim_parts(L) : 0;
     if (slim > 0) {
         cudaError_t err;
-        og::LaunchFn fn = og::prepare_gemm_slim(L, slim, &err);  // tensor maps built now, at record time
+        og::LaunchFn fn = og::prepare_gemm_slim(L, slim, g->self_test_ns, &err);  // tensor maps built now, at record time
         check_cuda(err, "Int8Gemm tensor maps");
+        g->self_test_ns = 0;
         g->last = staged ? "tensor-core-slim-staged" : "tensor-core-slim";
         enc->ops.push_back(std::move(fn));
         enc->dispatches += 1;
@@ -1352,6 +1354,16 @@ OG_API og_status og_int8_gemm_encode_dequantize(og_int8_gemm* g, og_encoder* enc
         L.epi.scale_a = reinterpret_cast<const float*>(operand_ptr(a_scale));
         L.epi.float_bias = reinterpret_cast<const float*>(operand_ptr(fbias));
         record_gemm(g, enc, L, nullptr);
+    });
+}
+
+OG_API og_status og_int8_gemm_activated_watchdog_selftest(og_int8_gemm* g, uint32_t limit_us) {
+    return guard([&] {
+        live_gemm(g);
+        if (limit_us < 1 || limit_us > 500000)
+            throw OgError{OG_ERROR_ARGUMENT_RANGE, kGemm, "limitMicroseconds",
+                          "the self-test wait limit is 1 .. 500000 microseconds", "", "", ""};
+        g->self_test_ns = uint64_t(limit_us) * 1000;
     });
 }
 

@@ -97,9 +97,10 @@ int64_t rows_tickets(const GemmLaunch& L);
 cudaError_t launch_gemm_rows(const GemmLaunch& L, cudaStream_t stream);
 
 // Activated product of few rows (og_gemm_slim.cu): K split over a cluster of slim_parts CTAs per column tile; 0 when the
-// kernel for whole tiles serves better. Needs no byte sums and no scratch.
+// kernel for whole tiles serves better. Needs no byte sums and no scratch. self_test_ns other than 0: a launch whose first CTA
+// leaves a load out and whose waits end after that time.
 int slim_parts(const GemmLaunch& L);
-LaunchFn prepare_gemm_slim(const GemmLaunch& L, int parts, cudaError_t* err);
+LaunchFn prepare_gemm_slim(const GemmLaunch& L, int parts, uint64_t self_test_ns, cudaError_t* err);
 
 // A 3-D byte tensor map (x innermost) with 128-byte swizzled box_x x box_y x box_z boxes (og_gemm_tc.cu).
 bool make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t x, uint64_t y, uint64_t z, uint64_t stride_y,

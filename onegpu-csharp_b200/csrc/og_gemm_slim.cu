@@ -54,6 +54,8 @@ struct SlimParams {
     int a_batched, b_batched;
     Epilogue epi;
     int* error_flag;
+    uint64_t wait_limit_ns;
+    int withhold;  // watchdog self-test: the first CTA leaves its last load out
 };
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
@@ -143,10 +145,12 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
         if (e.float_bias != nullptr) fbias = __ldg(e.float_bias + n);
     }
 
+    int issued = 0;  // by warp 0
     if (warp == 0) {
-        for (int kb = kb0; kb < kb1; kb++) {
+        const int last = p.withhold && blockIdx.x == 0 && part == 0 ? kb1 - 1 : kb1;
+        for (int kb = kb0; kb < last; kb++) {
             const int it = kb - kb0, s = it % C::STAGES;
-            const bool ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag);
+            const bool ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, p.wait_limit_ns);
             if (!__all_sync(0xFFFFFFFFu, ok)) break;  // a warp gives up as one
             if (lane == 0) {
                 mbar_arrive_expect_tx(&full[s], C::B_BYTES + C::A_BYTES);
@@ -156,13 +160,14 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
                     tma_load_3d(sB + s * C::B_BYTES, &tmap_b, &full[s], tile * slim::BN, kb * slim::BK, bb);
                 tma_load_3d(sX + s * C::A_BYTES, &tmap_a, &full[s], kb * slim::BK, row0, ba);
             }
+            issued++;
             __syncwarp();
         }
     } else if (warp == 1) {
         bool ok = true;
         for (int kb = kb0; kb < kb1; kb++) {
             const int it = kb - kb0, s = it % C::STAGES;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag, p.wait_limit_ns));
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
             int32_t sum = 0;
             for (int kb = kb0; kb < kb1; kb++) {
                 const int it = kb - kb0, s = it % C::STAGES;
-                const bool ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag);
+                const bool ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag, p.wait_limit_ns);
                 if (!__all_sync(0xFFFFFFFFu, ok)) break;
                 const uint4* box = reinterpret_cast<const uint4*>(sX + s * C::A_BYTES + r * slim::BK);
 #pragma unroll
@@ -213,7 +218,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
             for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
             if (t % LANES == 0) row_sum[r] = sum;
         }
-        if (t == 0) *ready = mbar_wait(tfull, 0, abort_flag) ? 1 : 0;
+        if (t == 0) *ready = mbar_wait(tfull, 0, abort_flag, p.wait_limit_ns) ? 1 : 0;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (*ready) {
             tc_fence_after();
@@ -246,6 +251,12 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
     }
     __syncwarp();
     cluster_sync_all();  // every CTA's partial sums are in its shared memory
+    if (warp == 0 && lane == 0 && *abort_flag) {
+        // A CTA that gave up waits (bounded) for its loads: none may land after it has gone.
+        int give_up = 0;
+        for (int it = max(0, issued - C::STAGES); it < issued; it++)
+            mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, &give_up);
+    }
 
     if (warp >= 2) {
         const int t = threadIdx.x - 64;
@@ -440,7 +451,7 @@ static LaunchFn bind_slim_m(const GemmLaunch& L, const SlimParams& p, const CUte
                : bind_slim_t<MR, false, OUT_ACT_F32>(p, ma, mb, grid, idesc, ones);
 }
 
-LaunchFn prepare_gemm_slim(const GemmLaunch& L, int parts, cudaError_t* err) {
+LaunchFn prepare_gemm_slim(const GemmLaunch& L, int parts, uint64_t self_test_ns, cudaError_t* err) {
     *err = cudaErrorInvalidValue;
     const int mr = slim_rows(L.m);
     const int ba = (L.batch > 1 && L.stride_a != 0) ? L.batch : 1;
@@ -465,6 +476,8 @@ LaunchFn prepare_gemm_slim(const GemmLaunch& L, int parts, cudaError_t* err) {
     p.b_batched = bb > 1;
     p.epi = L.epi;
     p.error_flag = L.error_flag;
+    p.wait_limit_ns = self_test_ns != 0 ? self_test_ns : OG_WAIT_LIMIT_NS;
+    p.withhold = self_test_ns != 0;
     const dim3 grid(static_cast<unsigned>(p.tiles * p.row_chunks * L.batch), static_cast<unsigned>(parts));
     switch (mr) {
         case 16: return bind_slim_m<16>(L, p, ma, mb, grid);

@@ -139,6 +139,7 @@ EXPORTS = {
     "og_int8_gemm_check_dequantize": [_PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD, _OPD, _OPD, _OPD],
     "og_int8_gemm_encode_activated": [_P, _P, _PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD, _OPD, _OPD, _OPD,
                                       ctypes.c_int32, _OPD],
+    "og_int8_gemm_activated_watchdog_selftest": [_P, ctypes.c_uint32],
     "og_int8_gemm_check_activated": [_PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD, _OPD, _OPD, _OPD, ctypes.c_int32, _OPD],
     "og_int8_gemm_int32_noalloc": [_P, _PROB, _BUF, _BUF, _BUF, _OPD, _OPD, _OPD],
     "og_int8_gemm_noalloc_status": [_P],
@@ -738,6 +739,11 @@ class Int8Gemm:
                                                   _buf(a), _buf(b), _buf(c), _opd(a_scale), _opd(b_scale),
                                                   _opd(zero_point_a), _opd(zero_point_b), _opd(float_bias),
                                                   _opd(int_bias), int(activation), _opd(residual)))
+
+    def activated_watchdog_selftest(self, limit_us: int) -> None:
+        """The next activated product recorded on the kernel for few rows leaves a load out and waits ``limit_us`` for it: the
+        next wait_idle raises GpuCommandFailedException with reason "Watchdog" and the instance stays usable."""
+        _check(_lib.og_int8_gemm_activated_watchdog_selftest(self.handle, limit_us))
 
     # The reference's member names.
     EncodeInt32 = encode_int32
