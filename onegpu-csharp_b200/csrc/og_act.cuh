@@ -9,7 +9,8 @@
 // Errors relative to the result, negative tails included: silu 2^-21, gelu 26 x 2^-24, gelu_tanh (5 + 9 |u|) 2^-23, whose
 // exponential's argument 2 u is itself a rounded one. Quotients are the fast ones (2 units in the last place for divisors
 // of this size), exponentials expf's; for tanh GELU the fast one (2 + 1.173 |2 u| units), which adds less than the argument's
-// rounding does: with expf 8192 x 8192 x 2048 into float32 took 199 us, so 186.
+// rounding does: with expf 8192 x 8192 x 2048 into float32 took 199 us, so 187, and the results' distance from 64 bits is
+// 6.0e-8 with either.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -26,7 +26,7 @@
 // largest value for float16 layers (D = 4) and 39 bits for float32 ones (D = 5): the step has to be small next to the quiet
 // channels of a row, not to its largest value, since an output's weights may leave the loud ones out. With a digit less (23
 // and 31 bits) such outputs were off by up to 15 roundings of float16 for channels 3000 to 60000 times the others; 64 tokens
-// through 6 of 64 experts (2048 x 1408) took 152 us then and 156 now, one token (2048 x 1024) 35.5 and 36.5.
+// through 6 of 64 experts (2048 x 1408) took 152 us then and 156 with one more, one token (2048 x 1024) 35.5 and 36.5.
 // Measured against converting the weights to bfloat16 in registers and multiplying two or three bfloat16 pieces, with three
 // digits: 239 instructions per 2 KB of weights became about 100, 8 tokens through 2 of 8 experts (4096 x 8192) went from
 // 163 to 149 us (6.1 TB/s while the weights stream), 64 tokens through 6 of 64 experts from 199 to 164 us. The tensor
@@ -725,6 +725,14 @@ __device__ __forceinline__ int moe_owner(int i, int total) {
     return static_cast<int>((static_cast<int64_t>(i + 1) * S::WARPS - 1) / total);
 }
 
+// Out of line for the same reason as grid_barrier: eight copies of five activations took 162 us (64 tokens through 6 of 64
+// experts) where this takes 154.
+static __device__ __noinline__ float moe_activate(float v, int kind) {
+    float f[1] = {v};
+    activate_all(f, kind);
+    return f[0];
+}
+
 // What the warp's ring loads next: phase 1's work, then phase 2's.
 struct MoeFeed {
     int phase;
@@ -1021,11 +1029,10 @@ struct MoeWarp {
                     float h[2] = {shifted_back(sum[m][t][i], shift) * scale[m].x,
                                   shifted_back(sum[m][t][2 + i], shift) * scale[m].y};
                     if (L.gated) {
-                        float f[1] = {h[0]};
-                        activate_all(f, L.activation);
-                        h[0] = f[0] * h[1];
+                        h[0] = moe_activate(h[0], L.activation) * h[1];
                     } else {
-                        activate_all(h, L.activation);
+                        h[0] = moe_activate(h[0], L.activation);
+                        h[1] = moe_activate(h[1], L.activation);
                         if (n < grp.count && j0 + 8 < L.expert) {
                             hidden[j0 + 8] = h[1];
                             most = max(most, __float_as_uint(h[1]) & 0x7FFFFFFFu);
