@@ -55,10 +55,11 @@ constexpr int GROUP_M_TALL = 16;
 // K block instead of 48 KB.
 //
 // Epilogue warps: two per TMEM lane quadrant, each taking half of the tile's columns, or four for the activated form (ACT),
-// each a quarter: its work per element (28 instructions, two of them exponentials or quotients at a quarter of the
-// rate) fits beside the MMAs of the next tile only with four warps to hide one another's latency on each scheduler. Their
-// boxes and the second set of column terms, filled while the accumulator is awaited, cost one stage of the operand ring.
-// 8192 x 8192 x 2048 into float32 with tanh GELU took 167 us with 8 warps and six stages, 134 us with 16 and five.
+// each a quarter: its work per element (32 instructions for tanh GELU into float32, two of them exponentials or quotients at
+// a quarter of the rate, 38 with zero points) fits beside the MMAs of the next tile only with four warps to hide one
+// another's latency on each scheduler. Their boxes and the second set of column terms, filled while the accumulator is
+// awaited, cost one stage of the operand ring. 8192 x 8192 x 2048 into float32 with tanh GELU and no zero points took 167 us
+// with 8 warps and six stages, 134 us with 16 and five (137 now; 187 with zero points).
 template <int CG, bool ACT = false>
 struct Cfg {
     static constexpr int EPI_WARPS = ACT ? 16 : 8;
