@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
             const int s = kb % rows::STAGES;
             const uint32_t ph = (kb / rows::STAGES) & 1;
             const int kc = (kb_begin + kb) * rows::BK;
-            if (!mbar_wait(&empty[s], ph ^ 1, abort_flag)) goto done;
+            if (!mbar_wait_warp(&empty[s], ph ^ 1, abort_flag)) goto done;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&full[s], rows::B_BYTES + (sums_only ? 0 : rows::A_BYTES));
                 if constexpr (B_KMAJOR)
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
         for (int kb = 0; kb < kb_count; kb++) {
             const int s = kb % rows::STAGES;
             const uint32_t ph = (kb / rows::STAGES) & 1;
-            if (!mbar_wait(&full[s], ph, abort_flag)) goto done;
+            if (!mbar_wait_warp(&full[s], ph, abort_flag)) goto done;
             tc_fence_after();
             if (lane == 0) {
                 const uint32_t b_addr = smem_u32(sB + s * rows::B_BYTES);
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
             if (part == 0) row_sum[r] = sum;
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps
-        if (!mbar_wait(tfull, 0, abort_flag)) goto done;
+        if (!mbar_wait_warp(tfull, 0, abort_flag)) goto done;
         tc_fence_after();
         uint32_t r[32];
         tmem_ld_sum(tmem_base + (static_cast<uint32_t>(q * 32) << 16), kb_count, r);
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
             const int kc = static_cast<int>(u - static_cast<int64_t>(t) * kbt) * rows::BK;
             const int tile = t % p.tiles, b = t / p.tiles;
             const int ba = p.a_batched ? b : 0, bb = p.b_batched ? b : 0;
-            if (!mbar_wait(&empty[st], ph ^ 1, abort_flag)) break;
+            if (!mbar_wait_warp(&empty[st], ph ^ 1, abort_flag)) break;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&full[st], rows::B_BYTES + rows::A_BYTES);
                 if constexpr (B_KMAJOR)
@@ -388,8 +388,8 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
             const bool first = u == u0 || kb == 0;
             const bool last = u == u1 - 1 || kb == kbt - 1;
             const int acc = seg & 1;
-            if (first && !mbar_wait(&tempty[acc], ((seg >> 1) & 1) ^ 1, abort_flag)) break;
-            if (!mbar_wait(&full[st], ph, abort_flag)) break;
+            if (first && !mbar_wait_warp(&tempty[acc], ((seg >> 1) & 1) ^ 1, abort_flag)) break;
+            if (!mbar_wait_warp(&full[st], ph, abort_flag)) break;
             tc_fence_after();
             if (lane == 0) {
                 const uint32_t b_addr = smem_u32(sB + st * rows::B_BYTES);
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
             const int s = kb % rows::SUMS_STAGES;
             const uint32_t ph = (kb / rows::SUMS_STAGES) & 1;
             const int kc = (kb_begin + kb) * rows::BK;
-            if (!mbar_wait(&empty[s], ph ^ 1, abort_flag)) goto done;
+            if (!mbar_wait_warp(&empty[s], ph ^ 1, abort_flag)) goto done;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&full[s], rows::B_BYTES);
                 if (job.kmajor)
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
         for (int kb = 0; kb < kb_count; kb++) {
             const int s = kb % rows::SUMS_STAGES;
             const uint32_t ph = (kb / rows::SUMS_STAGES) & 1;
-            if (!mbar_wait(&full[s], ph, abort_flag)) goto done;
+            if (!mbar_wait_warp(&full[s], ph, abort_flag)) goto done;
             tc_fence_after();
             if (lane == 0) {
                 const uint32_t t_addr = smem_u32(sB + s * rows::B_BYTES);
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
         __syncwarp();
     } else {
         const int q = warp & 3;
-        if (!mbar_wait(tfull, 0, abort_flag)) goto done;
+        if (!mbar_wait_warp(tfull, 0, abort_flag)) goto done;
         tc_fence_after();
         // Accumulator kk (one per K = 32 step of a block) holds its sum in all 16 of its columns kk*16 .. +15.
         uint32_t r[32], t[32];

@@ -150,8 +150,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
         const int last = p.withhold && blockIdx.x == 0 && part == 0 ? kb1 - 1 : kb1;
         for (int kb = kb0; kb < last; kb++) {
             const int it = kb - kb0, s = it % C::STAGES;
-            const bool ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, p.wait_limit_ns);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;  // a warp gives up as one
+            if (!mbar_wait_warp(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, p.wait_limit_ns)) break;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&full[s], C::B_BYTES + C::A_BYTES);
                 if constexpr (B_KMAJOR)
@@ -167,7 +166,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
         bool ok = true;
         for (int kb = kb0; kb < kb1; kb++) {
             const int it = kb - kb0, s = it % C::STAGES;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag, p.wait_limit_ns));
+            ok = mbar_wait_warp(&full[s], (it / C::STAGES) & 1, abort_flag, p.wait_limit_ns);
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
@@ -205,8 +204,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
             int32_t sum = 0;
             for (int kb = kb0; kb < kb1; kb++) {
                 const int it = kb - kb0, s = it % C::STAGES;
-                const bool ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag, p.wait_limit_ns);
-                if (!__all_sync(0xFFFFFFFFu, ok)) break;
+                if (!mbar_wait_warp(&full[s], (it / C::STAGES) & 1, abort_flag, p.wait_limit_ns)) break;
                 const uint4* box = reinterpret_cast<const uint4*>(sX + s * C::A_BYTES + r * slim::BK);
 #pragma unroll
                 for (int i = 0; i < UNITS; i++) sum = byte_sum(box[(u0 + i) ^ (r & 7)], e.za_signed, sum);
@@ -251,12 +249,7 @@ __global__ void __launch_bounds__(slim::THREADS, 2)
     }
     __syncwarp();
     cluster_sync_all();  // every CTA's partial sums are in its shared memory
-    if (warp == 0 && lane == 0 && *abort_flag) {
-        // A CTA that gave up waits (bounded) for its loads: none may land after it has gone.
-        int give_up = 0;
-        for (int it = max(0, issued - C::STAGES); it < issued; it++)
-            mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, &give_up);
-    }
+    if (warp == 0 && lane == 0 && *abort_flag) drain_ring(full, C::STAGES, issued);
 
     if (warp >= 2) {
         const int t = threadIdx.x - 64;

@@ -675,9 +675,10 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
     tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
 
-    if (warp == 0) {
-        // TMA producer: the whole warp walks the ring, lane 0 issues.
-        uint32_t it = 0;
+    uint32_t it = 0;  // the ring's steps: loads issued, of warp 0; of warp 1, stages multiplied
+    if (warp == 0 && lane == 0) {
+        // TMA producer. One lane walks the ring: in a warp that walked it together, a lane that gave up a wait alone would
+        // leave the others at their next __syncwarp for good.
         WorkCursor cur;
         work_begin<SPLIT>(p, worker, workers, cur);
         WorkItem wi;
@@ -697,35 +698,33 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                 const int s = it % C::STAGES;
                 const uint32_t ph = (it / C::STAGES) & 1;
                 if (!mbar_wait(&empty[s], ph ^ 1, abort_flag)) goto done;
-                if (lane == 0) {
-                    if constexpr (CG == 2) {
-                        const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-                        if (leader) mbar_arrive_expect_tx(&full[s], bytes);
-                        tma_load_3d_pair(sA + s * C::A_BYTES, &tmap_a, bar, kb * tc::BK, row0, ba);
-                        if constexpr (B_MN)
-                            tma_load_3d_pair(sB + s * C::B_BYTES, &tmap_b, bar, col0, kb * tc::BK, bb);
-                        else
-                            tma_load_3d_pair(sB + s * C::B_BYTES, &tmap_b, bar, kb * tc::BK, col0, bb);
+                if constexpr (CG == 2) {
+                    const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+                    if (leader) mbar_arrive_expect_tx(&full[s], bytes);
+                    tma_load_3d_pair(sA + s * C::A_BYTES, &tmap_a, bar, kb * tc::BK, row0, ba);
+                    if constexpr (B_MN)
+                        tma_load_3d_pair(sB + s * C::B_BYTES, &tmap_b, bar, col0, kb * tc::BK, bb);
+                    else
+                        tma_load_3d_pair(sB + s * C::B_BYTES, &tmap_b, bar, kb * tc::BK, col0, bb);
+                } else {
+                    mbar_arrive_expect_tx(&full[s], bytes);
+                    tma_load_3d(sA + s * C::A_BYTES, &tmap_a, &full[s], kb * tc::BK, row0, ba);
+                    if constexpr (B_MN) {
+                        tma_load_3d(sB + s * C::B_BYTES, &tmap_b, &full[s], col0, kb * tc::BK, bb);
+                        if (second_half)
+                            tma_load_3d(sB + s * C::B_BYTES + C::B_BOX, &tmap_b, &full[s], col0 + 128,
+                                        kb * tc::BK, bb);
                     } else {
-                        mbar_arrive_expect_tx(&full[s], bytes);
-                        tma_load_3d(sA + s * C::A_BYTES, &tmap_a, &full[s], kb * tc::BK, row0, ba);
-                        if constexpr (B_MN) {
-                            tma_load_3d(sB + s * C::B_BYTES, &tmap_b, &full[s], col0, kb * tc::BK, bb);
-                            if (second_half)
-                                tma_load_3d(sB + s * C::B_BYTES + C::B_BOX, &tmap_b, &full[s], col0 + 128,
-                                            kb * tc::BK, bb);
-                        } else {
-                            tma_load_3d(sB + s * C::B_BYTES, &tmap_b, &full[s], kb * tc::BK, col0, bb);
-                        }
+                        tma_load_3d(sB + s * C::B_BYTES, &tmap_b, &full[s], kb * tc::BK, col0, bb);
                     }
                 }
-                __syncwarp();
             }
         }
+    } else if (warp == 0) {
+        // The other lanes wait at the end.
     } else if (warp == 1) {
-        // MMA issuer (the leader CTA of a pair issues for both): four K = 32 MMAs per stage.
-        if (leader) {
-            uint32_t it = 0;
+        // MMA issuer (one lane; the leader CTA of a pair issues for both): four K = 32 MMAs per stage.
+        if (lane == 0 && leader) {
             WorkCursor cur;
             work_begin<SPLIT>(p, worker, workers, cur);
             WorkItem wi;
@@ -740,34 +739,28 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                     const uint32_t ph = (it / C::STAGES) & 1;
                     if (!mbar_wait(&full[s], ph, abort_flag)) goto done;
                     tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t a_addr = smem_u32(sA + s * C::A_BYTES);
-                        const uint32_t b_addr = smem_u32(sB + s * C::B_BYTES);
+                    const uint32_t a_addr = smem_u32(sA + s * C::A_BYTES);
+                    const uint32_t b_addr = smem_u32(sB + s * C::B_BYTES);
 #pragma unroll
-                        for (int kk = 0; kk < tc::BK / 32; kk++) {
-                            const uint64_t adesc = smem_desc_sw128(a_addr + kk * 32, 16, 1024);
-                            const uint64_t bdesc = B_MN ? smem_desc_sw128(b_addr + kk * 32 * 128, C::B_BOX, 1024)
-                                                        : smem_desc_sw128(b_addr + kk * 32, 16, 1024);
-                            const uint32_t accum = (kb != wi.kb0 || kk != 0) ? 1u : 0u;
-                            if constexpr (CG == 2)
-                                mma_i8_pair(d_tmem, adesc, bdesc, idesc, accum);
-                            else
-                                mma_i8(d_tmem, adesc, bdesc, idesc, accum);
-                        }
+                    for (int kk = 0; kk < tc::BK / 32; kk++) {
+                        const uint64_t adesc = smem_desc_sw128(a_addr + kk * 32, 16, 1024);
+                        const uint64_t bdesc = B_MN ? smem_desc_sw128(b_addr + kk * 32 * 128, C::B_BOX, 1024)
+                                                    : smem_desc_sw128(b_addr + kk * 32, 16, 1024);
+                        const uint32_t accum = (kb != wi.kb0 || kk != 0) ? 1u : 0u;
                         if constexpr (CG == 2)
-                            mma_commit_pair(&empty[s], 0x3);
+                            mma_i8_pair(d_tmem, adesc, bdesc, idesc, accum);
                         else
-                            mma_commit(&empty[s]);
+                            mma_i8(d_tmem, adesc, bdesc, idesc, accum);
                     }
-                    __syncwarp();
-                }
-                if (lane == 0) {
                     if constexpr (CG == 2)
-                        mma_commit_pair(&tfull[acc], 0x3);
+                        mma_commit_pair(&empty[s], 0x3);
                     else
-                        mma_commit(&tfull[acc]);
+                        mma_commit(&empty[s]);
                 }
-                __syncwarp();
+                if constexpr (CG == 2)
+                    mma_commit_pair(&tfull[acc], 0x3);
+                else
+                    mma_commit(&tfull[acc]);
             }
         }
     } else {

@@ -65,6 +65,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
+// The same by a whole warp, which gives up as one: a lane that left alone would keep the others waiting for it.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                               uint64_t limit_ns = OG_WAIT_LIMIT_NS) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort, limit_ns));
+}
+
+// One thread of a CTA that gave up waits (bounded) for the loads it has issued into a ring of `stages` slots, `issued` in
+// all: none may land in shared memory after the CTA has gone.
+__device__ __forceinline__ void drain_ring(uint64_t* full, int stages, int issued) {
+    int give_up = 0;
+    for (int it = issued > stages ? issued - stages : 0; it < issued; it++)
+        mbar_wait(&full[it % stages], (it / stages) & 1, &give_up);
+}
+
 // n / d for 0 <= n < 2^31 by multiplication (Granlund and Montgomery, "Division by Invariant Integers using
 // Multiplication", 1994): magic and shift from magic_for(d).
 __device__ __forceinline__ int32_t div_magic(int32_t n, uint32_t magic, int32_t shift) {
