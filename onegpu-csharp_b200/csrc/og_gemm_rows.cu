@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
     const int ba = p.a_batched ? b : 0;
     const int bb = p.b_batched ? b : 0;
 
+    int issued = 0;  // by warp 0
     if (warp == 0) {
         for (int kb = 0; kb < kb_count; kb++) {
             const int s = kb % rows::STAGES;
@@ -173,6 +174,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
                     tma_load_3d(sB + s * rows::B_BYTES, &tmap_b, &full[s], tile * rows::BN, kc, bb);
                 if (!sums_only) tma_load_3d(sX + s * rows::A_BYTES, &tmap_a, &full[s], kc, 0, ba);
             }
+            issued++;
             __syncwarp();
         }
     } else if (warp == 1) {
@@ -278,6 +280,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
 
 done:
     __syncthreads();
+    if (warp == 0 && lane == 0 && *abort_flag) drain_ring(full, rows::STAGES, issued);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, rows::TMEM_COLS);
@@ -358,6 +361,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
 
+    int issued = 0;  // by warp 0
     if (warp == 0) {
         for (int64_t u = u0; u < u1; u++) {
             const int it = static_cast<int>(u - u0);
@@ -376,6 +380,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
                     tma_load_3d(sB + st * rows::B_BYTES, &tmap_b, &full[st], tile * rows::BN, kc, bb);
                 tma_load_3d(sX + st * rows::A_BYTES, &tmap_a, &full[st], kc, 0, ba);
             }
+            issued++;
             __syncwarp();
         }
     } else if (warp == 1) {
@@ -552,6 +557,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
     }
 
     __syncthreads();
+    if (warp == 0 && lane == 0 && *abort_flag) drain_ring(full, rows::STAGES, issued);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 2 * rows::TMEM_COLS);
@@ -633,6 +639,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
     const uint32_t tmem_base = *tmem_holder;
     const int bz = job.batched ? b : 0;
 
+    int issued = 0;  // by warp 0
     if (warp == 0) {
         for (int kb = 0; kb < kb_count; kb++) {
             const int s = kb % rows::SUMS_STAGES;
@@ -646,6 +653,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
                 else
                     tma_load_3d(sB + s * rows::B_BYTES, tmap, &full[s], tile * rows::BN, kc, bz);
             }
+            issued++;
             __syncwarp();
         }
     } else if (warp == 1) {
@@ -688,6 +696,7 @@ __global__ void __launch_bounds__(rows::THREADS, 2)
 
 done:
     __syncthreads();
+    if (warp == 0 && lane == 0 && *abort_flag) drain_ring(full, rows::SUMS_STAGES, issued);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, rows::TMEM_COLS);

@@ -1042,6 +1042,8 @@ done:
     // The stores have read their boxes before shared memory goes (their global writes complete with the grid).
     if (tma_store && warp >= 2 && lane == 0) bulk_wait_group_read<0>();
     __syncthreads();
+    // The leader's barriers count the pair's loads.
+    if (warp == 0 && lane == 0 && leader && *abort_flag) drain_ring(full, C::STAGES, static_cast<int>(it));
     if constexpr (CG == 2) cluster_sync_all();  // neither CTA frees the pair's TMEM while the other still reads it
     if (warp == 1) {
         tc_fence_after();
