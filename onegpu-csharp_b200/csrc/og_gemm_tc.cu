@@ -856,6 +856,8 @@ __device__ __forceinline__ void gemm_tc_body(const CUtensorMap& tmap_a, const CU
                         mbar_arrive_expect_tx(sk_bar, SK_SLOT_BYTES);
                         bulk_load(sA, p.sk_part + static_cast<int64_t>(sk_slot) * SK_SLOT_INTS, SK_SLOT_BYTES, sk_bar);
                         ok = mbar_wait(sk_bar, 0, abort_flag);
+                        int give_up = 0;
+                        if (!ok) mbar_wait(sk_bar, 0, &give_up);  // the copy, too, lands before the CTA goes
                     }
                 }
                 epi_go[lt & 1] = ok ? 1 : 0;
